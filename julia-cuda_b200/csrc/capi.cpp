@@ -13,6 +13,7 @@
 #include <vector>
 
 #include "../../include/julia_cuda.h"
+#include "capi_guard.h"
 #include "checkpoint.h"
 #include "engine.h"
 #include "jc_internal.h"
@@ -22,31 +23,10 @@ struct JcEngine {
     jc::Engine *e;
 };
 
+using jc::guarded;
+using jc::report;
+
 namespace {
-
-void report(char *err, size_t len, const std::string &msg) {
-    jc::set_error(msg);
-    if (!err || len == 0) return;
-    const size_t n = std::min(msg.size(), len - 1);
-    std::memcpy(err, msg.data(), n);
-    err[n] = 0;
-}
-
-template <typename F>
-auto guarded(char *err, size_t len, F &&f) -> decltype(f()) {
-    try {
-        return f();
-    } catch (const std::exception &ex) {
-        report(err, len, std::string("julia-cuda: exception: ") + ex.what());
-    } catch (...) {
-        report(err, len, "julia-cuda: unknown exception");
-    }
-    // Failure: -1 for the int-returning entry points, NULL for the pointer-returning ones.
-    if constexpr (std::is_same_v<decltype(f()), int>)
-        return -1;
-    else
-        return decltype(f())();
-}
 
 bool set_device(int dev, char *err, size_t len) {
     cudaError_t e = cudaSetDevice(dev);

@@ -1,6 +1,7 @@
 // Internal declarations shared by the kernels (.cu) and the host runtime (.cpp).
 #pragma once
 #include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
@@ -35,6 +36,9 @@ bool cuda_ok(cudaError_t e, const char *what);
 
 // ---------------------------------------------------------------------------------------------
 // TMA descriptors
+
+// The CUDA driver's cuTensorMapEncodeTiled, or nullptr.
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn();
 
 // A row-major [rows, cols] f16 GEMM operand (cols a multiple of 64) seen as 3-D: (column inside a
 // 64-wide k-block, row, k-block), loaded in boxes of 64 x box_rows x GEMM_KPS with the 128-byte
@@ -165,6 +169,9 @@ bool enqueue_device_error_read(unsigned int *pinned, cudaStream_t s, unsigned in
 // Clears an error word (synchronous).
 bool clear_device_error(unsigned int *word);
 const char *device_error_name(unsigned int code);
+// The module's error word on the current device (nullptr, with the error set, on failure): what a
+// kernel outside kernels.cu is given to record into.
+unsigned int *module_error_word();
 
 // ---------------------------------------------------------------------------------------------
 // persistent kernel (persist.cuh): a phase list run by one cooperative launch

@@ -1,6 +1,7 @@
-// The library's only CUDA translation unit: every kernel template is instantiated here, next to
-// its host launcher (argument checks, launch shape, PDL attribute). Keeping one unit lets all
-// kernels share the device error word without relocatable device code.
+// The CUDA translation unit of the inference path: every kernel template of it is instantiated
+// here, next to its host launcher (argument checks, launch shape, PDL attribute). Keeping one unit
+// lets these kernels share the device error word without relocatable device code; kernels of other
+// units are given its address (module_error_word).
 #include <cudaTypedefs.h>
 
 #include <atomic>
@@ -15,6 +16,7 @@
 #include "gemm_pair.cuh"
 #include "gemm_persist.cuh"
 #include "jc_internal.h"
+#include "launch.h"
 #include "persist.cuh"
 
 namespace jc {
@@ -57,6 +59,18 @@ bool clear_device_error(unsigned int *word) {
     return cuda_ok(cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(zero)), "clear error word");
 }
 
+unsigned int *module_error_word() {
+    static std::atomic<unsigned int *> words[64];
+    int dev = 0;
+    if (!cuda_ok(cudaGetDevice(&dev), "cudaGetDevice")) return nullptr;
+    unsigned int *w = words[dev & 63].load();
+    if (w) return w;
+    void *p = nullptr;
+    if (!cuda_ok(cudaGetSymbolAddress(&p, g_dev_error), "error word")) return nullptr;
+    words[dev & 63].store(static_cast<unsigned int *>(p));
+    return static_cast<unsigned int *>(p);
+}
+
 const char *device_error_name(unsigned int code) {
     switch (code) {
         case 0: return "none";
@@ -71,87 +85,9 @@ const char *device_error_name(unsigned int code) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// launch helper: cudaLaunchKernelEx with programmatic stream serialization when `pdl`
-
-static uint32_t env_u32_early(const char *name, uint32_t dflt) {
-    const char *e = getenv(name);
-    return e ? (uint32_t)strtoul(e, nullptr, 10) : dflt;
-}
-
-// Programmatic dependent launch is on unless the environment sets JC_PDL=0 (for A/B timing).
-static bool pdl_allowed() {
-    static const bool on = [] {
-        const char *v = getenv("JC_PDL");
-        return !(v && v[0] == '0');
-    }();
-    return on;
-}
-
-template <typename... KArgs, typename... Args>
-static bool launch_ex(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
-                      bool pdl, const char *what, Args... args) {
-    pdl = pdl && pdl_allowed();
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = pdl ? attr : nullptr;
-    cfg.numAttrs = pdl ? 1 : 0;
-    return cuda_ok(cudaLaunchKernelEx(&cfg, kern, args...), what);
-}
-
-// launch_ex with the grid grouped into thread-block clusters of `cluster_z` CTAs along z (1: none).
-template <typename... KArgs, typename... Args>
-static bool launch_ex_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
-                              cudaStream_t s, bool pdl, int cluster_z, const char *what,
-                              Args... args) {
-    pdl = pdl && pdl_allowed();
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    unsigned n = 0;
-    if (pdl) {
-        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[n].val.programmaticStreamSerializationAllowed = 1;
-        n++;
-    }
-    if (cluster_z > 1) {
-        attr[n].id = cudaLaunchAttributeClusterDimension;
-        attr[n].val.clusterDim.x = 1;
-        attr[n].val.clusterDim.y = 1;
-        attr[n].val.clusterDim.z = (unsigned)cluster_z;
-        n++;
-    }
-    cfg.attrs = n ? attr : nullptr;
-    cfg.numAttrs = n;
-    return cuda_ok(cudaLaunchKernelEx(&cfg, kern, args...), what);
-}
-
-// Sets a kernel's dynamic shared-memory limit once per device.
-template <typename K>
-static bool ensure_smem(K kern, int bytes, std::atomic<uint64_t> &done_mask) {
-    int dev = 0;
-    if (!cuda_ok(cudaGetDevice(&dev), "cudaGetDevice")) return false;
-    const uint64_t bit = 1ull << (dev & 63);
-    if (done_mask.load() & bit) return true;
-    if (!cuda_ok(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
-                 "cudaFuncSetAttribute"))
-        return false;
-    done_mask.fetch_or(bit);
-    return true;
-}
-
-// ---------------------------------------------------------------------------------------------
 // TMA descriptors
 
-static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = []() {
         void *p = nullptr;
         cudaDriverEntryPointQueryResult q;
