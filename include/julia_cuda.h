@@ -389,6 +389,90 @@ const char *jc_last_error(void);
  * timeouts in. Engines keep their own (julia_cuda_device_error). */
 int jc_device_error(uint32_t *code);
 
+/* ============================ fine-tuning operators (device) ============================ */
+/* What training a head over the encoder needs: layer norm, linear layers, the loss over a request's
+ * choices and the optimizer's step, with their gradients. No counterpart in the reference (it only
+ * infers). Return 0, or -1 with jc_last_error(). Everything is queued on `stream`; nothing waits.
+ * Results do not depend on timing: sums are taken in a fixed order. Empty inputs (0 rows) are legal.
+ * `ld...` is the distance between rows in elements (at least the row's width); rows are contiguous.
+ * Any alignment of whole elements is legal; rows that start on 16-byte boundaries are faster. */
+
+/* Element types. */
+#define JC_F16 0u
+#define JC_BF16 1u
+#define JC_F32 2u
+
+/* y = (x - mean) rstd gamma + beta for each of `rows` rows of d elements (d up to 16384; x, y of
+ * `type`, gamma and beta [d] f32, beta may be NULL), rstd = 1 / sqrt(variance + eps). stats (may be
+ * NULL) receives [rows][2] f32: mean and rstd, which the backward pass reads. y may be x. */
+int jc_layer_norm(uint32_t type, const void *x, size_t ldx, const float *gamma, const float *beta,
+                  float eps, uint32_t rows, uint32_t d, void *y, size_t ldy, float *stats,
+                  void *stream);
+/* The gradients of jc_layer_norm: with xh = (x - mean) rstd and u = dy gamma,
+ * dx = rstd (u - mean(u) - xh mean(u xh)) [+ add, the gradient that reaches x past the norm],
+ * dgamma = sum over rows of dy xh, dbeta = sum over rows of dy (f32 [d], each may be NULL). dx may
+ * be dy or add. ws: jc_layer_norm_ws_floats(rows, d) floats of scratch (unused if neither dgamma
+ * nor dbeta is wanted). */
+int jc_layer_norm_backward(uint32_t type, const void *dy, size_t lddy, const void *x, size_t ldx,
+                           const float *gamma, const float *stats, const void *add, size_t ldadd,
+                           uint32_t rows, uint32_t d, void *dx, size_t lddx, float *dgamma,
+                           float *dbeta, float *ws, void *stream);
+size_t jc_layer_norm_ws_floats(uint32_t rows, uint32_t d);
+
+/* z = x w^T + bias, y = act(z) + res: x [m][k], w [n][k], y, z, res [m][n] of `type` (JC_F16 or
+ * JC_BF16), bias [n] f32; bias, res and z may be NULL. act: 0, JC_EPI_RELU or JC_EPI_GELU. z, when
+ * given, keeps the values before the activation, which the backward pass reads. Unlike jc_gemm, any
+ * m, n and k, both 16-bit types, strided rows. y may be res. */
+int jc_linear(uint32_t type, uint32_t act, const void *x, size_t ldx, const void *w, size_t ldw,
+              const float *bias, const void *res, size_t ldres, void *y, size_t ldy, void *z,
+              size_t ldz, uint32_t m, uint32_t n, uint32_t k, void *stream);
+/* The gradients of jc_linear: dz = dy act'(z), dx = dz w [m][k], dw = dz^T x [n][k], dbias = sum over
+ * rows of dz ([n] f32); each of dx, dw and dbias may be NULL. (res's gradient is dy itself.) z is
+ * read when act is not 0. dz is rounded to `type` before the products, as every tensor-core
+ * operand is; dbias sums it unrounded. With f16 a gradient below 6e-8 becomes 0: scale the loss.
+ * ws: jc_linear_ws_bytes(act, m, n, k) bytes of scratch, 256-byte aligned. */
+int jc_linear_backward(uint32_t type, uint32_t act, const void *dy, size_t lddy, const void *x,
+                       size_t ldx, const void *w, size_t ldw, const void *z, size_t ldz, uint32_t m,
+                       uint32_t n, uint32_t k, void *dx, size_t lddx, void *dw, size_t lddw,
+                       float *dbias, void *ws, void *stream);
+size_t jc_linear_ws_bytes(uint32_t act, uint32_t m, uint32_t n, uint32_t k);
+
+/* The loss of requests that each pick one of their markers: request r's logits are
+ * [offsets[r], offsets[r + 1]) of `logits` (n_logits in all; offsets int32 [requests + 1]) and its
+ * right marker gold[r], counted from its first (below 0: none). loss[r] = weight[r] (log(sum
+ * exp(logit)) - logit of the right marker), dlogits (may be NULL) its gradient, weight[r]
+ * (softmax - one-hot); weight NULL: 1. A request with no right marker, weight 0, no logits or only
+ * logits of -infinity gives 0 and 0. Offsets or a right marker out of range record device error 6
+ * (JC_DEV_BAD_INDEX, read by jc_device_error), give loss 0 and leave the request's dlogits alone. */
+int jc_choice_loss(const float *logits, uint32_t n_logits, const int32_t *offsets,
+                   const int32_t *gold, const float *weight, uint32_t requests, float *loss,
+                   float *dlogits, void *stream);
+
+/* AdamW over many tensors, one launch a step. */
+typedef struct JcAdamW JcAdamW;
+typedef struct jc_adamw_tensor {
+    float *p;             /* n parameters, f32 */
+    const void *g;        /* their gradients, of grad_type */
+    void *m, *v;          /* first and second moments: f32, or e4m3 bytes with 8-bit states */
+    float *m_scale, *v_scale; /* 8-bit states: one f32 for each 256 elements (the last may be short) */
+    void *copy;           /* if not NULL, the updated parameters in copy_type (JC_F16 or JC_BF16) */
+    uint64_t n;
+    float weight_decay;
+    uint32_t grad_type, copy_type;
+} jc_adamw_tensor;
+/* Keeps a device table of `count` tensors on the current device for later steps (bits: 32 or 8, the
+ * states' width); the tensors stay the caller's and must outlive it. m and v start at zero (8-bit:
+ * codes and scales zero). Waits for the table's copy. NULL on failure (jc_last_error()). */
+JcAdamW *jc_adamw_create(const jc_adamw_tensor *tensors, size_t count, uint32_t bits);
+/* Step t (from 1): g' = g grad_scale, m = beta1 m + (1 - beta1) g', v = beta2 v + (1 - beta2) g'^2,
+ * p = p (1 - lr weight_decay) - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps), all in
+ * f32. grad_scale: one f32 in device memory (NULL: 1), so a clipping factor need not visit the host.
+ * 8-bit states are read, updated in f32, and rounded to the nearest e4m3 under their 256 elements'
+ * new scale (largest magnitude / 448); a v above 0 stays above 0. */
+int jc_adamw_step(JcAdamW *opt, uint64_t t, float lr, double beta1, double beta2, float eps,
+                  const float *grad_scale, void *stream);
+void jc_adamw_free(JcAdamW *opt);
+
 /* ============================== host weight preparation ============================== */
 /* src/prep.rs. f16 outputs are bit patterns. */
 

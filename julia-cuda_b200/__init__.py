@@ -141,6 +141,18 @@ def lib():
         "jc_embed": ([P, u32, P, P, u32, f32, P, P, P], i32),
         "jc_norm_add": ([P, u32, u32, P, P, f32, P, P, P], i32),
         "jc_score": ([P, u32, P, f32, P, u32, P, P], i32),
+        "jc_layer_norm": ([u32, P, sz, P, P, f32, u32, u32, P, sz, P, P], i32),
+        "jc_layer_norm_backward": ([u32, P, sz, P, sz, P, P, P, sz, u32, u32, P, sz, P, P, P, P],
+                                   i32),
+        "jc_layer_norm_ws_floats": ([u32, u32], sz),
+        "jc_linear": ([u32, u32, P, sz, P, sz, P, P, sz, P, sz, P, sz, u32, u32, u32, P], i32),
+        "jc_linear_backward": ([u32, u32, P, sz, P, sz, P, sz, P, sz, u32, u32, u32, P, sz, P, sz, P,
+                                P, P], i32),
+        "jc_linear_ws_bytes": ([u32, u32, u32, u32], sz),
+        "jc_choice_loss": ([P, u32, P, P, P, u32, P, P, P], i32),
+        "jc_adamw_create": ([P, sz, u32], P),
+        "jc_adamw_step": ([P, u64, f32, ctypes.c_double, ctypes.c_double, f32, P, P], i32),
+        "jc_adamw_free": ([P], None),
         "jc_last_error": ([], ch),
         "jc_device_error": ([P], i32),
         "jc_prep_fold_layernorm": ([P, P, u32, u32, P, P], None),
@@ -612,3 +624,17 @@ class Engine:
         if rc != 0:
             raise JuliaCudaError(err.value.decode(errors="replace"))
         return code.value
+
+
+# ------------------------------------------------------------------------------------------------
+# fine-tuning operators (training.py; it needs torch, which the engine's host calls do not)
+
+_TRAINING = ("layer_norm", "layer_norm_backward", "linear", "linear_backward", "choice_loss", "AdamW")
+
+
+def __getattr__(name):
+    if name in _TRAINING:
+        from . import training
+        globals().update({n: getattr(training, n) for n in _TRAINING})
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

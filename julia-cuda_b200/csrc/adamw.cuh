@@ -1,0 +1,166 @@
+// One AdamW step over many tensors in one launch.
+//
+//   g' = g grad_scale
+//   m = beta1 m + (1 - beta1) g'        v = beta2 v + (1 - beta2) g'^2
+//   p = p (1 - lr decay) - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps)
+//
+// p, and m and v with 32-bit states, are f32. With 8-bit states m and v are e4m3 codes with one f32
+// scale for each 256 consecutive elements (the largest magnitude / 448), taken up and written back
+// each step around the same f32 arithmetic; a v above 0 never rounds to 0, so no step divides by
+// eps alone. v itself is held, not its root: nearest rounding then follows the 32-bit average with
+// no bias (its root within 0.85..1.25 of it for 90% of elements at beta2 0.999, 256 elements of
+// log-normal scale sharing a block; a root in e4m3: 0.78..1.34).
+#pragma once
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+#include "elem.cuh"
+#include "train.h"
+
+namespace jc {
+
+struct AdamwParams {
+    const AdamwTensor *tensors;
+    const uint2 *chunks;  // (tensor, chunk of it)
+    const float *grad_scale;
+    float beta1, beta2, one_minus_beta1, one_minus_beta2, lr, eps;
+    float inv_bias1, inv_bias2;  // 1 / (1 - beta^t)
+};
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// Eight consecutive values at p[0..n) (n up to 8; `vec`: 16-byte aligned and all eight there).
+template <class T>
+__device__ __forceinline__ void load8(const T *p, uint32_t n, bool vec, float *v) {
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < 8; i += VEC<T>) Elem<T, VEC<T>>::load(p + i, v + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = i < (int)n ? static_cast<float>(p[i]) : 0.0f;
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void store8(T *p, uint32_t n, bool vec, const float *v) {
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < 8; i += VEC<T>) Elem<T, VEC<T>>::store(p + i, v + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i < (int)n) p[i] = static_cast<T>(v[i]);
+    }
+}
+
+// Eight e4m3 codes as f32 times `scale`, and back.
+__device__ __forceinline__ void load_codes(const uint8_t *p, uint32_t n, bool vec, float scale, float *v) {
+    uint2 q = make_uint2(0, 0);
+    if (vec) {
+        q = *reinterpret_cast<const uint2 *>(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i < (int)n) (i < 4 ? q.x : q.y) |= (uint32_t)p[i] << (8 * (i & 3));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t w = (i < 2 ? q.x : q.y) >> (16 * (i & 1));
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xFFFF), __NV_E4M3);
+        const float2 f = __half22float2(__half2(h));
+        v[2 * i] = f.x * scale;
+        v[2 * i + 1] = f.y * scale;
+    }
+}
+
+__device__ __forceinline__ void store_codes(uint8_t *p, uint32_t n, bool vec, const float *v) {
+    uint32_t q[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t c = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+        q[i >> 1] |= c << (16 * (i & 1));
+    }
+    if (vec) {
+        *reinterpret_cast<uint2 *>(p) = make_uint2(q[0], q[1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i < (int)n) p[i] = (uint8_t)(q[i >> 2] >> (8 * (i & 3)));
+    }
+}
+
+constexpr float FP8_MAX = 448.0f, FP8_MIN = 0.001953125f;  // e4m3: largest, smallest above 0
+
+// One chunk a block, eight consecutive elements a thread: a warp holds the 256 elements that share
+// an 8-bit state's scale.
+template <int BITS>
+__global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const AdamwParams p) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const uint2 ch = p.chunks[blockIdx.x];
+    const AdamwTensor &t = p.tensors[ch.x];
+    const uint64_t at = (uint64_t)ch.y * ADAMW_CHUNK + threadIdx.x * 8;
+    if ((at & ~uint64_t(255)) >= t.n) return;  // the whole warp is past the end
+    const uint32_t n = at >= t.n ? 0 : (uint32_t)min((uint64_t)8, t.n - at);
+    const bool vec = t.aligned && n == 8;
+    const float gs = p.grad_scale ? *p.grad_scale : 1.0f;
+    float g[8], m[8], v[8], w[8];
+    if (t.grad_type == JC_F32)
+        load8(static_cast<const float *>(t.g) + at, n, vec, g);
+    else if (t.grad_type == JC_F16)
+        load8(static_cast<const __half *>(t.g) + at, n, vec, g);
+    else
+        load8(static_cast<const __nv_bfloat16 *>(t.g) + at, n, vec, g);
+    load8(t.p + at, n, vec, w);
+    if constexpr (BITS == 8) {
+        load_codes(static_cast<const uint8_t *>(t.m) + at, n, vec, t.m_scale[at / ADAMW_BLOCK], m);
+        load_codes(static_cast<const uint8_t *>(t.v) + at, n, vec, t.v_scale[at / ADAMW_BLOCK], v);
+    } else {
+        load8(static_cast<const float *>(t.m) + at, n, vec, m);
+        load8(static_cast<const float *>(t.v) + at, n, vec, v);
+    }
+    const float keep = 1.0f - p.lr * t.decay;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float gi = g[i] * gs;
+        m[i] = p.beta1 * m[i] + p.one_minus_beta1 * gi;
+        v[i] = p.beta2 * v[i] + p.one_minus_beta2 * gi * gi;
+        w[i] = w[i] * keep - p.lr * (m[i] * p.inv_bias1) / (sqrtf(v[i] * p.inv_bias2) + p.eps);
+    }
+    store8(t.p + at, n, vec, w);
+    if (t.copy_type == JC_F16)
+        store8(static_cast<__half *>(t.copy) + at, n, vec, w);
+    else if (t.copy_type == JC_BF16)
+        store8(static_cast<__nv_bfloat16 *>(t.copy) + at, n, vec, w);
+    if constexpr (BITS == 8) {
+        float mm = 0.0f, vm = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            mm = fmaxf(mm, fabsf(m[i]));
+            vm = fmaxf(vm, v[i]);
+        }
+        mm = warp_max(mm) / FP8_MAX;
+        vm = warp_max(vm) / FP8_MAX;
+        const float im = mm > 0.0f ? 1.0f / mm : 1.0f, iv = vm > 0.0f ? 1.0f / vm : 1.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            m[i] *= im;
+            v[i] = v[i] > 0.0f ? fmaxf(v[i] * iv, FP8_MIN) : v[i];
+        }
+        store_codes(static_cast<uint8_t *>(t.m) + at, n, vec, m);
+        store_codes(static_cast<uint8_t *>(t.v) + at, n, vec, v);
+        if ((threadIdx.x & 31) == 0) {
+            t.m_scale[at / ADAMW_BLOCK] = mm;
+            t.v_scale[at / ADAMW_BLOCK] = vm;
+        }
+    } else {
+        store8(static_cast<float *>(t.m) + at, n, vec, m);
+        store8(static_cast<float *>(t.v) + at, n, vec, v);
+    }
+}
+
+}  // namespace jc

@@ -1,0 +1,252 @@
+"""The fine-tuning operators on torch device tensors: layer norm, linear layers, the loss over a
+request's choices and the AdamW step, with their gradients (include/julia_cuda.h, "fine-tuning
+operators"). As with the inference kernels, outputs are the caller's tensors and everything is
+queued on the current stream (or `stream`). Also available from the package itself.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import EPI_GELU, EPI_RELU, JuliaCudaError, _check, _stream, last_error, lib
+
+F16, BF16, F32 = 0, 1, 2
+_TYPES = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}
+_ACTS = {"none": 0, "relu": EPI_RELU, "gelu": EPI_GELU}
+
+
+def _fail(what: str):
+    raise JuliaCudaError(what)
+
+
+def _matrix(op: str, name: str, t, rows: int, cols: int, dtype):
+    """(pointer, row stride) of a [rows, cols] device tensor with contiguous rows; (None, 0) of
+    None."""
+    if t is None:
+        return None, 0
+    if t.dtype is not dtype or tuple(t.shape) != (rows, cols) or not t.is_cuda:
+        _fail(f"{op}: {name} must be a [{rows}, {cols}] device tensor of {dtype}, "
+              f"not {list(t.shape)} of {t.dtype}")
+    sr, sc = t.stride()
+    if (cols > 1 and sc != 1) or (rows > 1 and sr < cols):
+        _fail(f"{op}: {name} must have contiguous rows that do not overlap")
+    return t.data_ptr(), sr if rows > 1 else cols
+
+
+def _vector(op: str, name: str, t, n: int, dtype=torch.float32):
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.numel() != n or not t.is_cuda or not t.is_contiguous():
+        _fail(f"{op}: {name} must be a contiguous device tensor of {n} elements of {dtype}")
+    return t.data_ptr()
+
+
+def _type(op: str, t, halves: bool = False) -> int:
+    code = _TYPES.get(t.dtype)
+    if code is None or t.dim() != 2 or (halves and code == F32):
+        _fail(f"{op}: x must be a matrix of float16{', ' if not halves else ' or '}bfloat16"
+              f"{'' if halves else ' or float32'}")
+    if t.device.index != torch.cuda.current_device():
+        _fail(f"{op}: the tensors are not on the current device")
+    return code
+
+
+def _scratch(n: int, dtype, like, stream):
+    """Scratch of the allocator's own, which must not reuse it before `stream` is done with it."""
+    ws = torch.empty(max(n, 1), dtype=dtype, device=like.device)
+    if stream is not None:
+        ws.record_stream(stream if isinstance(stream, torch.cuda.Stream)
+                         else torch.cuda.ExternalStream(stream))
+    return ws
+
+
+def layer_norm(x, gamma, beta, y, stats=None, eps: float = 1e-5, stream=None) -> None:
+    """y = (x - mean) rstd gamma + beta per row (jc_layer_norm). x, y [rows, d] of one type (f16, bf16
+    or f32), gamma and beta [d] f32 (beta may be None); stats, if given, [rows, 2] f32 receives mean
+    and rstd for the backward pass."""
+    t = _type("layer_norm", x)
+    rows, d = x.shape
+    xp, ldx = _matrix("layer_norm", "x", x, rows, d, x.dtype)
+    yp, ldy = _matrix("layer_norm", "y", y, rows, d, x.dtype)
+    _check(lib().jc_layer_norm(t, xp, ldx, _vector("layer_norm", "gamma", gamma, d),
+                               _vector("layer_norm", "beta", beta, d), eps, rows, d, yp, ldy,
+                               _vector("layer_norm", "stats", stats, 2 * rows), _stream(stream)),
+           "jc_layer_norm")
+
+
+def layer_norm_backward(dy, x, gamma, stats, dx, dgamma=None, dbeta=None, add=None, ws=None,
+                        stream=None) -> None:
+    """The gradients of layer_norm (jc_layer_norm_backward): dx (plus `add`, the gradient that
+    reaches x past the norm), dgamma and dbeta [d] f32. ws: jc_layer_norm_ws_floats(rows, d) floats
+    (allocated here when not given)."""
+    op = "layer_norm_backward"
+    t = _type(op, x)
+    rows, d = x.shape
+    xp, ldx = _matrix(op, "x", x, rows, d, x.dtype)
+    dyp, lddy = _matrix(op, "dy", dy, rows, d, x.dtype)
+    dxp, lddx = _matrix(op, "dx", dx, rows, d, x.dtype)
+    ap, ldadd = _matrix(op, "add", add, rows, d, x.dtype)
+    need = lib().jc_layer_norm_ws_floats(rows, d) if dgamma is not None or dbeta is not None else 0
+    if ws is None:
+        ws = _scratch(need, torch.float32, x, stream)
+    elif ws.numel() < need:
+        _fail(f"{op}: ws needs {need} floats")
+    _check(lib().jc_layer_norm_backward(t, dyp, lddy, xp, ldx, _vector(op, "gamma", gamma, d),
+                                        _vector(op, "stats", stats, 2 * rows), ap, ldadd, rows, d,
+                                        dxp, lddx, _vector(op, "dgamma", dgamma, d),
+                                        _vector(op, "dbeta", dbeta, d), ws.data_ptr(),
+                                        _stream(stream)), "jc_layer_norm_backward")
+
+
+def _act(op: str, act: str) -> int:
+    code = _ACTS.get(act)
+    if code is None:
+        _fail(f"{op}: act must be one of {', '.join(_ACTS)}")
+    return code
+
+
+def linear(x, w, y, *, bias=None, act: str = "none", res=None, z=None, stream=None) -> None:
+    """y = act(x w^T + bias) + res (jc_linear): x [m, k], w [n, k], y, res [m, n] of one 16-bit type,
+    bias [n] f32. z, if given, keeps the values before the activation for the backward pass."""
+    t = _type("linear", x, halves=True)
+    m, k = x.shape
+    n = w.shape[0]
+    xp, ldx = _matrix("linear", "x", x, m, k, x.dtype)
+    wp, ldw = _matrix("linear", "w", w, n, k, x.dtype)
+    rp, ldres = _matrix("linear", "res", res, m, n, x.dtype)
+    yp, ldy = _matrix("linear", "y", y, m, n, x.dtype)
+    zp, ldz = _matrix("linear", "z", z, m, n, x.dtype)
+    _check(lib().jc_linear(t, _act("linear", act), xp, ldx, wp, ldw,
+                           _vector("linear", "bias", bias, n), rp, ldres, yp, ldy, zp, ldz, m, n, k,
+                           _stream(stream)), "jc_linear")
+
+
+def linear_backward(dy, x, w, *, z=None, act: str = "none", dx=None, dw=None, dbias=None, ws=None,
+                    stream=None) -> None:
+    """The gradients of linear (jc_linear_backward), each written if its tensor is given: dx [m, k],
+    dw [n, k] of x's type, dbias [n] f32. z (linear's) is read unless act is "none". ws:
+    jc_linear_ws_bytes(act, m, n, k) bytes (allocated here when not given)."""
+    op = "linear_backward"
+    t = _type(op, x, halves=True)
+    m, k = x.shape
+    n = w.shape[0]
+    a = _act(op, act)
+    xp, ldx = _matrix(op, "x", x, m, k, x.dtype)
+    wp, ldw = _matrix(op, "w", w, n, k, x.dtype)
+    dyp, lddy = _matrix(op, "dy", dy, m, n, x.dtype)
+    zp, ldz = _matrix(op, "z", z, m, n, x.dtype)
+    dxp, lddx = _matrix(op, "dx", dx, m, k, x.dtype)
+    dwp, lddw = _matrix(op, "dw", dw, n, k, x.dtype)
+    need = lib().jc_linear_ws_bytes(a, m, n, k)
+    if ws is None:
+        ws = _scratch(need, torch.uint8, x, stream)
+    elif ws.numel() * ws.element_size() < need:
+        _fail(f"{op}: ws needs {need} bytes")
+    _check(lib().jc_linear_backward(t, a, dyp, lddy, xp, ldx, wp, ldw, zp, ldz, m, n, k, dxp, lddx,
+                                    dwp, lddw, _vector(op, "dbias", dbias, n), ws.data_ptr(),
+                                    _stream(stream)), "jc_linear_backward")
+
+
+def choice_loss(logits, offsets, gold, loss, dlogits=None, weight=None, stream=None) -> None:
+    """Each request's loss over its own markers and its gradient (jc_choice_loss): logits f32,
+    offsets int32 [requests + 1], gold int32 [requests] (the right marker of each request, below 0:
+    none), weight f32 [requests]; writes loss [requests] and dlogits (as logits)."""
+    op = "choice_loss"
+    n, r = logits.numel(), gold.numel()
+    if logits.is_cuda and logits.device.index != torch.cuda.current_device():
+        _fail(f"{op}: the tensors are not on the current device")
+    _check(lib().jc_choice_loss(_vector(op, "logits", logits, n), n,
+                                _vector(op, "offsets", offsets, r + 1, torch.int32),
+                                _vector(op, "gold", gold, r, torch.int32),
+                                _vector(op, "weight", weight, r), r, _vector(op, "loss", loss, r),
+                                _vector(op, "dlogits", dlogits, n), _stream(stream)),
+           "jc_choice_loss")
+
+
+class AdamwTensor(ctypes.Structure):
+    """jc_adamw_tensor."""
+
+    _fields_ = [("p", ctypes.c_void_p), ("g", ctypes.c_void_p), ("m", ctypes.c_void_p),
+                ("v", ctypes.c_void_p), ("m_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("copy", ctypes.c_void_p), ("n", ctypes.c_uint64), ("weight_decay", ctypes.c_float),
+                ("grad_type", ctypes.c_uint32), ("copy_type", ctypes.c_uint32)]
+
+
+class AdamW:
+    """AdamW over many tensors, one launch a step (jc_adamw_create / jc_adamw_step).
+
+    params: contiguous f32 device tensors; grads: a tensor of as many elements for each (f16, bf16 or
+    f32), whose storage every step reads, so gradients are written in place; copies: optional f16 or
+    bf16 tensors (or None) that receive the updated parameters. weight_decay: one number, or one for
+    each tensor. bits: 32 or 8, the width of the states exp_avg and exp_avg_sq (f32, or float8_e4m3fn
+    with a scale for each 256 elements in exp_avg_scale and exp_avg_sq_scale), made here as zeros
+    unless given."""
+
+    BLOCK = 256
+
+    def __init__(self, params, grads, *, bits: int = 32, weight_decay=0.0, copies=None, exp_avg=None,
+                 exp_avg_sq=None, exp_avg_scale=None, exp_avg_sq_scale=None):
+        self._h = None
+        n = len(params)
+        if bits not in (8, 32):
+            _fail("AdamW: states of 32 or 8 bits")
+        state = torch.float32 if bits == 32 else torch.float8_e4m3fn
+        blocks = [-(-p.numel() // self.BLOCK) for p in params]
+        new = lambda dt, sizes: [torch.zeros(k, dtype=dt, device=p.device)  # noqa: E731
+                                 for p, k in zip(params, sizes)]
+        sizes = [p.numel() for p in params]
+        self.params, self.grads, self.bits = list(params), list(grads), bits
+        self.copies = list(copies) if copies is not None else [None] * n
+        self.exp_avg = list(exp_avg) if exp_avg is not None else new(state, sizes)
+        self.exp_avg_sq = list(exp_avg_sq) if exp_avg_sq is not None else new(state, sizes)
+        scaled = bits == 8
+        self.exp_avg_scale = (list(exp_avg_scale) if exp_avg_scale is not None
+                              else new(torch.float32, blocks) if scaled else [None] * n)
+        self.exp_avg_sq_scale = (list(exp_avg_sq_scale) if exp_avg_sq_scale is not None
+                                 else new(torch.float32, blocks) if scaled else [None] * n)
+        decay = list(weight_decay) if hasattr(weight_decay, "__len__") else [weight_decay] * n
+        if any(len(x) != n for x in (self.grads, self.copies, self.exp_avg, self.exp_avg_sq, decay,
+                                     self.exp_avg_scale, self.exp_avg_sq_scale)):
+            _fail("AdamW: as many gradients, states, copies and decays as parameters")
+        table = (AdamwTensor * max(n, 1))()
+        for i, p in enumerate(self.params):
+            k, g, c, at = p.numel(), self.grads[i], self.copies[i], f"of tensor {i}"
+            if p.device.index != torch.cuda.current_device():
+                _fail("AdamW: the tensors are not on the current device")
+            if g.dtype not in _TYPES:
+                _fail(f"AdamW: the gradient {at} must be float16, bfloat16 or float32")
+            if c is not None and c.dtype not in (torch.float16, torch.bfloat16):
+                _fail(f"AdamW: the copy {at} must be float16 or bfloat16")
+            sc = blocks[i] if scaled else 0
+            table[i] = AdamwTensor(
+                _vector("AdamW", f"the parameter {at}", p, k),
+                _vector("AdamW", f"the gradient {at}", g, k, g.dtype),
+                _vector("AdamW", f"exp_avg {at}", self.exp_avg[i], k, state),
+                _vector("AdamW", f"exp_avg_sq {at}", self.exp_avg_sq[i], k, state),
+                _vector("AdamW", f"exp_avg_scale {at}", self.exp_avg_scale[i], sc),
+                _vector("AdamW", f"exp_avg_sq_scale {at}", self.exp_avg_sq_scale[i], sc),
+                None if c is None else _vector("AdamW", f"the copy {at}", c, k, c.dtype), k,
+                float(decay[i]), _TYPES[g.dtype], F32 if c is None else _TYPES[c.dtype])
+        # The table's copy waits for nothing: zeros made above are queued before any step.
+        self._h = lib().jc_adamw_create(table, n, bits)
+        if not self._h:
+            raise JuliaCudaError(last_error())
+
+    def step(self, t: int, *, lr: float, betas=(0.9, 0.999), eps: float = 1e-8, grad_scale=None,
+             stream=None) -> None:
+        """Step t (from 1). grad_scale: one f32 on the device that every gradient is multiplied by."""
+        _check(lib().jc_adamw_step(self._h, t, lr, betas[0], betas[1], eps,
+                                   _vector("AdamW", "grad_scale", grad_scale, 1), _stream(stream)),
+               "jc_adamw_step")
+
+    def close(self) -> None:
+        if self._h:
+            lib().jc_adamw_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
