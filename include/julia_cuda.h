@@ -430,12 +430,12 @@ int jc_linear(uint32_t type, uint32_t act, const void *x, size_t ldx, const void
  * rows of dz ([n] f32); each of dx, dw and dbias may be NULL. (res's gradient is dy itself.) z is
  * read when act is not 0. dz is rounded to `type` before the products, as every tensor-core
  * operand is; dbias sums it unrounded. With f16 a gradient below 6e-8 becomes 0: scale the loss.
- * ws: jc_linear_ws_bytes(act, m, n, k) bytes of scratch, 256-byte aligned. */
+ * ws: jc_linear_ws_bytes(m, n, k) bytes of scratch, 256-byte aligned. */
 int jc_linear_backward(uint32_t type, uint32_t act, const void *dy, size_t lddy, const void *x,
                        size_t ldx, const void *w, size_t ldw, const void *z, size_t ldz, uint32_t m,
                        uint32_t n, uint32_t k, void *dx, size_t lddx, void *dw, size_t lddw,
                        float *dbias, void *ws, void *stream);
-size_t jc_linear_ws_bytes(uint32_t act, uint32_t m, uint32_t n, uint32_t k);
+size_t jc_linear_ws_bytes(uint32_t m, uint32_t n, uint32_t k);
 
 /* The loss of requests that each pick one of their markers: request r's logits are
  * [offsets[r], offsets[r + 1]) of `logits` (n_logits in all; offsets int32 [requests + 1]) and its

@@ -95,6 +95,15 @@ __device__ __forceinline__ void store_codes(uint8_t *p, uint32_t n, bool vec, co
 
 constexpr float FP8_MAX = 448.0f, FP8_MIN = 0.001953125f;  // e4m3: largest, smallest above 0
 
+// x / s, given inv = 1 / s rounded to nearest: the product's remainder, exact in one fused
+// multiply-add, corrects it (Markstein, "Computation of elementary functions on the IBM RISC
+// System/6000 processor", 1990). The correctly rounded quotient wherever that remainder does not
+// underflow, at a fifth of a division's instructions; below that a code is 0 either way.
+__device__ __forceinline__ float div_by(float x, float s, float inv) {
+    const float q = __fmul_rn(x, inv);
+    return __fmaf_rn(__fmaf_rn(-q, s, x), inv, q);
+}
+
 // One chunk a block, eight consecutive elements a thread: a warp holds the 256 elements that share
 // an 8-bit state's scale.
 template <int BITS>
@@ -126,9 +135,11 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const AdamwParams 
     const float keep = 1.0f - p.lr * t.decay;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const float gi = g[i] * gs;
-        m[i] = p.beta1 * m[i] + p.one_minus_beta1 * gi;
-        v[i] = p.beta2 * v[i] + p.one_minus_beta2 * gi * gi;
+        // Each operation of the states rounded by itself, so that an 8-bit code does not depend on
+        // how a compiler contracts them.
+        const float gi = __fmul_rn(g[i], gs);
+        m[i] = __fadd_rn(__fmul_rn(p.beta1, m[i]), __fmul_rn(p.one_minus_beta1, gi));
+        v[i] = __fadd_rn(__fmul_rn(p.beta2, v[i]), __fmul_rn(__fmul_rn(p.one_minus_beta2, gi), gi));
         w[i] = w[i] * keep - p.lr * (m[i] * p.inv_bias1) / (sqrtf(v[i] * p.inv_bias2) + p.eps);
     }
     store8(t.p + at, n, vec, w);
@@ -143,13 +154,15 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const AdamwParams 
             mm = fmaxf(mm, fabsf(m[i]));
             vm = fmaxf(vm, v[i]);
         }
-        mm = warp_max(mm) / FP8_MAX;
-        vm = warp_max(vm) / FP8_MAX;
-        const float im = mm > 0.0f ? 1.0f / mm : 1.0f, iv = vm > 0.0f ? 1.0f / vm : 1.0f;
+        mm = __fmul_rn(warp_max(mm), 1.0f / FP8_MAX);
+        vm = __fmul_rn(warp_max(vm), 1.0f / FP8_MAX);
+        const float sm = mm > 0.0f ? mm : 1.0f, sv = vm > 0.0f ? vm : 1.0f;
+        const float im = __frcp_rn(sm), iv = __frcp_rn(sv);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            m[i] *= im;
-            v[i] = v[i] > 0.0f ? fmaxf(v[i] * iv, FP8_MIN) : v[i];
+            const float q = div_by(v[i], sv, iv);
+            v[i] = v[i] > 0.0f ? fmaxf(q, FP8_MIN) : v[i];
+            m[i] = div_by(m[i], sm, im);
         }
         store_codes(static_cast<uint8_t *>(t.m) + at, n, vec, m);
         store_codes(static_cast<uint8_t *>(t.v) + at, n, vec, v);

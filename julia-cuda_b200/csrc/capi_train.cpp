@@ -177,8 +177,8 @@ int jc_linear(uint32_t type, uint32_t act, const void *x, size_t ldx, const void
     });
 }
 
-size_t jc_linear_ws_bytes(uint32_t act, uint32_t m, uint32_t n, uint32_t k) {
-    return n && k ? jc::linear_bwd_ws_bytes(act, m, n, k) : 0;
+size_t jc_linear_ws_bytes(uint32_t m, uint32_t n, uint32_t k) {
+    return n && k ? jc::linear_bwd_ws_bytes(m, n, k) : 0;
 }
 
 int jc_linear_backward(uint32_t type, uint32_t act, const void *dy, size_t lddy, const void *x, size_t ldx,
@@ -195,7 +195,7 @@ int jc_linear_backward(uint32_t type, uint32_t act, const void *dy, size_t lddy,
             !check_matrix(op, "z", z, ldz, n, 2, any && act) ||
             !check_matrix(op, "dx", dx, lddx, k, 2, false) || !check_matrix(op, "dw", dw, lddw, k, 2, false) ||
             !check_vector(op, "dbias", dbias, 4, false) ||
-            !check_vector(op, "ws", ws, 256, any && jc::linear_bwd_ws_bytes(act, m, n, k) > 0))
+            !check_vector(op, "ws", ws, 256, any && jc::linear_bwd_ws_bytes(m, n, k) > 0))
             return -1;
         jc::LinearBwdArgs a;
         a.type = type;

@@ -43,89 +43,6 @@ struct LinearOperand {
     size_t si, sk;
 };
 
-struct LinearParams {
-    LinearOperand a, b;
-    uint32_t m, n, k;  // c [m][n] = a [m][k] b [n][k]^T
-    uint32_t act;
-    const float *bias;
-    const void *res;
-    size_t ldres;
-    void *c;
-    size_t ldc;
-    void *z;
-    size_t ldz;
-    float *ws;  // split over k: [gridDim.z][m][n] partial sums instead of c
-};
-
-constexpr int LIN_T = 64, LIN_K = 16;  // the tile and its depth
-
-template <class T>
-__device__ __forceinline__ void lin_load(const LinearOperand &o, uint32_t i0, uint32_t rows, uint32_t k0,
-                                         uint32_t k1, float (*s)[LIN_T + 4]) {
-#pragma unroll
-    for (int l = 0; l < LIN_T * LIN_K / 256; l++) {
-        const uint32_t e = threadIdx.x + 256 * l;
-        // Consecutive threads read along the operand's contiguous axis.
-        const uint32_t i = o.sk == 1 ? e / LIN_K : e % LIN_T, k = o.sk == 1 ? e % LIN_K : e / LIN_T;
-        float v = 0.0f;
-        if (i0 + i < rows && k0 + k < k1)
-            v = static_cast<float>(static_cast<const T *>(o.p)[(size_t)(i0 + i) * o.si + (size_t)(k0 + k) * o.sk]);
-        s[k][i] = v;
-    }
-}
-
-template <class T, uint32_t ACT>
-__global__ void __launch_bounds__(256) linear_kernel(const LinearParams p) {
-    __shared__ float sa[LIN_K][LIN_T + 4], sb[LIN_K][LIN_T + 4];
-    pdl_wait();
-    pdl_launch_dependents();
-    const uint32_t m0 = blockIdx.y * LIN_T, n0 = blockIdx.x * LIN_T;
-    const uint32_t tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    const uint32_t blocks = (p.k + LIN_K - 1) / LIN_K;
-    const uint32_t kb = (uint32_t)((uint64_t)blocks * blockIdx.z / gridDim.z) * LIN_K;
-    const uint32_t ke = min(p.k, (uint32_t)((uint64_t)blocks * (blockIdx.z + 1) / gridDim.z) * LIN_K);
-    float acc[4][4] = {};
-    for (uint32_t k0 = kb; k0 < ke; k0 += LIN_K) {
-        __syncthreads();
-        lin_load<T>(p.a, m0, p.m, k0, ke, sa);
-        lin_load<T>(p.b, n0, p.n, k0, ke, sb);
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < LIN_K; k++) {
-            float a[4], b[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                a[i] = sa[k][ty * 4 + i];
-                b[i] = sb[k][tx * 4 + i];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t r = m0 + ty * 4 + i;
-        if (r >= p.m) continue;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint32_t c = n0 + tx * 4 + j;
-            if (c >= p.n) continue;
-            float v = acc[i][j];
-            if (p.ws) {
-                p.ws[((size_t)blockIdx.z * p.m + r) * p.n + c] = v;
-                continue;
-            }
-            if (p.bias) v += p.bias[c];
-            if (p.z) static_cast<T *>(p.z)[r * p.ldz + c] = static_cast<T>(v);
-            v = act_fwd<ACT>(v);
-            if (p.res) v += static_cast<float>(static_cast<const T *>(p.res)[r * p.ldres + c]);
-            static_cast<T *>(p.c)[r * p.ldc + c] = static_cast<T>(v);
-        }
-    }
-}
-
 // c [m][n] = the sum of `splits` partial products in ws, in their order.
 template <class T>
 __global__ void __launch_bounds__(256) linear_join_kernel(const float *ws, uint32_t splits, uint32_t m,
@@ -146,7 +63,7 @@ struct DzParams {
     const void *z;
     size_t ldz;
     uint32_t m, n;
-    void *dz;  // [m][n] dense, or nullptr
+    void *dz;  // [m][n], or nullptr
     size_t lddz;
     float *part;  // [gridDim.y][n] column sums, or nullptr
 };
@@ -173,10 +90,11 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const DzParams p) {
             if constexpr (ACT != 0) {
                 float z[V];
                 Elem<T, V>::load(static_cast<const T *>(p.z) + r * p.ldz + c, z);
+                // Rounded by itself: the sums must not depend on whether dz is stored too.
 #pragma unroll
-                for (int i = 0; i < V; i++) d[i] *= act_bwd<ACT>(z[i]);
-                Elem<T, V>::store(static_cast<T *>(p.dz) + r * p.lddz + c, d);
+                for (int i = 0; i < V; i++) d[i] = __fmul_rn(d[i], act_bwd<ACT>(z[i]));
             }
+            if (p.dz) Elem<T, V>::store(static_cast<T *>(p.dz) + r * p.lddz + c, d);
 #pragma unroll
             for (int i = 0; i < V; i++) sum[i] += d[i];
         }

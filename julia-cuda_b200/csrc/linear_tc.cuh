@@ -1,0 +1,540 @@
+// The linear layer's products on the tensor cores: c [m][n] = a b^T, a [m][k], b [n][k] of one 16-bit
+// type, f32 accumulators in tensor memory (tcgen05.mma, kind::f16).
+//
+// The three products of a training step differ in which axis of their operands is contiguous:
+//   forward   y  = x w^T    contracts over k, contiguous in both
+//   dx        dx = dz w     contracts over n: contiguous in dz, the row axis of w
+//   dw        dw = dz^T x   contracts over m: the row axis of both
+// An operand whose contiguous axis is not the contracted one needs no transposed copy: it is loaded
+// as it lies, in blocks of 64 (contiguous) x 64 (contracted), and its shared-memory descriptor says
+// so ("MN-major").
+//
+// Two kernels share the tiles, the epilogue and the roles:
+//   linear_tc_kernel   TMA loads; the operands' rows on 16-byte boundaries. One CTA per SM walks the 128 x BN
+//                      tiles; the epilogue of one runs under the main loop of the next (two
+//                      accumulators).
+//   linear_any_kernel  any strides and alignment: eight warps load elements and write them into the
+//                      same swizzled tiles. One tile a CTA.
+// Both: one warp issues the MMAs, eight run the epilogue.
+#pragma once
+#include <type_traits>
+
+#include "common.cuh"
+#include "elem.cuh"
+#include "linear.cuh"
+
+namespace jc {
+
+constexpr int LT_BM = 128, LT_BK = 64;
+constexpr int LT_EPI_WARPS = 8;
+constexpr int LT_STAGE_BUF = 4096;  // a warp's staging tile: 32 rows x 128 bytes
+
+// The instruction descriptor: umma_idesc_f16 with the operands' type and major axes.
+template <class T>
+__host__ __device__ constexpr uint32_t lt_idesc(int n, bool a_mn, bool b_mn) {
+    const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    return umma_idesc_f16(LT_BM, n) | (fmt << 7) | (fmt << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16);
+}
+
+// Shared-memory descriptor of an operand tile at saddr (1024-byte aligned), 128-byte swizzle.
+//   K-major:  rows of 64 contracted elements (128 bytes), 8-row groups 1024 bytes apart.
+//   MN-major: blocks of 64 rows of the contracted axis x 64 elements of the other (8 KB); the next
+//             8 contracted rows 1024 bytes on, the next 64 of the other axis a block on.
+template <bool MN>
+__device__ __forceinline__ uint64_t lt_desc(uint32_t saddr) {
+    uint64_t d = umma_desc_sw128(saddr);
+    if (MN) d = (d & ~((uint64_t)0x3FFF << 16)) | ((uint64_t)(8192 >> 4) << 16);
+    return d;
+}
+
+// Descriptor step (16-byte units) for the next 16 contracted elements: 32 bytes inside a row, or 16
+// rows on.
+template <bool MN>
+constexpr uint32_t LT_STEP = MN ? (16 * 128) >> 4 : 32 >> 4;
+
+struct LinearTcParams {
+    uint32_t m, n, k;
+    LinearOperand a, b;  // linear_any_kernel; linear_tc_kernel's come as tensor maps
+    const float *bias;
+    const void *res;
+    size_t ldres;
+    void *c;
+    size_t ldc;
+    void *z;
+    size_t ldz;
+    float *ws;        // split over k: [splits][m][n] partial sums instead of c
+    uint32_t splits;
+    uint32_t tiles_m, tiles_n;
+    unsigned int *err;
+};
+
+struct LinearTcKernelParams {
+    CUtensorMap map_a, map_b;
+    LinearTcParams p;
+};
+
+template <int BN>
+struct LtShape {
+    static constexpr int HALVES = BN >= 64 ? 2 : 1;        // column halves the eight warps split
+    static constexpr int CW = BN / HALVES < 64 ? BN / HALVES : 64;  // columns of an epilogue chunk
+    static constexpr int CHUNKS = BN / HALVES / CW;
+    static constexpr int B_ROWS = BN < 64 ? 64 : BN;       // an MN-major block is 64 wide
+    static constexpr int A_BYTES = LT_BM * 128, B_BYTES = B_ROWS * 128, STAGE = A_BYTES + B_BYTES;
+    static constexpr int TMEM = BN < 32 ? 32 : BN;         // columns of one accumulator
+};
+
+// ---------------------------------------------------------------------------------------------
+// epilogue
+
+// Moves a warp's 32 x CW tile between global memory and its staging buffer (rows of 128 bytes, 16-byte
+// chunk c of row r at chunk c ^ (r % 8), so that both a lane's own row and eight lanes to a row are
+// free of bank conflicts). VEC: global rows are on 16-byte boundaries; r0, c0: the tile's place; W:
+// bytes of an element.
+template <int CW, int W, bool VEC>
+__device__ __forceinline__ void lt_copy_out(const uint8_t *buf, uint8_t *g, size_t ld, uint32_t r0,
+                                            uint32_t c0, uint32_t rows, uint32_t cols) {
+    const uint32_t lane = threadIdx.x & 31;
+    if constexpr (VEC) {
+        constexpr int PER = CW * W / 16, STEP = 32 / PER;  // 16-byte chunks a row, rows a pass
+        const uint32_t c = lane % PER;
+#pragma unroll
+        for (int i = 0; i < 32 / STEP; i++) {
+            const uint32_t r = i * STEP + lane / PER;
+            const uint4 v = *reinterpret_cast<const uint4 *>(buf + r * 128 + ((c ^ (r & 7)) << 4));
+            if (r0 + r < rows && c0 + c * (16 / W) < cols)
+                *reinterpret_cast<uint4 *>(g + ((size_t)(r0 + r) * ld + c0) * W + c * 16) = v;
+        }
+    } else {
+        for (uint32_t e = lane; e < 32u * CW; e += 32) {
+            const uint32_t r = e / CW, c = e % CW, at = c * W;
+            const uint8_t *s = buf + r * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 15);
+            uint8_t *d = g + ((size_t)(r0 + r) * ld + c0 + c) * W;
+            if (r0 + r < rows && c0 + c < cols) {
+                if constexpr (W == 2)
+                    *reinterpret_cast<uint16_t *>(d) = *reinterpret_cast<const uint16_t *>(s);
+                else
+                    *reinterpret_cast<uint32_t *>(d) = *reinterpret_cast<const uint32_t *>(s);
+            }
+        }
+    }
+}
+
+// The 16-byte chunks lt_copy_out would write, read instead: into registers, then into the buffer.
+template <int CW>
+struct LtRes {
+    static constexpr int PER = CW * 2 / 16, STEP = 32 / PER, N = 32 / STEP;
+    uint4 v[N];
+    __device__ __forceinline__ void load(const uint8_t *g, size_t ld, uint32_t r0, uint32_t c0, uint32_t rows,
+                                         uint32_t cols) {
+        const uint32_t lane = threadIdx.x & 31, c = lane % PER;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const uint32_t r = i * STEP + lane / PER;
+            v[i] = make_uint4(0, 0, 0, 0);
+            if (r0 + r < rows && c0 + c * 8 < cols)
+                v[i] = *reinterpret_cast<const uint4 *>(g + ((size_t)(r0 + r) * ld + c0) * 2 + c * 16);
+        }
+    }
+    __device__ __forceinline__ void stage(uint8_t *buf) const {
+        const uint32_t lane = threadIdx.x & 31, c = lane % PER;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const uint32_t r = i * STEP + lane / PER;
+            *reinterpret_cast<uint4 *>(buf + r * 128 + ((c ^ (r & 7)) << 4)) = v[i];
+        }
+    }
+};
+
+// Any alignment: element by element into the buffer.
+template <int CW>
+__device__ __forceinline__ void lt_copy_in(uint8_t *buf, const uint8_t *g, size_t ld, uint32_t r0, uint32_t c0,
+                                           uint32_t rows, uint32_t cols) {
+    for (uint32_t e = threadIdx.x & 31; e < 32u * CW; e += 32) {
+        const uint32_t r = e / CW, c = e % CW, at = c * 2;
+        uint16_t v = 0;
+        if (r0 + r < rows && c0 + c < cols)
+            v = *reinterpret_cast<const uint16_t *>(g + ((size_t)(r0 + r) * ld + c0 + c) * 2);
+        *reinterpret_cast<uint16_t *>(buf + r * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 15)) = v;
+    }
+}
+
+// A lane's own row of the buffer, written or read eight elements at a time.
+template <class T, int CW>
+__device__ __forceinline__ void lt_put_row(uint8_t *buf, const float *v) {
+    const uint32_t r = threadIdx.x & 31;
+#pragma unroll
+    for (int c = 0; c < CW / 8; c++)
+        Elem<T, 8>::store(reinterpret_cast<T *>(buf + r * 128 + ((c ^ (r & 7)) << 4)), v + 8 * c);
+}
+
+template <class T, int CW>
+__device__ __forceinline__ void lt_add_row(const uint8_t *buf, float *v) {
+    const uint32_t r = threadIdx.x & 31;
+#pragma unroll
+    for (int c = 0; c < CW / 8; c++) {
+        float t[8];
+        Elem<T, 8>::load(reinterpret_cast<const T *>(buf + r * 128 + ((c ^ (r & 7)) << 4)), t);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[8 * c + i] += t[i];
+    }
+}
+
+// CW columns of this lane's accumulator row.
+template <int CW>
+__device__ __forceinline__ void lt_acc(uint32_t taddr, float *v) {
+    if constexpr (CW == 16) {
+        tmem_ld<16>(taddr, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < CW; i += 32) tmem_ld32(taddr + i, *reinterpret_cast<float(*)[32]>(v + i));
+    }
+    tc_wait_ld();
+}
+
+// One warp's share of a finished tile: rows 32 (warp % 4).. and half warp / 4 of the columns. `acc`:
+// the tile's accumulator; `res`: the first chunk's residual where it was requested early (VEC).
+template <class T, int BN, uint32_t ACT, bool VEC>
+__device__ __forceinline__ void lt_epilogue(const LinearTcParams &p, uint32_t acc, uint8_t *buf, uint32_t warp,
+                                            uint32_t m0, uint32_t n0, uint32_t split,
+                                            LtRes<LtShape<BN>::CW> &res) {
+    using S = LtShape<BN>;
+    constexpr int CW = S::CW;
+    if (warp / 4 >= (uint32_t)S::HALVES) return;
+    const uint32_t r0 = m0 + 32 * (warp & 3);
+    const uint32_t lane_acc = acc + ((32 * (warp & 3)) << 16);
+#pragma unroll 1
+    for (int ch = 0; ch < S::CHUNKS; ch++) {
+        const uint32_t cc = (warp >> 2) * (BN / 2) + ch * CW, c0 = n0 + cc;
+        float v[CW];
+        lt_acc<CW>(lane_acc + cc, v);
+        if (p.ws) {
+            // Partial sums, f32, 32 columns (128 bytes) at a time.
+            uint8_t *ws = reinterpret_cast<uint8_t *>(p.ws + (size_t)split * p.m * p.n);
+            constexpr int PW = CW < 32 ? CW : 32;
+#pragma unroll
+            for (int h = 0; h < CW / PW; h++) {
+                const uint32_t r = threadIdx.x & 31;
+                __syncwarp();
+#pragma unroll
+                for (int c = 0; c < PW / 4; c++)
+                    *reinterpret_cast<float4 *>(buf + r * 128 + ((c ^ (r & 7)) << 4)) =
+                        make_float4(v[h * PW + 4 * c], v[h * PW + 4 * c + 1], v[h * PW + 4 * c + 2], v[h * PW + 4 * c + 3]);
+                __syncwarp();
+                lt_copy_out<PW, 4, VEC>(buf, ws, p.n, r0, c0 + h * PW, p.m, p.n);
+            }
+            continue;
+        }
+        if (p.bias) {
+#pragma unroll
+            for (int j = 0; j < CW; j++)
+                if (VEC || c0 + j < p.n) v[j] += __ldg(p.bias + min(c0 + j, p.n - 1));
+        }
+        if (p.z) {
+            __syncwarp();
+            lt_put_row<T, CW>(buf, v);
+            __syncwarp();
+            lt_copy_out<CW, 2, VEC>(buf, static_cast<uint8_t *>(p.z), p.ldz, r0, c0, p.m, p.n);
+        }
+        if constexpr (ACT != 0) {
+#pragma unroll
+            for (int j = 0; j < CW; j++) v[j] = act_fwd<ACT>(v[j]);
+        }
+        if (p.res) {
+            const uint8_t *g = static_cast<const uint8_t *>(p.res);
+            __syncwarp();
+            if constexpr (VEC) {
+                if (ch > 0) res.load(g, p.ldres, r0, c0, p.m, p.n);
+                res.stage(buf);
+            } else {
+                lt_copy_in<CW>(buf, g, p.ldres, r0, c0, p.m, p.n);
+            }
+            __syncwarp();
+            lt_add_row<T, CW>(buf, v);
+        }
+        __syncwarp();
+        lt_put_row<T, CW>(buf, v);
+        __syncwarp();
+        lt_copy_out<CW, 2, VEC>(buf, static_cast<uint8_t *>(p.c), p.ldc, r0, c0, p.m, p.n);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// TMA kernel
+
+// An operand's tile of one stage: rows [row0, row0 + ROWS) x the 64 contracted from k0.
+template <int ROWS, bool MN>
+__device__ __forceinline__ void lt_tma(uint8_t *dst, const CUtensorMap *map, uint64_t *bar, uint32_t row0,
+                                       uint32_t k0) {
+    if constexpr (MN) {
+#pragma unroll
+        for (int j = 0; j < ROWS / 64; j++)
+            tma_load_2d(dst + j * 8192, map, bar, (int32_t)(row0 + 64 * j), (int32_t)k0);
+    } else {
+        tma_load_2d(dst, map, bar, (int32_t)k0, (int32_t)row0);
+    }
+}
+
+template <int BN>
+struct LtTcSmem {
+    using S = LtShape<BN>;
+    static constexpr int STAGES = BN == 256 ? 4 : 6;
+    static constexpr int BYTES = STAGES * S::STAGE + LT_EPI_WARPS * LT_STAGE_BUF + 256 + 1024;
+};
+
+constexpr int LT_TC_THREADS = 32 * (LT_EPI_WARPS + 2);
+
+template <class T, int BN, bool A_MN, bool B_MN, uint32_t ACT, bool VEC>
+__global__ void __launch_bounds__(LT_TC_THREADS, 1)
+    linear_tc_kernel(const __grid_constant__ LinearTcKernelParams kp) {
+    using S = LtShape<BN>;
+    constexpr int STAGES = LtTcSmem<BN>::STAGES;
+    const LinearTcParams &p = kp.p;
+    dev_err_bind(p.err);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *bufs = base + STAGES * S::STAGE;
+    uint64_t *full = reinterpret_cast<uint64_t *>(bufs + LT_EPI_WARPS * LT_STAGE_BUF);
+    uint64_t *empty = full + STAGES, *acc_full = empty + STAGES, *acc_empty = acc_full + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr uint32_t COLS = 2 * S::TMEM;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&acc_full[i], 1);
+            mbar_init(&acc_empty[i], LT_EPI_WARPS);
+        }
+        fence_barrier_init();
+    }
+    if (warp == LT_EPI_WARPS + 1) tmem_alloc(tmem_slot, COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+    pdl_launch_dependents();
+
+    const uint32_t tiles = p.tiles_m * p.tiles_n, items = tiles * p.splits;
+    const uint32_t blocks = (p.k + LT_BK - 1) / LT_BK;
+    if (warp == LT_EPI_WARPS) {
+        if (lane == 0) {
+            tma_prefetch_desc(&kp.map_a);
+            tma_prefetch_desc(&kp.map_b);
+            uint32_t it = 0;
+            bool ok = true;
+            for (uint32_t i = blockIdx.x; ok && i < items; i += gridDim.x) {
+                const uint32_t t = i % tiles, z = i / tiles, n0 = t % p.tiles_n * BN, m0 = t / p.tiles_n * LT_BM;
+                const uint32_t k1 = (uint32_t)((uint64_t)blocks * (z + 1) / p.splits);
+                for (uint32_t kb = (uint32_t)((uint64_t)blocks * z / p.splits); kb < k1; kb++, it++) {
+                    const uint32_t s = it % STAGES, round = it / STAGES;
+                    if (round > 0 && !mbar_wait(&empty[s], (round & 1) ^ 1, JC_DEV_TIMEOUT_EMPTY)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t *st = base + s * S::STAGE;
+                    mbar_arrive_expect_tx(&full[s], S::A_BYTES + S::B_BYTES);
+                    lt_tma<LT_BM, A_MN>(st, &kp.map_a, &full[s], m0, kb * LT_BK);
+                    lt_tma<BN, B_MN>(st + S::A_BYTES, &kp.map_b, &full[s], n0, kb * LT_BK);
+                }
+            }
+            // After a wait that gave up, the copies still in flight land before the CTA may leave.
+            if (!ok)
+                for (uint32_t j = it > STAGES ? it - STAGES : 0; j < it; j++)
+                    mbar_wait(&full[j % STAGES], (j / STAGES) & 1, JC_DEV_TIMEOUT_FULL);
+        }
+    } else if (warp == LT_EPI_WARPS + 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = lt_idesc<T>(BN, A_MN, B_MN);
+            uint32_t it = 0, done = 0;
+            bool ok = true;
+            for (uint32_t i = blockIdx.x; ok && i < items; i += gridDim.x, done++) {
+                const uint32_t z = i / tiles, buf = done & 1, use = done >> 1;
+                if (use > 0 && !mbar_wait(&acc_empty[buf], (use & 1) ^ 1, JC_DEV_TIMEOUT_MMA)) break;
+                tc_fence_after();
+                const uint32_t acc = tmem + buf * S::TMEM;
+                const uint32_t k0 = (uint32_t)((uint64_t)blocks * z / p.splits);
+                const uint32_t k1 = (uint32_t)((uint64_t)blocks * (z + 1) / p.splits);
+                for (uint32_t kb = k0; kb < k1; kb++, it++) {
+                    const uint32_t s = it % STAGES;
+                    if (!mbar_wait(&full[s], (it / STAGES) & 1, JC_DEV_TIMEOUT_FULL)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t ad = lt_desc<A_MN>(smem_u32(base + s * S::STAGE));
+                    const uint64_t bd = lt_desc<B_MN>(smem_u32(base + s * S::STAGE + S::A_BYTES));
+#pragma unroll
+                    for (int kk = 0; kk < LT_BK / 16; kk++)
+                        tc_mma_f16(acc, ad + kk * LT_STEP<A_MN>, bd + kk * LT_STEP<B_MN>, idesc, kb > k0 || kk > 0);
+                    tc_commit(&empty[s]);
+                }
+                tc_commit(&acc_full[buf]);
+            }
+        }
+    } else {
+        uint8_t *buf = bufs + warp * LT_STAGE_BUF;
+        LtRes<S::CW> res;
+        uint32_t done = 0;
+        for (uint32_t i = blockIdx.x; i < items; i += gridDim.x, done++) {
+            const uint32_t t = i % tiles, n0 = t % p.tiles_n * BN, m0 = t / p.tiles_n * LT_BM;
+            // The first chunk's residual is on its way while the accumulator is still being summed.
+            if (VEC && p.res && warp / 4 < (uint32_t)S::HALVES)
+                res.load(static_cast<const uint8_t *>(p.res), p.ldres, m0 + 32 * (warp & 3),
+                         n0 + (warp >> 2) * (BN / 2), p.m, p.n);
+            if (!mbar_wait_sleep(&acc_full[done & 1], (done >> 1) & 1, JC_DEV_TIMEOUT_MMA)) break;
+            tc_fence_after();
+            lt_epilogue<T, BN, ACT, VEC>(p, tmem + (done & 1) * S::TMEM, buf, warp, m0, n0, i / tiles, res);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[done & 1]);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == LT_EPI_WARPS + 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, COLS);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// any strides and alignment
+
+// ROWS x 64 of an operand from (row0, k0) into a stage's tile by eight warps, zeros past (rows, k1). A
+// warp reads along the contiguous axis, two elements a lane; `pairs`: every row starts on a 4-byte
+// boundary.
+template <int ROWS, bool MN>
+__device__ __forceinline__ void lt_gather(uint8_t *dst, const LinearOperand &o, uint32_t row0, uint32_t rows,
+                                          uint32_t k0, uint32_t k1, bool pairs) {
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint16_t *g = static_cast<const uint16_t *>(o.p);
+    constexpr int LINES = MN ? 64 * ((ROWS + 63) / 64) : ROWS;  // 128-byte lines of the tile
+    constexpr int BATCH = LINES / 8 < 16 ? LINES / 8 : 16;
+#pragma unroll 1
+    for (int l0 = 0; l0 < LINES / 8; l0 += BATCH) {
+        uint32_t v[BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; j++) {
+            const uint32_t line = warp + 8 * (l0 + j);
+            // The line's place, and how many of this lane's two elements exist.
+            const uint32_t across = MN ? row0 + line / 64 * 64 + 2 * lane : k0 + 2 * lane;
+            const uint32_t end = MN ? min(rows, row0 + ROWS) : k1;
+            const uint32_t other = MN ? k0 + line % 64 : row0 + line;
+            const bool there = other < (MN ? k1 : rows);
+            const uint16_t *s = g + (size_t)other * (MN ? o.sk : o.si) + across;
+            uint32_t lo = 0, hi = 0;
+            if (there && across + 1 < end && pairs) {
+                lo = *reinterpret_cast<const uint32_t *>(s);
+            } else if (there) {
+                if (across < end) lo = s[0];
+                if (across + 1 < end) hi = s[1];
+            }
+            v[j] = lo | hi << 16;
+        }
+#pragma unroll
+        for (int j = 0; j < BATCH; j++) {
+            const uint32_t line = warp + 8 * (l0 + j), r = line & 7;
+            *reinterpret_cast<uint32_t *>(dst + line * 128 + (((lane >> 2) ^ r) << 4) + (lane & 3) * 4) = v[j];
+        }
+    }
+}
+
+template <int BN>
+struct LtAnySmem {
+    using S = LtShape<BN>;
+    static constexpr int STAGES = 3;
+    static constexpr int BYTES = STAGES * S::STAGE + LT_EPI_WARPS * LT_STAGE_BUF + 256 + 1024;
+};
+
+constexpr int LT_ANY_THREADS = 32 * (LT_EPI_WARPS + 1);
+
+template <class T, int BN, bool A_MN, bool B_MN, uint32_t ACT>
+__global__ void __launch_bounds__(LT_ANY_THREADS)
+    linear_any_kernel(const __grid_constant__ LinearTcParams p) {
+    using S = LtShape<BN>;
+    constexpr int STAGES = LtAnySmem<BN>::STAGES;
+    dev_err_bind(p.err);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *bufs = base + STAGES * S::STAGE;
+    uint64_t *full = reinterpret_cast<uint64_t *>(bufs + LT_EPI_WARPS * LT_STAGE_BUF);
+    uint64_t *empty = full + STAGES, *acc_full = empty + STAGES;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_full + 1);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(&full[s], LT_EPI_WARPS);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(acc_full, 1);
+        fence_barrier_init();
+    }
+    if (warp == LT_EPI_WARPS) tmem_alloc(tmem_slot, S::TMEM);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+    pdl_launch_dependents();
+
+    const uint32_t tiles = p.tiles_m * p.tiles_n, t = blockIdx.x % tiles, z = blockIdx.x / tiles;
+    const uint32_t n0 = t % p.tiles_n * BN, m0 = t / p.tiles_n * LT_BM;
+    const uint32_t blocks = (p.k + LT_BK - 1) / LT_BK;
+    const uint32_t kb0 = (uint32_t)((uint64_t)blocks * z / p.splits);
+    const uint32_t count = (uint32_t)((uint64_t)blocks * (z + 1) / p.splits) - kb0;
+    if (warp == LT_EPI_WARPS) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = lt_idesc<T>(BN, A_MN, B_MN);
+            for (uint32_t it = 0; it < count; it++) {
+                const uint32_t s = it % STAGES;
+                if (!mbar_wait(&full[s], (it / STAGES) & 1, JC_DEV_TIMEOUT_FULL)) break;
+                tc_fence_after();
+                const uint64_t ad = lt_desc<A_MN>(smem_u32(base + s * S::STAGE));
+                const uint64_t bd = lt_desc<B_MN>(smem_u32(base + s * S::STAGE + S::A_BYTES));
+#pragma unroll
+                for (int kk = 0; kk < LT_BK / 16; kk++)
+                    tc_mma_f16(tmem, ad + kk * LT_STEP<A_MN>, bd + kk * LT_STEP<B_MN>, idesc, it > 0 || kk > 0);
+                tc_commit(&empty[s]);
+            }
+            tc_commit(acc_full);
+        }
+    } else {
+        auto pairs = [](const LinearOperand &o, bool mn) {
+            return (reinterpret_cast<uintptr_t>(o.p) % 4 == 0) && (mn ? o.sk : o.si) % 2 == 0;
+        };
+        const bool pa = pairs(p.a, A_MN), pb = pairs(p.b, B_MN);
+        bool ok = true;
+        for (uint32_t it = 0; it < count; it++) {
+            const uint32_t s = it % STAGES, round = it / STAGES;
+            // All lanes wait: each writes into the stage.
+            if (round > 0 && !mbar_wait(&empty[s], (round & 1) ^ 1, JC_DEV_TIMEOUT_EMPTY)) ok = false;
+            if (!__all_sync(0xffffffffu, ok)) break;
+            const uint32_t k0 = (kb0 + it) * LT_BK;
+            uint8_t *st = base + s * S::STAGE;
+            lt_gather<LT_BM, A_MN>(st, p.a, m0, p.m, k0, p.k, pa);
+            lt_gather<BN, B_MN>(st + S::A_BYTES, p.b, n0, p.n, k0, p.k, pb);
+            fence_proxy_async();  // the MMAs read shared memory through the async proxy
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[s]);
+        }
+        ok = mbar_wait_sleep(acc_full, 0, JC_DEV_TIMEOUT_MMA);
+        if (__all_sync(0xffffffffu, ok)) {
+            tc_fence_after();
+            LtRes<S::CW> res;
+            lt_epilogue<T, BN, ACT, false>(p, tmem, bufs + warp * LT_STAGE_BUF, warp, m0, n0, z, res);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == LT_EPI_WARPS) {
+        tc_fence_after();
+        tmem_dealloc(tmem, S::TMEM);
+    }
+}
+
+}  // namespace jc

@@ -8,7 +8,7 @@
 
 #include "adamw.cuh"
 #include "launch.h"
-#include "linear.cuh"
+#include "linear_tc.cuh"
 #include "loss.cuh"
 #include "norm.cuh"
 
@@ -122,79 +122,214 @@ static bool with_act(uint32_t act, F &&f) {
     return f(std::integral_constant<uint32_t, 0>());
 }
 
+// One product c = a b^T and how it is run.
+struct Product {
+    LinearOperand a{}, b{};  // the contiguous axis of each has stride 1
+    uint32_t m = 0, n = 0, k = 0, act = 0;
+    const float *bias = nullptr;
+    const void *res = nullptr;
+    size_t ldres = 0;
+    void *c = nullptr;
+    size_t ldc = 0;
+    void *z = nullptr;
+    size_t ldz = 0;
+    float *ws = nullptr;
+    uint32_t splits = 1;
+};
+
+// The tensor map of an operand: boxes of 64 contracted elements x `rows` rows where the contracted
+// axis is contiguous, else of 64 x 64.
 template <class T>
-static bool launch_product(uint32_t act, const LinearParams &p, uint32_t splits, cudaStream_t s) {
-    const dim3 grid((p.n + LIN_T - 1) / LIN_T, (p.m + LIN_T - 1) / LIN_T, splits);
-    if (grid.y > 65535) {
-        set_error("linear: too many rows");
+static bool make_operand_map(CUtensorMap *map, const LinearOperand &o, uint32_t rows, uint32_t k, bool mn,
+                             uint32_t box_rows) {
+    auto fn = encode_fn();
+    if (!fn) {
+        set_error("cuTensorMapEncodeTiled is not available from the CUDA driver");
         return false;
     }
-    return with_act(act, [&](auto a) {
-        return launch_ex(linear_kernel<T, decltype(a)::value>, grid, dim3(256), 0, s, true, "linear", p);
-    });
+    cuuint64_t dims[2] = {mn ? rows : k, mn ? k : rows};
+    cuuint64_t strides[1] = {(mn ? o.sk : o.si) * 2};
+    cuuint32_t box[2] = {64, mn ? 64 : box_rows}, es[2] = {1, 1};
+    const CUresult r =
+        fn(map, std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+           2, const_cast<void *>(o.p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r == CUDA_SUCCESS) return true;
+    set_error("linear: cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+    return false;
+}
+
+// Whether TMA can load an operand: its rows on 16-byte boundaries (and a row distance it can hold).
+static bool tma_ok(const LinearOperand &o, bool mn) {
+    const size_t ld = mn ? o.sk : o.si;
+    return aligned16(o.p, ld, 2) && ld * 2 < ((size_t)1 << 40);
+}
+
+static bool out_vec(const Product &q) {
+    return q.n % 8 == 0 && aligned16(q.c, q.ldc, 2) && (!q.z || aligned16(q.z, q.ldz, 2)) &&
+           (!q.res || aligned16(q.res, q.ldres, 2));
+}
+
+template <class T, int BN, bool A_MN, bool B_MN, uint32_t ACT, bool VEC>
+static bool launch_tc(const Product &q, LinearTcParams &p, cudaStream_t s) {
+    static std::atomic<uint64_t> smem_set{0};
+    auto kern = linear_tc_kernel<T, BN, A_MN, B_MN, ACT, VEC>;
+    LinearTcKernelParams kp;
+    kp.p = p;
+    if (!ensure_smem(kern, LtTcSmem<BN>::BYTES, smem_set) ||
+        !make_operand_map<T>(&kp.map_a, q.a, q.m, q.k, A_MN, LT_BM) ||
+        !make_operand_map<T>(&kp.map_b, q.b, q.n, q.k, B_MN, BN))
+        return false;
+    const uint64_t items = (uint64_t)p.tiles_m * p.tiles_n * p.splits;
+    const uint32_t grid = (uint32_t)std::min<uint64_t>(items, (uint64_t)sm_count());
+    return launch_ex(kern, dim3(grid), dim3(LT_TC_THREADS), LtTcSmem<BN>::BYTES, s, true, "linear", kp);
+}
+
+template <class T, int BN, bool A_MN, bool B_MN, uint32_t ACT>
+static bool launch_any(const LinearTcParams &p, cudaStream_t s) {
+    static std::atomic<uint64_t> smem_set{0};
+    auto kern = linear_any_kernel<T, BN, A_MN, B_MN, ACT>;
+    if (!ensure_smem(kern, LtAnySmem<BN>::BYTES, smem_set)) return false;
+    return launch_ex(kern, dim3(p.tiles_m * p.tiles_n * p.splits), dim3(LT_ANY_THREADS), LtAnySmem<BN>::BYTES, s,
+                     true, "linear", p);
+}
+
+// Microseconds a product takes by the TMA kernel with BN-column tiles: the busiest CTA's items, each a
+// main loop of about 0.28 us per 64 contracted elements whatever BN is (one thread's MMAs complete in
+// order at about 130 cycles each) plus the part of its epilogue that nothing hides.
+static double tc_us(uint32_t m, uint32_t n, uint32_t k, uint32_t bn, uint32_t splits, uint32_t sms) {
+    const uint64_t items = (uint64_t)((m + LT_BM - 1) / LT_BM) * ((n + bn - 1) / bn) * splits;
+    const uint32_t blocks = ((k + LT_BK - 1) / LT_BK + splits - 1) / splits;
+    return (double)((items + sms - 1) / sms) * (0.28 * blocks + 0.5) + 2.0 + 0.008 * bn;
+}
+
+static uint32_t pick_bn(uint32_t m, uint32_t n, uint32_t k, uint32_t splits, uint32_t sms) {
+    uint32_t best = 64;
+    for (uint32_t bn : {128u, 256u})
+        if (tc_us(m, n, k, bn, splits, sms) <= tc_us(m, n, k, best, splits, sms)) best = bn;
+    return best;
+}
+
+// Runs a product: A_MN / B_MN say that the operand's contiguous axis is not the contracted one.
+template <class T, bool A_MN, bool B_MN, uint32_t ACT>
+static bool launch_product(const Product &q, cudaStream_t s) {
+    LinearTcParams p{};
+    p.m = q.m;
+    p.n = q.n;
+    p.k = q.k;
+    p.a = q.a;
+    p.b = q.b;
+    p.bias = q.bias;
+    p.res = q.res;
+    p.ldres = q.ldres;
+    p.c = q.c;
+    p.ldc = q.ldc;
+    p.z = q.z;
+    p.ldz = q.ldz;
+    p.ws = q.ws;
+    p.splits = q.splits;
+    p.err = module_error_word();
+    if (!p.err) return false;
+    p.tiles_m = (q.m + LT_BM - 1) / LT_BM;
+    auto tiles = [&](uint32_t bn) {
+        p.tiles_n = (q.n + bn - 1) / bn;
+        if ((uint64_t)p.tiles_m * p.tiles_n * p.splits <= 0x7FFFFFFFull) return true;
+        set_error("linear: too many tiles");
+        return false;
+    };
+    if (tma_ok(q.a, A_MN) && tma_ok(q.b, B_MN)) {
+        const uint32_t bn = pick_bn(q.m, q.n, q.k, q.splits, (uint32_t)sm_count());
+        const bool vec = out_vec(q);
+        if (!tiles(bn)) return false;
+        auto run = [&](auto w) {
+            constexpr int BN = decltype(w)::value;
+            // The gradients' outputs are as aligned as the operands they sit beside, or go the other way.
+            return vec ? launch_tc<T, BN, A_MN, B_MN, ACT, true>(q, p, s)
+                       : launch_tc<T, BN, A_MN, B_MN, ACT, false>(q, p, s);
+        };
+        return bn == 256 ? run(Int<256>()) : bn == 128 ? run(Int<128>()) : run(Int<64>());
+    }
+    if (q.n <= 16) return tiles(16) && launch_any<T, 16, A_MN, B_MN, ACT>(p, s);
+    if (q.n <= 64) return tiles(64) && launch_any<T, 64, A_MN, B_MN, ACT>(p, s);
+    return tiles(128) && launch_any<T, 128, A_MN, B_MN, ACT>(p, s);
 }
 
 bool launch_linear(const LinearArgs &a, cudaStream_t s) {
     if (a.m == 0) return true;
-    LinearParams p{};
-    p.a = LinearOperand{a.x, a.ldx, 1};
-    p.b = LinearOperand{a.w, a.ldw, 1};
-    p.m = a.m;
-    p.n = a.n;
-    p.k = a.k;
-    p.bias = a.bias;
-    p.res = a.res;
-    p.ldres = a.ldres;
-    p.c = a.y;
-    p.ldc = a.ldy;
-    p.z = a.z;
-    p.ldz = a.ldz;
-    return with_half(a.type, [&](auto t) { return launch_product<decltype(t)>(a.act, p, 1, s); });
+    Product q;
+    q.a = LinearOperand{a.x, a.ldx, 1};
+    q.b = LinearOperand{a.w, a.ldw, 1};
+    q.m = a.m;
+    q.n = a.n;
+    q.k = a.k;
+    q.bias = a.bias;
+    q.res = a.res;
+    q.ldres = a.ldres;
+    q.c = a.y;
+    q.ldc = a.ldy;
+    q.z = a.z;
+    q.ldz = a.ldz;
+    return with_half(a.type, [&](auto t) {
+        return with_act(a.act, [&](auto act) {
+            return launch_product<decltype(t), false, false, decltype(act)::value>(q, s);
+        });
+    });
 }
 
-// The backward pass's workspace: dz (16 bits), the column sums' parts, dw's partial products, each
-// from a 256-byte boundary.
+// The backward pass's workspace: dz (16 bits, rows padded to 16 bytes), the column sums' parts, dw's
+// partial products, each from a 256-byte boundary.
 struct LinearBwdPlan {
     uint32_t dz_parts, splits;
-    size_t lddz, dz_at, part_at, ws_at, bytes;
+    size_t lddz, part_at, ws_at, bytes;
 };
 
-static LinearBwdPlan plan_linear_bwd(uint32_t act, uint32_t m, uint32_t n, uint32_t k) {
+static LinearBwdPlan plan_linear_bwd(uint32_t m, uint32_t n, uint32_t k) {
     LinearBwdPlan p{};
     auto up = [](size_t v) { return (v + 255) / 256 * 256; };
     p.dz_parts = (m + DZ_ROWS - 1) / DZ_ROWS;
-    p.lddz = n;
-    p.part_at = act ? up((size_t)m * p.lddz * 2) : 0;
+    p.lddz = (n + 7) / 8 * 8;
+    p.part_at = up((size_t)m * p.lddz * 2);
     p.ws_at = p.part_at + up((size_t)p.dz_parts * n * 4);
-    const uint64_t tiles = (uint64_t)((n + LIN_T - 1) / LIN_T) * ((k + LIN_T - 1) / LIN_T);
-    p.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(64, 296 / tiles), m / 64));
+    // dw's contraction runs over the rows: split so that its few tiles still fill the SMs.
+    const uint32_t sms = 148, blocks = (m + LT_BK - 1) / LT_BK;
+    p.splits = 1;
+    double best = 1e30;
+    for (uint32_t s = 1; s <= std::min(32u, std::max(1u, blocks)); s++) {
+        const double us = tc_us(n, k, m, pick_bn(n, k, m, s, sms), s, sms) + (s > 1 ? 2.0 + 8e-6 * s * n * k / 3.0 : 0.0);
+        if (us < best) {
+            best = us;
+            p.splits = s;
+        }
+    }
     p.bytes = p.ws_at + (p.splits > 1 ? up((size_t)p.splits * n * k * 4) : 0);
     return p;
 }
 
-size_t linear_bwd_ws_bytes(uint32_t act, uint32_t m, uint32_t n, uint32_t k) {
-    return plan_linear_bwd(act, m, n, k).bytes;
-}
+size_t linear_bwd_ws_bytes(uint32_t m, uint32_t n, uint32_t k) { return plan_linear_bwd(m, n, k).bytes; }
 
 bool launch_linear_bwd(const LinearBwdArgs &a, cudaStream_t s) {
-    const LinearBwdPlan plan = plan_linear_bwd(a.act, a.m, a.n, a.k);
+    const LinearBwdPlan plan = plan_linear_bwd(a.m, a.n, a.k);
     uint8_t *ws = static_cast<uint8_t *>(a.ws);
     float *part = reinterpret_cast<float *>(ws + plan.part_at);
     return with_half(a.type, [&](auto t) {
         using T = decltype(t);
-        const T *dz = static_cast<const T *>(a.dy);
+        const void *dz = a.dy;
         size_t lddz = a.lddy;
-        const bool need_dz = a.act && (a.dx || a.dw);
-        if (a.m > 0 && (need_dz || a.dbias)) {
-            T *out = reinterpret_cast<T *>(ws + plan.dz_at);
-            const DzParams p{a.dy, a.lddy, a.z, a.ldz, a.m, a.n, out, plan.lddz, a.dbias ? part : nullptr};
-            if (a.act) {
-                dz = out;
+        // dz is dy itself where there is no activation and TMA can load dy.
+        const bool write = (a.dx || a.dw) && (a.act || !aligned16(a.dy, a.lddy, 2));
+        if (a.m > 0 && (write || a.dbias)) {
+            const DzParams p{a.dy, a.lddy, a.z, a.ldz, a.m, a.n, write ? ws : nullptr, plan.lddz, a.dbias ? part : nullptr};
+            if (write) {
+                dz = ws;
                 lddz = plan.lddz;
             }
             const bool vec = a.n % 8 == 0 && aligned16(a.dy, a.lddy, 2) && (!a.act || aligned16(a.z, a.ldz, 2));
             const uint32_t cols = vec ? 256 : 32;
             const dim3 grid((a.n + cols - 1) / cols, plan.dz_parts);
+            if (grid.y > 65535) {
+                set_error("linear_backward: too many rows");
+                return false;
+            }
             if (!with_act(a.act, [&](auto act) {
                     constexpr uint32_t ACT = decltype(act)::value;
                     return vec ? launch_ex(linear_dz_kernel<T, ACT, 8>, grid, dim3(256), 0, s, true, "dz", p)
@@ -204,32 +339,36 @@ bool launch_linear_bwd(const LinearBwdArgs &a, cudaStream_t s) {
         }
         if (a.dbias && !launch_column_sum(part, a.m ? plan.dz_parts : 0, a.n, a.n, a.dbias, nullptr, s)) return false;
         if (a.dx && a.m > 0) {
-            LinearParams p{};
-            p.a = LinearOperand{dz, lddz, 1};
-            p.b = LinearOperand{a.w, 1, a.ldw};
-            p.m = a.m;
-            p.n = a.k;
-            p.k = a.n;
-            p.c = a.dx;
-            p.ldc = a.lddx;
-            if (!launch_product<T>(0, p, 1, s)) return false;
+            Product q;
+            q.a = LinearOperand{dz, lddz, 1};
+            q.b = LinearOperand{a.w, 1, a.ldw};
+            q.m = a.m;
+            q.n = a.k;
+            q.k = a.n;
+            q.c = a.dx;
+            q.ldc = a.lddx;
+            if (!launch_product<T, false, true, 0>(q, s)) return false;
         }
         if (a.dw) {
-            LinearParams p{};
-            p.a = LinearOperand{dz, 1, lddz};
-            p.b = LinearOperand{a.x, 1, a.ldx};
-            p.m = a.n;
-            p.n = a.k;
-            p.k = a.m;
-            p.c = a.dw;
-            p.ldc = a.lddw;
-            p.ws = plan.splits > 1 ? reinterpret_cast<float *>(ws + plan.ws_at) : nullptr;
-            if (!launch_product<T>(0, p, plan.splits, s)) return false;
-            if (p.ws) {
+            float *parts = nullptr;
+            if (a.m > 0) {
+                Product q;
+                q.a = LinearOperand{dz, 1, lddz};
+                q.b = LinearOperand{a.x, 1, a.ldx};
+                q.m = a.n;
+                q.n = a.k;
+                q.k = a.m;
+                q.c = a.dw;
+                q.ldc = a.lddw;
+                q.splits = plan.splits;
+                if (plan.splits > 1) q.ws = parts = reinterpret_cast<float *>(ws + plan.ws_at);
+                if (!launch_product<T, true, true, 0>(q, s)) return false;
+            }
+            if (parts || a.m == 0) {
                 const size_t all = (size_t)a.n * a.k;
                 const uint32_t blocks = (uint32_t)std::min<size_t>((all + 255) / 256, 148 * 8);
                 if (!launch_ex(linear_join_kernel<T>, dim3(blocks), dim3(256), 0, s, true, "linear join",
-                               (const float *)p.ws, plan.splits, a.n, a.k, static_cast<T *>(a.dw), a.lddw))
+                               (const float *)parts, a.m ? plan.splits : 0u, a.n, a.k, static_cast<T *>(a.dw), a.lddw))
                     return false;
             }
         }

@@ -76,7 +76,7 @@ struct LinearBwdArgs {
     float *dbias = nullptr;
     void *ws = nullptr;
 };
-size_t linear_bwd_ws_bytes(uint32_t act, uint32_t m, uint32_t n, uint32_t k);
+size_t linear_bwd_ws_bytes(uint32_t m, uint32_t n, uint32_t k);
 bool launch_linear_bwd(const LinearBwdArgs &a, cudaStream_t s);
 
 struct LossArgs {

@@ -126,7 +126,7 @@ def linear_backward(dy, x, w, *, z=None, act: str = "none", dx=None, dw=None, db
                     stream=None) -> None:
     """The gradients of linear (jc_linear_backward), each written if its tensor is given: dx [m, k],
     dw [n, k] of x's type, dbias [n] f32. z (linear's) is read unless act is "none". ws:
-    jc_linear_ws_bytes(act, m, n, k) bytes (allocated here when not given)."""
+    jc_linear_ws_bytes(m, n, k) bytes (allocated here when not given)."""
     op = "linear_backward"
     t = _type(op, x, halves=True)
     m, k = x.shape
@@ -138,7 +138,7 @@ def linear_backward(dy, x, w, *, z=None, act: str = "none", dx=None, dw=None, db
     zp, ldz = _matrix(op, "z", z, m, n, x.dtype)
     dxp, lddx = _matrix(op, "dx", dx, m, k, x.dtype)
     dwp, lddw = _matrix(op, "dw", dw, n, k, x.dtype)
-    need = lib().jc_linear_ws_bytes(a, m, n, k)
+    need = lib().jc_linear_ws_bytes(m, n, k)
     if ws is None:
         ws = _scratch(need, torch.uint8, x, stream)
     elif ws.numel() * ws.element_size() < need:

@@ -62,8 +62,8 @@ def test_linear_refusals(jc, buf):
                     (dict(act=RELU), "z is null"), (dict(lddw=1), "dw's rows"), (dict(ws=None), "ws is null"),
                     (dict(ws=p + 16), "ws is misaligned")):
         assert bwd(**kw) == -1 and why in jc.last_error(), (kw, jc.last_error())
-    assert L.jc_linear_ws_bytes(RELU, 4096, 2048, 768) >= 4096 * 2048 * 2   # dz
-    assert L.jc_linear_ws_bytes(0, 10, 0, 5) == 0
+    assert L.jc_linear_ws_bytes(4096, 2048, 768) >= 4096 * 2048 * 2   # dz
+    assert L.jc_linear_ws_bytes(10, 0, 5) == 0
 
 
 def test_choice_loss_refusals(jc, buf):
