@@ -203,8 +203,9 @@ def _t_ptr(t):
 
 def _stream(stream):
     if stream is None:
+        # The current stream's handle without building a Stream object (3 us of a 7 us call).
         import torch
-        return torch.cuda.current_stream().cuda_stream
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
     return getattr(stream, "cuda_stream", stream)
 
 

@@ -453,7 +453,7 @@ struct LtAnySmem {
 constexpr int LT_ANY_THREADS = 32 * (LT_EPI_WARPS + 1);
 
 template <class T, int BN, bool A_MN, bool B_MN, uint32_t ACT>
-__global__ void __launch_bounds__(LT_ANY_THREADS)
+__global__ void __launch_bounds__(LT_ANY_THREADS, 1)
     linear_any_kernel(const __grid_constant__ LinearTcParams p) {
     using S = LtShape<BN>;
     constexpr int STAGES = LtAnySmem<BN>::STAGES;

@@ -21,42 +21,150 @@ struct LossParams {
     unsigned int *err;
 };
 
-// One warp a request.
-__global__ void __launch_bounds__(128) choice_loss_kernel(const LossParams p) {
-    dev_err_bind(p.err);
-    pdl_wait();
-    pdl_launch_dependents();
-    const uint32_t r = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (r >= p.requests) return;
-    const int64_t a = p.offsets[r], b = p.offsets[r + 1];
-    int32_t gold = p.gold[r];
-    float w = p.weight ? p.weight[r] : 1.0f;
-    if (a < 0 || b < a || b > (int64_t)p.n_logits || gold >= b - a) {
+// Request r's span and right marker, checked: false (recorded) if they are out of range.
+__device__ __forceinline__ bool loss_request(const LossParams &p, uint32_t r, uint32_t &a, uint32_t &b, int32_t &gold,
+                                             float &w) {
+    const int32_t lo = p.offsets[r], hi = p.offsets[r + 1];
+    gold = p.gold[r];
+    w = p.weight ? p.weight[r] : 1.0f;
+    a = (uint32_t)lo;
+    b = (uint32_t)hi;
+    return lo >= 0 && hi >= lo && b <= p.n_logits && gold < hi - lo;
+}
+
+// Sums and maxima over a group of G threads: a warp or the block.
+template <int G>
+__device__ __forceinline__ float loss_sum(float v, float *part) {
+    v = warp_sum(v);
+    if constexpr (G > 32) {
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < G / 32; i++) v += part[i];
+    }
+    return v;
+}
+template <int G>
+__device__ __forceinline__ float loss_max(float v, float *part) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if constexpr (G > 32) {
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < G / 32; i++) v = fmaxf(v, part[i]);
+    }
+    return v;
+}
+
+// One request by a group of G threads; its first LOSS_KEEP G logits stay in registers between the
+// three passes (maximum, sum, gradient), the others are read again. exp is taken twice rather than
+// kept: the second is free beside the memory.
+constexpr int LOSS_KEEP = 4;
+
+template <int G>
+__device__ __forceinline__ void loss_group(const LossParams &p, uint32_t r, uint32_t t, float *part) {
+    uint32_t a, b;
+    int32_t gold;
+    float w;
+    if (!loss_request(p, r, a, b, gold, w)) {
         // Nothing of the request is read or written but its loss.
-        if (lane == 0) {
+        if (t == 0) {
             p.loss[r] = 0.0f;
             dev_fail(JC_DEV_BAD_INDEX);
         }
         return;
     }
-    float top = -INFINITY;
-    for (int64_t i = a + lane; i < b; i += 32) top = fmaxf(top, p.logits[i]);
+    float v[LOSS_KEEP], top = -INFINITY;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int k = 0; k < LOSS_KEEP; k++) v[k] = b - a > k * G + t ? p.logits[a + k * G + t] : -INFINITY;
+    const float right = gold >= 0 ? p.logits[a + gold] : 0.0f;
+#pragma unroll
+    for (int k = 0; k < LOSS_KEEP; k++) top = fmaxf(top, v[k]);
+    for (uint32_t i = LOSS_KEEP * G + t; i < b - a; i += G) top = fmaxf(top, p.logits[a + i]);
+    top = loss_max<G>(top, part);
     if (top == -INFINITY) top = 0.0f;
     float sum = 0.0f;
-    for (int64_t i = a + lane; i < b; i += 32) sum += expf(p.logits[i] - top);
-    sum = warp_sum(sum);
-    if (gold < 0 || w == 0.0f || sum == 0.0f) {
-        gold = -1;
-        w = 0.0f;
-    }
-    if (lane == 0) p.loss[r] = w == 0.0f ? 0.0f : w * (top + logf(sum) - p.logits[a + gold]);
+#pragma unroll
+    for (int k = 0; k < LOSS_KEEP; k++) sum += expf(v[k] - top);
+    for (uint32_t i = LOSS_KEEP * G + t; i < b - a; i += G) sum += expf(p.logits[a + i] - top);
+    sum = loss_sum<G>(sum, part);
+    const bool counts = gold >= 0 && w != 0.0f && sum != 0.0f;
+    if (t == 0) p.loss[r] = counts ? w * (top + logf(sum) - right) : 0.0f;
     if (!p.dlogits) return;
-    const float inv = w == 0.0f ? 0.0f : 1.0f / sum;
-    for (int64_t i = a + lane; i < b; i += 32)
-        p.dlogits[i] = w == 0.0f ? 0.0f
-                                 : w * (expf(p.logits[i] - top) * inv - (i == a + gold ? 1.0f : 0.0f));
+    const float inv = 1.0f / sum;
+    auto grad = [&](uint32_t i, float l) {
+        p.dlogits[a + i] = counts ? w * (expf(l - top) * inv - (i == (uint32_t)gold ? 1.0f : 0.0f)) : 0.0f;
+    };
+#pragma unroll
+    for (int k = 0; k < LOSS_KEEP; k++)
+        if (b - a > k * G + t) grad(k * G + t, v[k]);
+    for (uint32_t i = LOSS_KEEP * G + t; i < b - a; i += G) grad(i, p.logits[a + i]);
+}
+
+// G 32: four requests a block; G 256: one.
+template <int G>
+__global__ void __launch_bounds__(G < 128 ? 128 : G) loss_group_kernel(const LossParams p) {
+    constexpr int PER = G < 128 ? 128 / G : 1;
+    __shared__ float part[G / 32];
+    dev_err_bind(p.err);
+    pdl_wait();
+    pdl_launch_dependents();
+    const uint32_t r = blockIdx.x * PER + threadIdx.x / G;
+    if (r < p.requests) loss_group<G>(p, r, threadIdx.x % G, part);
+}
+
+// Requests of a few markers: a block takes LOSS_BLOCK consecutive requests, whose logits lie together
+// whatever their lengths, and moves them through shared memory in whole lines; a thread works on a
+// request there. A block whose logits do not fit (a long request among short ones) or lie out of
+// order takes them a warp at a time instead.
+constexpr int LOSS_BLOCK = 128, LOSS_SMEM = 4096;
+
+__global__ void __launch_bounds__(LOSS_BLOCK) loss_short_kernel(const LossParams p) {
+    __shared__ float s[LOSS_SMEM];
+    __shared__ uint32_t ends[2];
+    dev_err_bind(p.err);
+    pdl_wait();
+    pdl_launch_dependents();
+    const uint32_t r0 = blockIdx.x * LOSS_BLOCK, n = min((uint32_t)LOSS_BLOCK, p.requests - r0), t = threadIdx.x;
+    uint32_t a = 0, b = 0;
+    int32_t gold = -1;
+    float w = 0.0f;
+    const bool ok = t >= n || loss_request(p, r0 + t, a, b, gold, w);
+    if (t == 0) ends[0] = a;
+    if (t == n - 1) ends[1] = b;
+    __syncthreads();
+    const uint32_t lo = ends[0], hi = ends[1];
+    const bool inside = t >= n || (a >= lo && b <= hi);
+    if (!__syncthreads_and(ok && inside && hi >= lo && hi - lo <= LOSS_SMEM)) {
+        for (uint32_t k = t / 32; k < n; k += LOSS_BLOCK / 32) loss_group<32>(p, r0 + k, t & 31, nullptr);
+        return;
+    }
+    for (uint32_t i = t; i < hi - lo; i += LOSS_BLOCK) s[i] = p.logits[lo + i];
+    __syncthreads();
+    if (t < n) {
+        float *l = s + (a - lo);
+        const uint32_t len = b - a;
+        float top = -INFINITY, sum = 0.0f;
+        for (uint32_t i = 0; i < len; i++) top = fmaxf(top, l[i]);
+        if (top == -INFINITY) top = 0.0f;
+        const float right = gold >= 0 ? l[gold] : 0.0f;
+        for (uint32_t i = 0; i < len; i++) {
+            l[i] = expf(l[i] - top);
+            sum += l[i];
+        }
+        const bool counts = gold >= 0 && w != 0.0f && sum != 0.0f;
+        p.loss[r0 + t] = counts ? w * (top + logf(sum) - right) : 0.0f;
+        const float f = counts ? w / sum : 0.0f;
+        for (uint32_t i = 0; i < len; i++) l[i] = counts ? l[i] * f : 0.0f;
+        if (counts) l[gold] -= w;
+    }
+    if (!p.dlogits) return;
+    __syncthreads();
+    for (uint32_t i = t; i < hi - lo; i += LOSS_BLOCK) p.dlogits[lo + i] = s[i];
 }
 
 }  // namespace jc

@@ -6,11 +6,21 @@
 //             dx = rstd (u - sum(u) / d - xh sum(u xh) / d) [+ add]
 //             dgamma = sum over rows of dy xh, dbeta = sum over rows of dy
 //
-// A row is held by G threads, E of its elements in each thread's registers as f32 (G x E >= d), so
-// it is read once: the mean is known before the squared deviations are summed, from the same
-// registers. Thread t of the row's group holds chunks t, t + G, ... of V elements (16 bytes, or one
-// element where the rows are not 16-byte aligned).
+// Both are bound by memory: each row is read once, held by G threads with E of its elements in each
+// one's registers as f32, so the mean is known before the squared deviations are summed, from the
+// same registers; the next row is requested before the current one is worked on. Blocks stay and
+// walk rows, with gamma and beta in shared memory.
+//
+// Rows are read in 16-byte chunks whatever their width: a row that starts `shift` elements into a
+// 16-byte chunk is worked on as the chunks that cover it, the first and last element by element.
+// Rows P apart start alike (P: elements in 16 bytes; 1 when every row starts on a boundary), so
+// block b takes rows that are b modulo P and one shifted copy of gamma and beta serves it. Tensors
+// whose rows start differently from each other are read element by element (V = 1).
 #pragma once
+#include <string.h>
+
+#include <type_traits>
+
 #include "common.cuh"
 #include "elem.cuh"
 
@@ -18,35 +28,112 @@ namespace jc {
 
 constexpr int NORM_MAX_D = 16384;
 
-// Sum over the G threads of a row's group (G 32: a warp; else the whole block), in a fixed order.
-// `part`: one float a warp in shared memory; every thread of the block calls it.
+// Threads of a block whose rows take G threads each. Backward: as many as the registers of a row's
+// four f32 copies (x, dy and the two sums) and the next row's raw elements allow on one SM.
 template <int G>
-__device__ __forceinline__ float norm_sum(float v, float *part) {
-    v = warp_sum(v);
-    if constexpr (G > 32) {
-        const uint32_t warp = threadIdx.x >> 5;
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) part[warp] = v;
-        __syncthreads();
-        v = 0.0f;
+constexpr int NORM_BLOCK = G > 128 ? G : 128;
+template <class T, int V, int G, int E>
+constexpr int NORM_BWD_BLOCK = G > 256 ? G : sizeof(T) == 2 && V > 1 && E <= 24 ? 384 : 256;
+
+// Sums of a and b over the G threads of a row's group, in a fixed order. `part`: two floats a warp in
+// shared memory; G > 32: every thread of the block calls it.
+template <int G>
+__device__ __forceinline__ void norm_sum2(float &a, float &b, float2 *part) {
 #pragma unroll
-        for (int w = 0; w < G / 32; w++) v += part[w];
+    for (int o = 16; o > 0; o >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, o);
+        b += __shfl_xor_sync(0xffffffffu, b, o);
     }
-    return v;
+    if constexpr (G > 32) {
+        const uint32_t warp = threadIdx.x >> 5, first = warp / (G / 32) * (G / 32);
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) part[warp] = make_float2(a, b);
+        __syncthreads();
+        a = b = 0.0f;
+#pragma unroll
+        for (int w = 0; w < G / 32; w++) {
+            a += part[first + w].x;
+            b += part[first + w].y;
+        }
+    }
 }
 
-// This thread's elements of a row; places past d are 0.
+// Thread t's share of a row of d elements that starts `shift` elements into its first chunk: chunk c
+// holds elements first(c) .. first(c) + V.
 template <class T, int V, int G, int E>
-__device__ __forceinline__ void norm_load(const T *row, uint32_t t, uint32_t d, float *v) {
+struct NormRow {
+    static constexpr int N = E / V;
+    using Raw = std::conditional_t<V == 1, T, uint4>;
+    uint32_t t, shift, d;
+    __device__ __forceinline__ uint32_t place(int c) const { return (c * G + t) * V; }
+    __device__ __forceinline__ int first(int c) const { return (int)place(c) - (int)shift; }
+    __device__ __forceinline__ bool whole(int c) const {
+        return V == 1 ? place(c) < d : first(c) >= 0 && first(c) + V <= (int)d;
+    }
+    __device__ __forceinline__ bool some(int c) const {
+        return V == 1 ? place(c) < d : first(c) + V > 0 && first(c) < (int)d;
+    }
+    __device__ __forceinline__ bool has(int c, int i) const {
+        return (uint32_t)(first(c) + i) < d;  // below 0 wraps past d
+    }
+    // Requests the row; places outside it are 0.
+    __device__ __forceinline__ void load(const T *row, Raw *q) const {
 #pragma unroll
-    for (int c = 0; c < E / V; c++) {
-        const uint32_t j = (c * G + t) * V;
-        if (j < d) {
-            Elem<T, V>::load(row + j, v + c * V);
-        } else {
+        for (int c = 0; c < N; c++) {
+            if constexpr (V == 1) {
+                q[c] = whole(c) ? row[place(c)] : T(0.0f);
+            } else {
+                q[c] = make_uint4(0, 0, 0, 0);
+                if (whole(c)) {
+                    q[c] = *reinterpret_cast<const uint4 *>(row + first(c));
+                } else if (some(c)) {
+                    T e[V];
 #pragma unroll
-            for (int i = 0; i < V; i++) v[c * V + i] = 0.0f;
+                    for (int i = 0; i < V; i++) e[i] = has(c, i) ? row[first(c) + i] : T(0.0f);
+                    memcpy(&q[c], e, 16);
+                }
+            }
         }
+    }
+    static __device__ __forceinline__ void unpack(const Raw &q, float *v) {
+        if constexpr (V == 1)
+            v[0] = static_cast<float>(q);
+        else
+            Elem<T, V>::load(reinterpret_cast<const T *>(&q), v);
+    }
+    __device__ __forceinline__ void store(T *row, int c, const float *v) const {
+        if (whole(c)) {
+            Elem<T, V>::store(row + first(c), v);
+        } else if (V > 1 && some(c)) {
+#pragma unroll
+            for (int i = 0; i < V; i++)
+                if (has(c, i)) row[first(c) + i] = static_cast<T>(v[i]);
+        }
+    }
+};
+
+// gamma or beta in shared memory at the places the rows' elements have, 0 outside the row. Eight a
+// chunk are kept as two arrays of four, so that a warp's 16-byte reads are free of bank conflicts.
+template <int V, int G, int E>
+__device__ __forceinline__ uint32_t norm_param_at(uint32_t place) {
+    if constexpr (V == 8) return (place & 4) / 4 * (G * E / 2) + place / 8 * 4 + (place & 3);
+    return place;
+}
+
+template <int V, int G, int E>
+__device__ __forceinline__ void norm_stage_param(float *s, const float *g, uint32_t shift, uint32_t d,
+                                                 uint32_t threads) {
+    for (uint32_t k = threadIdx.x; k < (uint32_t)(G * E); k += threads)
+        s[norm_param_at<V, G, E>(k)] = g && k - shift < d ? g[k - shift] : 0.0f;
+}
+
+template <int V, int G, int E>
+__device__ __forceinline__ void norm_param(const float *s, uint32_t place, float *v) {
+    if constexpr (V == 1) {
+        v[0] = s[place];
+    } else {
+        Elem<float, 4>::load(s + norm_param_at<V, G, E>(place), v);
+        if constexpr (V == 8) Elem<float, 4>::load(s + norm_param_at<V, G, E>(place + 4), v + 4);
     }
 }
 
@@ -55,51 +142,82 @@ struct NormParams {
     size_t ldx;
     const float *gamma, *beta;
     float eps;
-    uint32_t rows, d;
+    uint32_t rows, d, period;  // period: P above; gridDim.x is a multiple of it
     void *y;
     size_t ldy;
     float *stats;
 };
 
 template <class T, int V, int G, int E>
-__global__ void __launch_bounds__(G < 128 ? 128 : G) norm_kernel(const NormParams p) {
-    constexpr int THREADS = G < 128 ? 128 : G;
-    __shared__ float part[THREADS / 32];
+__global__ void __launch_bounds__(NORM_BLOCK<G>) norm_kernel(const NormParams p) {
+    constexpr int THREADS = NORM_BLOCK<G>, GROUPS = THREADS / G;
+    using Row = NormRow<T, V, G, E>;
+    __shared__ float2 part[THREADS / 32];
+    extern __shared__ float params[];  // gamma, beta: G x E each
     pdl_wait();
     pdl_launch_dependents();
-    const uint32_t t = threadIdx.x % G;
-    const uint32_t r = blockIdx.x * (THREADS / G) + threadIdx.x / G;
-    if (G == 32 && r >= p.rows) return;  // a whole warp
-    float v[E];
-    norm_load<T, V, G, E>(static_cast<const T *>(p.x) + (size_t)r * p.ldx, t, p.d, v);
-    float s = 0.0f;
+    const uint32_t g = threadIdx.x / G, cls = blockIdx.x % p.period, step = gridDim.x / p.period * GROUPS;
+    const T *x = static_cast<const T *>(p.x);
+    Row row;
+    row.t = threadIdx.x % G;
+    row.d = p.d;
+    row.shift = V == 1 ? 0 : (uint32_t)(reinterpret_cast<uintptr_t>(x + (size_t)cls * p.ldx) % 16 / sizeof(T));
+    // Row i of this group is row cls + i period; a group that is out of rows keeps its block's company.
+    uint32_t i = blockIdx.x / p.period * GROUPS + g;
+    auto at = [&](uint32_t k) { return (uint64_t)cls + (uint64_t)k * p.period; };
+    typename Row::Raw raw[Row::N];
+    if (at(i) < p.rows) row.load(x + at(i) * p.ldx, raw);
+    float *gs = params, *bs = params + G * E;
+    norm_stage_param<V, G, E>(gs, p.gamma, row.shift, p.d, THREADS);
+    norm_stage_param<V, G, E>(bs, p.beta, row.shift, p.d, THREADS);
+    __syncthreads();
+    const float inv_d = 1.0f / (float)p.d;
+    for (uint32_t k = blockIdx.x / p.period * GROUPS; at(k) < p.rows; k += step, i += step) {
+        const bool mine = at(i) < p.rows;
+        if (G == 32 && !mine) break;  // a warp by itself
+        float v[E];
+        float s = 0.0f, none = 0.0f;
 #pragma unroll
-    for (int i = 0; i < E; i++) s += v[i];
-    const float mean = norm_sum<G>(s, part) / (float)p.d;
-    s = 0.0f;
+        for (int c = 0; c < Row::N; c++) {
+            Row::unpack(raw[c], v + c * V);
 #pragma unroll
-    for (int c = 0; c < E / V; c++)
-        if ((c * G + t) * V < p.d)
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                const float u = v[c * V + i] - mean;
-                s = fmaf(u, u, s);
-            }
-    const float rstd = rsqrtf(norm_sum<G>(s, part) / (float)p.d + p.eps);
-    T *out = static_cast<T *>(p.y) + (size_t)r * p.ldy;
-#pragma unroll
-    for (int c = 0; c < E / V; c++) {
-        const uint32_t j = (c * G + t) * V;
-        if (j >= p.d) continue;
-        float o[V];
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            o[i] = (v[c * V + i] - mean) * rstd * __ldg(p.gamma + j + i);
-            if (p.beta) o[i] += __ldg(p.beta + j + i);
+            for (int e = 0; e < V; e++) s += v[c * V + e];
         }
-        Elem<T, V>::store(out + j, o);
+        if (at(i + step) < p.rows) row.load(x + at(i + step) * p.ldx, raw);
+        norm_sum2<G>(s, none, part);
+        const float mean = s * inv_d;
+        s = 0.0f;
+#pragma unroll
+        for (int c = 0; c < Row::N; c++) {
+            if (row.whole(c)) {
+#pragma unroll
+                for (int e = 0; e < V; e++) {
+                    const float u = v[c * V + e] - mean;
+                    s = fmaf(u, u, s);
+                }
+            } else if (V > 1 && row.some(c)) {
+#pragma unroll
+                for (int e = 0; e < V; e++) {
+                    const float u = row.has(c, e) ? v[c * V + e] - mean : 0.0f;
+                    s = fmaf(u, u, s);
+                }
+            }
+        }
+        norm_sum2<G>(s, none, part);
+        const float rstd = rsqrtf(s * inv_d + p.eps);
+        if (!mine) continue;
+        T *out = static_cast<T *>(p.y) + at(i) * p.ldy;
+#pragma unroll
+        for (int c = 0; c < Row::N; c++) {
+            float ga[V], be[V];
+            norm_param<V, G, E>(gs, row.place(c), ga);
+            norm_param<V, G, E>(bs, row.place(c), be);
+#pragma unroll
+            for (int e = 0; e < V; e++) v[c * V + e] = fmaf((v[c * V + e] - mean) * rstd, ga[e], be[e]);
+            row.store(out, c, v + c * V);
+        }
+        if (p.stats && row.t == 0) *reinterpret_cast<float2 *>(p.stats + 2 * at(i)) = make_float2(mean, rstd);
     }
-    if (p.stats && t == 0) *reinterpret_cast<float2 *>(p.stats + 2 * (size_t)r) = make_float2(mean, rstd);
 }
 
 struct NormBwdParams {
@@ -110,92 +228,125 @@ struct NormBwdParams {
     const float *gamma, *stats;
     const void *add;
     size_t ldadd;
-    uint32_t rows, d;
+    uint32_t rows, d, period;
     void *dx;
     size_t lddx;
     float *ws;  // [gridDim.x][2][d]: each block's sums for dgamma and dbeta (nullptr: neither is wanted)
 };
 
+// A block's groups keep their sums for dgamma and dbeta in registers over all their rows and add them
+// up in shared memory once, group after group; one row of sums a block goes to ws.
 template <class T, int V, int G, int E>
-__global__ void __launch_bounds__(G < 128 ? 128 : G) norm_bwd_kernel(const NormBwdParams p) {
-    constexpr int THREADS = G < 128 ? 128 : G, ROWS = THREADS / G;
-    __shared__ float part[THREADS / 32];
-    extern __shared__ float sums[];  // [2][d], for blocks that hold several rows
+__global__ void __launch_bounds__(NORM_BWD_BLOCK<T, V, G, E>, 1) norm_bwd_kernel(const NormBwdParams p) {
+    constexpr int THREADS = NORM_BWD_BLOCK<T, V, G, E>, GROUPS = THREADS / G;
+    using Row = NormRow<T, V, G, E>;
+    __shared__ float2 part[THREADS / 32];
+    extern __shared__ float smem[];  // gamma [G E], then the groups' sums [GROUPS][2][G E]
     pdl_wait();
     pdl_launch_dependents();
-    const uint32_t t = threadIdx.x % G, g = threadIdx.x / G;
+    const uint32_t g = threadIdx.x / G, cls = blockIdx.x % p.period, step = gridDim.x / p.period * GROUPS;
+    const T *x = static_cast<const T *>(p.x), *dy = static_cast<const T *>(p.dy);
+    Row row;
+    row.t = threadIdx.x % G;
+    row.d = p.d;
+    row.shift = V == 1 ? 0 : (uint32_t)(reinterpret_cast<uintptr_t>(x + (size_t)cls * p.ldx) % 16 / sizeof(T));
+    uint32_t i = blockIdx.x / p.period * GROUPS + g;
+    auto at = [&](uint32_t k) { return (uint64_t)cls + (uint64_t)k * p.period; };
+    typename Row::Raw rx[Row::N], rdy[Row::N], radd[Row::N];
+    float2 st = make_float2(0.0f, 0.0f);
+    auto fetch = [&](uint64_t r) {
+        row.load(x + r * p.ldx, rx);
+        row.load(dy + r * p.lddy, rdy);
+        st = *reinterpret_cast<const float2 *>(p.stats + 2 * r);
+    };
+    if (at(i) < p.rows) fetch(at(i));
+    norm_stage_param<V, G, E>(smem, p.gamma, row.shift, p.d, THREADS);
+    __syncthreads();
     float dg[E], db[E];
 #pragma unroll
-    for (int i = 0; i < E; i++) dg[i] = db[i] = 0.0f;
+    for (int e = 0; e < E; e++) dg[e] = db[e] = 0.0f;
     const float inv_d = 1.0f / (float)p.d;
-    for (uint32_t r = blockIdx.x * ROWS + g; r < p.rows; r += gridDim.x * ROWS) {
-        float x[E], dy[E];
-        norm_load<T, V, G, E>(static_cast<const T *>(p.x) + (size_t)r * p.ldx, t, p.d, x);
-        norm_load<T, V, G, E>(static_cast<const T *>(p.dy) + (size_t)r * p.lddy, t, p.d, dy);
-        const float2 st = *reinterpret_cast<const float2 *>(p.stats + 2 * (size_t)r);
+    for (uint32_t k = blockIdx.x / p.period * GROUPS; at(k) < p.rows; k += step, i += step) {
+        const bool mine = at(i) < p.rows;
+        if (G == 32 && !mine) break;  // a warp by itself
+        const uint64_t r = at(i);
+        const float mean = st.x, rstd = st.y;
+        float xh[E], u[E];
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-        for (int c = 0; c < E / V; c++) {
-            const uint32_t j = (c * G + t) * V;
-            if (j >= p.d) continue;
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                const int e = c * V + i;
-                const float xh = (x[e] - st.x) * st.y, u = dy[e] * __ldg(p.gamma + j + i);
-                s1 += u;
-                s2 = fmaf(u, xh, s2);
-                dg[e] = fmaf(dy[e], xh, dg[e]);
-                db[e] += dy[e];
-                x[e] = xh;
-                dy[e] = u;
-            }
+        for (int c = 0; c < Row::N; c++) {
+            Row::unpack(rx[c], xh + c * V);
+            Row::unpack(rdy[c], u + c * V);
         }
-        s1 = norm_sum<G>(s1, part) * inv_d;
-        s2 = norm_sum<G>(s2, part) * inv_d;
+        if (mine && p.add) row.load(static_cast<const T *>(p.add) + r * p.ldadd, radd);
+        if (at(i + step) < p.rows) fetch(at(i + step));
+        if (mine) {
 #pragma unroll
-        for (int c = 0; c < E / V; c++) {
-            const uint32_t j = (c * G + t) * V;
-            if (j >= p.d) continue;
-            float o[V];
+            for (int c = 0; c < Row::N; c++) {
+                float ga[V];
+                norm_param<V, G, E>(smem, row.place(c), ga);
 #pragma unroll
-            for (int i = 0; i < V; i++) o[i] = st.y * (dy[c * V + i] - s1 - x[c * V + i] * s2);
-            if (p.add) {
-                float a[V];
-                Elem<T, V>::load(static_cast<const T *>(p.add) + (size_t)r * p.ldadd + j, a);
-#pragma unroll
-                for (int i = 0; i < V; i++) o[i] += a[i];
-            }
-            Elem<T, V>::store(static_cast<T *>(p.dx) + (size_t)r * p.lddx + j, o);
-        }
-    }
-    if (!p.ws) return;
-    // The block's rows meet in shared memory, group after group, so the order of the sums is fixed.
-    float *out = p.ws + (size_t)blockIdx.x * 2 * p.d;
-#pragma unroll 1
-    for (uint32_t k = 0; k < (uint32_t)ROWS; k++) {
-        if (g == k) {
-#pragma unroll
-            for (int c = 0; c < E / V; c++) {
-                const uint32_t j = (c * G + t) * V;
-                if (j >= p.d) continue;
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    float a = dg[c * V + i], b = db[c * V + i];
-                    if (k > 0) {
-                        a += sums[j + i];
-                        b += sums[p.d + j + i];
-                    }
-                    if (k + 1 < (uint32_t)ROWS) {
-                        sums[j + i] = a;
-                        sums[p.d + j + i] = b;
-                    } else {
-                        out[j + i] = a;
-                        out[p.d + j + i] = b;
-                    }
+                for (int e = 0; e < V; e++) {
+                    // Outside the row dy and gamma are 0: nothing is added there.
+                    const int j = c * V + e;
+                    xh[j] = (xh[j] - mean) * rstd;
+                    dg[j] = fmaf(u[j], xh[j], dg[j]);
+                    db[j] += u[j];
+                    u[j] *= ga[e];
+                    s1 += u[j];
+                    s2 = fmaf(u[j], xh[j], s2);
                 }
             }
         }
-        if (ROWS > 1) __syncthreads();
+        norm_sum2<G>(s1, s2, part);
+        if (!mine) continue;
+        s1 *= inv_d;
+        s2 *= inv_d;
+        T *out = static_cast<T *>(p.dx) + r * p.lddx;
+#pragma unroll
+        for (int c = 0; c < Row::N; c++) {
+            float o[V];
+#pragma unroll
+            for (int e = 0; e < V; e++) o[e] = rstd * (u[c * V + e] - s1 - xh[c * V + e] * s2);
+            if (p.add) {
+                float a[V];
+                Row::unpack(radd[c], a);
+#pragma unroll
+                for (int e = 0; e < V; e++) o[e] += a[e];
+            }
+            row.store(out, c, o);
+        }
+    }
+    if (!p.ws) return;
+    // Every group's sums into shared memory (chunk order, conflict-free), then one thread a column.
+    float *sums = smem + G * E;
+#pragma unroll
+    for (int c = 0; c < Row::N; c++) {
+        float *a = sums + (size_t)g * 2 * G * E, *b = a + G * E;
+        if constexpr (V == 1) {
+            a[row.place(c)] = dg[c];
+            b[row.place(c)] = db[c];
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; e += 4) {
+                const uint32_t at4 = norm_param_at<V, G, E>(row.place(c) + e);
+                Elem<float, 4>::store(a + at4, dg + c * V + e);
+                Elem<float, 4>::store(b + at4, db + c * V + e);
+            }
+        }
+    }
+    __syncthreads();
+    float *out = p.ws + (size_t)blockIdx.x * 2 * p.d;
+    for (uint32_t j = threadIdx.x; j < p.d; j += THREADS) {
+        const uint32_t k = norm_param_at<V, G, E>(j + row.shift);
+        float a = 0.0f, b = 0.0f;
+#pragma unroll 1
+        for (int q = 0; q < GROUPS; q++) {
+            a += sums[(size_t)(2 * q) * G * E + k];
+            b += sums[(size_t)(2 * q + 1) * G * E + k];
+        }
+        out[j] = a;
+        out[p.d + j] = b;
     }
 }
 

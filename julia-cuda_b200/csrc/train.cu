@@ -4,7 +4,9 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <string>
+#include <utility>
 
 #include "adamw.cuh"
 #include "launch.h"
@@ -40,7 +42,7 @@ template <int N>
 using Int = std::integral_constant<int, N>;
 
 // The group that holds a row of d elements: the smallest G x E that does (a warp up to 1024, so
-// that no reduction crosses warps, then four warps, then sixteen).
+// that no reduction crosses warps, then four to sixteen).
 template <class F>
 static bool with_group(uint32_t d, F &&f) {
     if (d <= 256) return f(Int<32>(), Int<8>());
@@ -49,31 +51,78 @@ static bool with_group(uint32_t d, F &&f) {
     if (d <= 1024) return f(Int<32>(), Int<32>());
     if (d <= 2048) return f(Int<128>(), Int<16>());
     if (d <= 4096) return f(Int<128>(), Int<32>());
+    if (d <= 8192) return f(Int<256>(), Int<32>());
     return f(Int<512>(), Int<32>());
+}
+
+// How a layer norm's tensors are read. All rows that start alike (the same remainder by 16 bytes in
+// every tensor, row for row) are read in 16-byte chunks; the others element by element.
+struct NormLayout {
+    bool chunks = true;
+    uint32_t period = 1;  // rows this far apart start alike
+    uint32_t span;        // the elements a row's chunks hold
+};
+
+static NormLayout norm_layout(uint32_t d, size_t size, std::initializer_list<std::pair<const void *, size_t>> ts) {
+    NormLayout l;
+    const uint32_t v = (uint32_t)(16 / size);
+    const auto [p0, ld0] = *ts.begin();
+    bool aligned = true;
+    for (const auto &[p, ld] : ts) {
+        if (!p) continue;
+        if ((reinterpret_cast<uintptr_t>(p) - reinterpret_cast<uintptr_t>(p0)) % 16 || (ld - ld0) * size % 16) l.chunks = false;
+        if (!aligned16(p, ld, size)) aligned = false;
+    }
+    l.period = l.chunks && !aligned ? v : 1;
+    l.span = l.period > 1 ? d + v - 1 : d;
+    if (l.span > NORM_MAX_D) {
+        l.chunks = false;
+        l.period = 1;
+        l.span = d;
+    }
+    return l;
+}
+
+// A multiple of `period` blocks, enough for `groups` rows each but no more than `most`.
+static uint32_t norm_blocks(uint32_t rows, uint32_t groups, uint32_t period, uint32_t most) {
+    const uint32_t per = (rows + period - 1) / period;  // rows of a class
+    return std::min((per + groups - 1) / groups, most / period) * period;
 }
 
 bool launch_norm(const NormArgs &a, cudaStream_t s) {
     if (a.rows == 0) return true;
     return with_type(a.type, [&](auto t) {
         using T = decltype(t);
-        const bool vec = a.d % VEC<T> == 0 && aligned16(a.x, a.ldx, sizeof(T)) && aligned16(a.y, a.ldy, sizeof(T));
-        return with_group(a.d, [&](auto g, auto e) {
-            constexpr int G = g, E = e, ROWS = G < 128 ? 128 / G : 1;
-            const NormParams p{a.x, a.ldx, a.gamma, a.beta, a.eps, a.rows, a.d, a.y, a.ldy, a.stats};
-            const dim3 grid((a.rows + ROWS - 1) / ROWS), block(G < 128 ? 128 : G);
-            return vec ? launch_ex(norm_kernel<T, VEC<T>, G, E>, grid, block, 0, s, true, "layer_norm", p)
-                       : launch_ex(norm_kernel<T, 1, G, E>, grid, block, 0, s, true, "layer_norm", p);
+        const NormLayout l = norm_layout(a.d, sizeof(T), {{a.x, a.ldx}, {a.y, a.ldy}});
+        return with_group(l.span, [&](auto g, auto e) {
+            constexpr int G = g, E = e, THREADS = NORM_BLOCK<G>;
+            const NormParams p{a.x, a.ldx, a.gamma, a.beta, a.eps, a.rows, a.d, l.period, a.y, a.ldy, a.stats};
+            const int smem = 2 * G * E * (int)sizeof(float);
+            auto go = [&](auto kern, std::atomic<uint64_t> &set, std::atomic<int> &resident) {
+                if (!ensure_smem(kern, smem, set)) return false;
+                int per_sm = resident.load();
+                if (per_sm == 0) {
+                    if (!cuda_ok(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, THREADS, smem), "occupancy"))
+                        return false;
+                    resident.store(per_sm);
+                }
+                const dim3 grid(norm_blocks(a.rows, THREADS / G, l.period, (uint32_t)(sm_count() * per_sm)));
+                return launch_ex(kern, grid, dim3(THREADS), smem, s, true, "layer_norm", p);
+            };
+            static std::atomic<uint64_t> set_v{0}, set_1{0};
+            static std::atomic<int> res_v{0}, res_1{0};
+            return l.chunks ? go(norm_kernel<T, VEC<T>, G, E>, set_v, res_v) : go(norm_kernel<T, 1, G, E>, set_1, res_1);
         });
     });
 }
 
-// Blocks of the backward kernel: each leaves a row of partial sums.
-static uint32_t norm_bwd_blocks(uint32_t rows, uint32_t d) {
-    const uint32_t per = d <= 1024 ? 4 : 1;
-    return std::min((rows + per - 1) / per, 148u * 4);
-}
+// Blocks of the backward kernel at most: one a SM. Each leaves a row of partial sums (up to seven
+// blocks more than rows: a multiple of the period).
+constexpr uint32_t NORM_BWD_BLOCKS = 148;
 
-size_t norm_bwd_ws_floats(uint32_t rows, uint32_t d) { return (size_t)norm_bwd_blocks(rows, d) * 2 * d; }
+size_t norm_bwd_ws_floats(uint32_t rows, uint32_t d) {
+    return rows ? (size_t)std::min(rows + 7, NORM_BWD_BLOCKS) * 2 * d : 0;
+}
 
 static bool launch_column_sum(const float *ws, uint32_t parts, uint32_t n, uint32_t columns, float *a,
                               float *b, cudaStream_t s) {
@@ -83,23 +132,24 @@ static bool launch_column_sum(const float *ws, uint32_t parts, uint32_t n, uint3
 
 bool launch_norm_bwd(const NormBwdArgs &a, cudaStream_t s) {
     const bool sums = a.dgamma || a.dbeta;
-    const uint32_t blocks = norm_bwd_blocks(a.rows, a.d);
+    uint32_t blocks = 0;
     if (a.rows > 0) {
         const bool ok = with_type(a.type, [&](auto t) {
             using T = decltype(t);
-            const bool vec = a.d % VEC<T> == 0 && aligned16(a.x, a.ldx, sizeof(T)) &&
-                             aligned16(a.dy, a.lddy, sizeof(T)) && aligned16(a.dx, a.lddx, sizeof(T)) &&
-                             (!a.add || aligned16(a.add, a.ldadd, sizeof(T)));
-            return with_group(a.d, [&](auto g, auto e) {
+            const NormLayout l = norm_layout(a.d, sizeof(T), {{a.x, a.ldx}, {a.dy, a.lddy}, {a.dx, a.lddx}, {a.add, a.ldadd}});
+            return with_group(l.span, [&](auto g, auto e) {
                 constexpr int G = g, E = e;
                 const NormBwdParams p{a.dy, a.lddy, a.x, a.ldx, a.gamma, a.stats, a.add, a.ldadd, a.rows,
-                                      a.d, a.dx, a.lddx, sums ? a.ws : nullptr};
-                const dim3 block(G < 128 ? 128 : G);
-                const size_t smem = G == 32 ? 2 * (size_t)a.d * sizeof(float) : 0;
-                return vec ? launch_ex(norm_bwd_kernel<T, VEC<T>, G, E>, dim3(blocks), block, smem, s, true,
-                                       "layer_norm_backward", p)
-                           : launch_ex(norm_bwd_kernel<T, 1, G, E>, dim3(blocks), block, smem, s, true,
-                                       "layer_norm_backward", p);
+                                      a.d, l.period, a.dx, a.lddx, sums ? a.ws : nullptr};
+                auto go = [&](auto kern, std::atomic<uint64_t> &set, int threads) {
+                    const int groups = threads / G, smem = (1 + 2 * groups) * G * E * (int)sizeof(float);
+                    blocks = norm_blocks(a.rows, groups, l.period, NORM_BWD_BLOCKS);
+                    return ensure_smem(kern, smem, set) &&
+                           launch_ex(kern, dim3(blocks), dim3(threads), smem, s, true, "layer_norm_backward", p);
+                };
+                static std::atomic<uint64_t> set_v{0}, set_1{0};
+                return l.chunks ? go(norm_bwd_kernel<T, VEC<T>, G, E>, set_v, NORM_BWD_BLOCK<T, VEC<T>, G, E>)
+                                : go(norm_bwd_kernel<T, 1, G, E>, set_1, NORM_BWD_BLOCK<T, 1, G, E>);
             });
         });
         if (!ok) return false;
@@ -379,12 +429,20 @@ bool launch_linear_bwd(const LinearBwdArgs &a, cudaStream_t s) {
 // ---------------------------------------------------------------------------------------------
 // loss and optimizer
 
+// Requests of up to this many logits on average go a thread each.
+constexpr uint32_t LOSS_SHORT = 24;
+
 bool launch_choice_loss(const LossArgs &a, cudaStream_t s) {
     if (a.requests == 0) return true;
     unsigned int *err = module_error_word();
     if (!err) return false;
     const LossParams p{a.logits, a.n_logits, a.offsets, a.gold, a.weight, a.requests, a.loss, a.dlogits, err};
-    return launch_ex(choice_loss_kernel, dim3((a.requests + 3) / 4), dim3(128), 0, s, true, "choice_loss", p);
+    const uint32_t mean = a.n_logits / a.requests;
+    if (mean <= LOSS_SHORT)
+        return launch_ex(loss_short_kernel, dim3((a.requests + LOSS_BLOCK - 1) / LOSS_BLOCK), dim3(LOSS_BLOCK), 0, s, true,
+                         "choice_loss", p);
+    if (mean <= 512) return launch_ex(loss_group_kernel<32>, dim3((a.requests + 3) / 4), dim3(128), 0, s, true, "choice_loss", p);
+    return launch_ex(loss_group_kernel<256>, dim3(a.requests), dim3(256), 0, s, true, "choice_loss", p);
 }
 
 bool launch_adamw(const AdamwStep &a, cudaStream_t s) {

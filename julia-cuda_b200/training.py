@@ -25,9 +25,11 @@ def _matrix(op: str, name: str, t, rows: int, cols: int, dtype):
     None."""
     if t is None:
         return None, 0
-    if t.dtype is not dtype or tuple(t.shape) != (rows, cols) or not t.is_cuda:
+    if t.dtype is not dtype or t.shape != (rows, cols) or not t.is_cuda:
         _fail(f"{op}: {name} must be a [{rows}, {cols}] device tensor of {dtype}, "
               f"not {list(t.shape)} of {t.dtype}")
+    if t.is_contiguous():
+        return t.data_ptr(), cols
     sr, sc = t.stride()
     if (cols > 1 and sc != 1) or (rows > 1 and sr < cols):
         _fail(f"{op}: {name} must have contiguous rows that do not overlap")
@@ -47,7 +49,7 @@ def _type(op: str, t, halves: bool = False) -> int:
     if code is None or t.dim() != 2 or (halves and code == F32):
         _fail(f"{op}: x must be a matrix of float16{', ' if not halves else ' or '}bfloat16"
               f"{'' if halves else ' or float32'}")
-    if t.device.index != torch.cuda.current_device():
+    if t.get_device() != torch.cuda.current_device():
         _fail(f"{op}: the tensors are not on the current device")
     return code
 
@@ -154,7 +156,7 @@ def choice_loss(logits, offsets, gold, loss, dlogits=None, weight=None, stream=N
     none), weight f32 [requests]; writes loss [requests] and dlogits (as logits)."""
     op = "choice_loss"
     n, r = logits.numel(), gold.numel()
-    if logits.is_cuda and logits.device.index != torch.cuda.current_device():
+    if logits.get_device() != torch.cuda.current_device():
         _fail(f"{op}: the tensors are not on the current device")
     _check(lib().jc_choice_loss(_vector(op, "logits", logits, n), n,
                                 _vector(op, "offsets", offsets, r + 1, torch.int32),
