@@ -152,22 +152,6 @@ __device__ __forceinline__ void k_range(uint32_t kb_total, uint32_t z, uint32_t 
     nkb = (z + 1) * kb_total / splits - kb0;
 }
 
-// The shared::cluster address of local shared address `a` in cluster CTA `rank`.
-__device__ __forceinline__ uint32_t map_to_rank(uint32_t a, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
-    return r;
-}
-
-// A barrier across the CTAs of a thread-block cluster (every thread of every CTA) in two halves:
-// arrive (release) early, wait (acquire) when needed.
-__device__ __forceinline__ void cluster_arrive() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_wait() {
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 // Four floats into shared memory of another CTA of the cluster (addr, remote_bar: its
 // shared::cluster addresses), asynchronously: the 16 bytes count towards the transaction bytes of
 // that CTA's mbarrier remote_bar.

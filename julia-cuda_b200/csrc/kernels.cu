@@ -167,7 +167,7 @@ static bool launch_gemm_inst(const GemmKernelParams &p, dim3 grid, cudaStream_t 
     constexpr int smem = Sh::SMEM_BYTES + Sh::template RECV_BYTES<CS>;
     static_assert(smem <= 227 * 1024, "a GEMM CTA's shared memory");
     if (!ensure_smem(kern, smem, smem_set)) return false;
-    return launch_ex_cluster(kern, grid, dim3(GEMM_THREADS), smem, s, pdl, CS, "gemm launch", p);
+    return launch_ex_cluster(kern, grid, dim3(GEMM_THREADS), smem, s, pdl, dim3(1, 1, CS), "gemm launch", p);
 }
 
 template <int BN, int STAGES, int CS, int BM = GEMM_BM>

@@ -41,10 +41,10 @@ bool launch_ex(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaS
     return cuda_ok(cudaLaunchKernelEx(&cfg, kern, args...), what);
 }
 
-// launch_ex with the grid grouped into thread-block clusters of `cluster_z` CTAs along z (1: none).
+// launch_ex with the grid grouped into thread-block clusters.
 template <typename... KArgs, typename... Args>
 bool launch_ex_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
-                       bool pdl, int cluster_z, const char *what, Args... args) {
+                       bool pdl, dim3 cluster, const char *what, Args... args) {
     pdl = pdl && pdl_allowed();
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
@@ -58,16 +58,39 @@ bool launch_ex_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t sme
         attr[n].val.programmaticStreamSerializationAllowed = 1;
         n++;
     }
-    if (cluster_z > 1) {
+    if (cluster.x * cluster.y * cluster.z > 1) {
         attr[n].id = cudaLaunchAttributeClusterDimension;
-        attr[n].val.clusterDim.x = 1;
-        attr[n].val.clusterDim.y = 1;
-        attr[n].val.clusterDim.z = (unsigned)cluster_z;
+        attr[n].val.clusterDim.x = cluster.x;
+        attr[n].val.clusterDim.y = cluster.y;
+        attr[n].val.clusterDim.z = cluster.z;
         n++;
     }
     cfg.attrs = n ? attr : nullptr;
     cfg.numAttrs = n;
     return cuda_ok(cudaLaunchKernelEx(&cfg, kern, args...), what);
+}
+
+// How many clusters of `size` CTAs along x the current device holds at once.
+template <typename K>
+bool max_clusters(K kern, int size, int threads, int smem, int *clusters) {
+    int dev = 0, sms = 0;
+    if (!cuda_ok(cudaGetDevice(&dev), "cudaGetDevice") ||
+        !cuda_ok(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "sm count"))
+        return false;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)size;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)(sms / size * size));
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (!cuda_ok(cudaOccupancyMaxActiveClusters(clusters, kern, &cfg), "cluster occupancy")) return false;
+    if (*clusters > 0) return true;
+    set_error("no cluster of a kernel fits this device");
+    return false;
 }
 
 // Sets a kernel's dynamic shared-memory limit once per device.

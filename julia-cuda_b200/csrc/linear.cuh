@@ -12,11 +12,27 @@
 
 namespace jc {
 
-// act(z) and act'(z); act: 0, JC_EPI_RELU or JC_EPI_GELU (the GELU of the forward GEMMs).
+// z Phi(z) = z / (1 + 2^(-z q(z^2))): q is a polynomial of degree 6 fitted (iteratively reweighted
+// least squares) to log2(Phi(z) / Phi(-z)) / z on |z| <= 5.5, weighted by its effect on the result:
+// within 6.7e-8 everywhere, and Phi's tails keep their relative size. Past 5.5 q stays and the
+// exponent grows with z. Half the instructions of gelu_as, which set the pace of the GELU epilogue.
+__device__ __forceinline__ float gelu_fit(float z) {
+    const float u = fminf(z * z, 30.25f);
+    float q = 5.20991383e-9f;
+    q = fmaf(q, u, -3.85045240e-7f);
+    q = fmaf(q, u, 1.14524337e-5f);
+    q = fmaf(q, u, -1.59389441e-4f);
+    q = fmaf(q, u, -9.55928408e-5f);
+    q = fmaf(q, u, 0.10483858f);
+    q = fmaf(q, u, 2.30220723f);
+    return __fdividef(z, 1.0f + ex2_approx(-z * q));
+}
+
+// act(z) and act'(z); act: 0, JC_EPI_RELU or JC_EPI_GELU.
 template <uint32_t ACT>
 __device__ __forceinline__ float act_fwd(float z) {
     if constexpr (ACT == JC_EPI_RELU) return z < 0.0f ? 0.0f : z;  // a NaN stays one
-    if constexpr (ACT == JC_EPI_GELU) return gelu_as(z);
+    if constexpr (ACT == JC_EPI_GELU) return gelu_fit(z);
     return z;
 }
 
@@ -43,17 +59,57 @@ struct LinearOperand {
     size_t si, sk;
 };
 
-// c [m][n] = the sum of `splits` partial products in ws, in their order.
-template <class T>
-__global__ void __launch_bounds__(256) linear_join_kernel(const float *ws, uint32_t splits, uint32_t m,
-                                                          uint32_t n, T *c, size_t ldc) {
+// The backward pass's last kernel: the first `join_blocks` blocks write c [m][n] = the sum of `splits`
+// partial products in ws, in their order, V columns a thread; the others dbias = the sums of `parts`
+// rows of column sums, 32 columns a block, eight threads a column.
+struct LinearFinishParams {
+    const float *ws;
+    uint32_t splits, m, n, join_blocks;
+    void *c;
+    size_t ldc;
+    const float *part;
+    uint32_t parts, bias_n;
+    float *dbias;
+};
+
+template <class T, int V>
+__global__ void __launch_bounds__(256) linear_finish_kernel(const LinearFinishParams p) {
+    __shared__ float sh[8][32];
     pdl_wait();
     pdl_launch_dependents();
-    const size_t all = (size_t)m * n;
-    for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < all; i += (size_t)gridDim.x * 256) {
+    if (blockIdx.x >= p.join_blocks) {
+        const uint32_t c = threadIdx.x & 31, k = threadIdx.x >> 5, j = (blockIdx.x - p.join_blocks) * 32 + c;
         float v = 0.0f;
-        for (uint32_t s = 0; s < splits; s++) v += ws[s * all + i];
-        c[i / n * ldc + i % n] = static_cast<T>(v);
+        if (j < p.bias_n)
+            for (uint32_t i = k; i < p.parts; i += 8) v += p.part[(size_t)i * p.bias_n + j];
+        sh[k][c] = v;
+        __syncthreads();
+        if (k == 0 && j < p.bias_n) {
+#pragma unroll
+            for (int i = 1; i < 8; i++) v += sh[i][c];
+            p.dbias[j] = v;
+        }
+        return;
+    }
+    const size_t all = (size_t)p.m * p.n;
+    const uint32_t width = p.n / V;
+    for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < all / V; i += (size_t)p.join_blocks * 256) {
+        const uint32_t r = (uint32_t)(i / width), c = (uint32_t)(i % width) * V;
+        float v[V];
+#pragma unroll
+        for (int j = 0; j < V; j++) v[j] = 0.0f;
+#pragma unroll 4
+        for (uint32_t s = 0; s < p.splits; s++) {
+            const float *src = p.ws + s * all + i * V;
+#pragma unroll
+            for (int j = 0; j < V; j += V == 1 ? 1 : 4) {
+                float t[4];
+                Elem<float, V == 1 ? 1 : 4>::load(src + j, t);
+#pragma unroll
+                for (int q = 0; q < (V == 1 ? 1 : 4); q++) v[j + q] += t[q];
+            }
+        }
+        Elem<T, V>::store(static_cast<T *>(p.c) + (size_t)r * p.ldc + c, v);
     }
 }
 

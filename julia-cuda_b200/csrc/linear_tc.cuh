@@ -10,9 +10,12 @@
 // so ("MN-major").
 //
 // Two kernels share the tiles, the epilogue and the roles:
-//   linear_tc_kernel   TMA loads; the operands' rows on 16-byte boundaries. One CTA per SM walks the 128 x BN
+//   linear_tc_kernel   TMA loads; the operands' rows on 16-byte boundaries. One CTA per SM walks the
 //                      tiles; the epilogue of one runs under the main loop of the next (two
-//                      accumulators).
+//                      accumulators). CTAS 2: pairs of CTAs on 256 x BN tiles (cta_group::2), each
+//                      with 128 rows of a and half of the rows of b, for a third fewer operand bytes
+//                      per SM than a 128 x 256 tile: alone, such a tile asks an SM for 48 KB per 512
+//                      tensor cycles, more than the 64 bytes a cycle it can take in.
 //   linear_any_kernel  any strides and alignment: eight warps load elements and write them into the
 //                      same swizzled tiles. One tile a CTA.
 // Both: one warp issues the MMAs, eight run the epilogue.
@@ -31,9 +34,9 @@ constexpr int LT_STAGE_BUF = 4096;  // a warp's staging tile: 32 rows x 128 byte
 
 // The instruction descriptor: umma_idesc_f16 with the operands' type and major axes.
 template <class T>
-__host__ __device__ constexpr uint32_t lt_idesc(int n, bool a_mn, bool b_mn) {
+__host__ __device__ constexpr uint32_t lt_idesc(int m, int n, bool a_mn, bool b_mn) {
     const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-    return umma_idesc_f16(LT_BM, n) | (fmt << 7) | (fmt << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16);
+    return umma_idesc_f16(m, n) | (fmt << 7) | (fmt << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16);
 }
 
 // Shared-memory descriptor of an operand tile at saddr (1024-byte aligned), 128-byte swizzle.
@@ -158,6 +161,34 @@ __device__ __forceinline__ void lt_copy_in(uint8_t *buf, const uint8_t *g, size_
     }
 }
 
+// A chunk's bias: requested early, a lane or two columns each; added by way of the staging buffer (16
+// broadcast reads of 16 bytes). Read from global memory where it is used, each of those reads would
+// wait for the one before it: 3.4 us a tile.
+template <int CW>
+struct LtBias {
+    float v[CW > 32 ? 2 : 1];
+    __device__ __forceinline__ void load(const float *bias, uint32_t c0, uint32_t n) {
+#pragma unroll
+        for (int i = 0; i < (CW > 32 ? 2 : 1); i++) {
+            const uint32_t c = c0 + 32 * i + (threadIdx.x & 31);
+            v[i] = bias && c < n ? __ldg(bias + c) : 0.0f;
+        }
+    }
+    __device__ __forceinline__ void add(uint8_t *buf, float *acc) const {
+        float *s = reinterpret_cast<float *>(buf);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < (CW > 32 ? 2 : 1); i++) s[32 * i + (threadIdx.x & 31)] = v[i];
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < CW; j += 4) {
+            const float4 b = *reinterpret_cast<const float4 *>(s + j);
+            acc[j] += b.x; acc[j + 1] += b.y; acc[j + 2] += b.z; acc[j + 3] += b.w;
+        }
+        __syncwarp();
+    }
+};
+
 // A lane's own row of the buffer, written or read eight elements at a time.
 template <class T, int CW>
 __device__ __forceinline__ void lt_put_row(uint8_t *buf, const float *v) {
@@ -192,11 +223,12 @@ __device__ __forceinline__ void lt_acc(uint32_t taddr, float *v) {
 }
 
 // One warp's share of a finished tile: rows 32 (warp % 4).. and half warp / 4 of the columns. `acc`:
-// the tile's accumulator; `res`: the first chunk's residual where it was requested early (VEC).
+// the tile's accumulator; `bias`, `res`: the first chunk's, requested before the accumulator was ready
+// (the residual only with VEC).
 template <class T, int BN, uint32_t ACT, bool VEC>
 __device__ __forceinline__ void lt_epilogue(const LinearTcParams &p, uint32_t acc, uint8_t *buf, uint32_t warp,
                                             uint32_t m0, uint32_t n0, uint32_t split,
-                                            LtRes<LtShape<BN>::CW> &res) {
+                                            LtBias<LtShape<BN>::CW> &bias, LtRes<LtShape<BN>::CW> &res) {
     using S = LtShape<BN>;
     constexpr int CW = S::CW;
     if (warp / 4 >= (uint32_t)S::HALVES) return;
@@ -225,9 +257,8 @@ __device__ __forceinline__ void lt_epilogue(const LinearTcParams &p, uint32_t ac
             continue;
         }
         if (p.bias) {
-#pragma unroll
-            for (int j = 0; j < CW; j++)
-                if (VEC || c0 + j < p.n) v[j] += __ldg(p.bias + min(c0 + j, p.n - 1));
+            bias.add(buf, v);
+            if (ch + 1 < S::CHUNKS) bias.load(p.bias, c0 + CW, p.n);
         }
         if (p.z) {
             __syncwarp();
@@ -243,8 +274,9 @@ __device__ __forceinline__ void lt_epilogue(const LinearTcParams &p, uint32_t ac
             const uint8_t *g = static_cast<const uint8_t *>(p.res);
             __syncwarp();
             if constexpr (VEC) {
-                if (ch > 0) res.load(g, p.ldres, r0, c0, p.m, p.n);
+                // This chunk's residual into the buffer, the next one's requested.
                 res.stage(buf);
+                if (ch + 1 < S::CHUNKS) res.load(g, p.ldres, r0, c0 + CW, p.m, p.n);
             } else {
                 lt_copy_in<CW>(buf, g, p.ldres, r0, c0, p.m, p.n);
             }
@@ -261,57 +293,72 @@ __device__ __forceinline__ void lt_epilogue(const LinearTcParams &p, uint32_t ac
 // ---------------------------------------------------------------------------------------------
 // TMA kernel
 
-// An operand's tile of one stage: rows [row0, row0 + ROWS) x the 64 contracted from k0.
-template <int ROWS, bool MN>
-__device__ __forceinline__ void lt_tma(uint8_t *dst, const CUtensorMap *map, uint64_t *bar, uint32_t row0,
-                                       uint32_t k0) {
-    if constexpr (MN) {
+// An operand's tile of one stage: rows [row0, row0 + ROWS) x the 64 contracted from k0. CTAS 2: `bar`
+// is the leader's barrier.
+template <int CTAS, int ROWS, bool MN>
+__device__ __forceinline__ void lt_tma(uint8_t *dst, const CUtensorMap *map, uint64_t *bar, uint32_t leader_bar,
+                                       uint32_t row0, uint32_t k0) {
 #pragma unroll
-        for (int j = 0; j < ROWS / 64; j++)
-            tma_load_2d(dst + j * 8192, map, bar, (int32_t)(row0 + 64 * j), (int32_t)k0);
-    } else {
-        tma_load_2d(dst, map, bar, (int32_t)k0, (int32_t)row0);
+    for (int j = 0; j < (MN ? ROWS / 64 : 1); j++) {
+        const int32_t x = (int32_t)(MN ? row0 + 64 * j : k0), y = (int32_t)(MN ? k0 : row0);
+        if constexpr (CTAS == 2)
+            tma_load_2d_pair(dst + j * 8192, map, leader_bar, x, y);
+        else
+            tma_load_2d(dst + j * 8192, map, bar, x, y);
     }
 }
 
-template <int BN>
+template <int BN, int CTAS>
 struct LtTcSmem {
-    using S = LtShape<BN>;
-    static constexpr int STAGES = BN == 256 ? 4 : 6;
-    static constexpr int BYTES = STAGES * S::STAGE + LT_EPI_WARPS * LT_STAGE_BUF + 256 + 1024;
+    static constexpr int A_BYTES = LT_BM * 128, B_BYTES = BN / CTAS * 128, STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = 196608 / STAGE < 8 ? 196608 / STAGE : 8;
+    static constexpr int BYTES = STAGES * STAGE + LT_EPI_WARPS * LT_STAGE_BUF + 256 + 1024;
 };
 
 constexpr int LT_TC_THREADS = 32 * (LT_EPI_WARPS + 2);
 
-template <class T, int BN, bool A_MN, bool B_MN, uint32_t ACT, bool VEC>
+template <class T, int BN, int CTAS, bool A_MN, bool B_MN, uint32_t ACT, bool VEC>
 __global__ void __launch_bounds__(LT_TC_THREADS, 1)
     linear_tc_kernel(const __grid_constant__ LinearTcKernelParams kp) {
     using S = LtShape<BN>;
-    constexpr int STAGES = LtTcSmem<BN>::STAGES;
+    using M = LtTcSmem<BN, CTAS>;
+    constexpr int STAGES = M::STAGES;
     const LinearTcParams &p = kp.p;
     dev_err_bind(p.err);
     extern __shared__ uint8_t smem_raw[];
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *bufs = base + STAGES * S::STAGE;
+    uint8_t *bufs = base + STAGES * M::STAGE;
     uint64_t *full = reinterpret_cast<uint64_t *>(bufs + LT_EPI_WARPS * LT_STAGE_BUF);
     uint64_t *empty = full + STAGES, *acc_full = empty + STAGES, *acc_empty = acc_full + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = CTAS == 2 ? cluster_rank() : 0, unit = blockIdx.x / CTAS, units = gridDim.x / CTAS;
     constexpr uint32_t COLS = 2 * S::TMEM;
     if (threadIdx.x == 0) {
+        // Pairs: the leader's producer arms a stage for both CTAs' bytes, and its commits release it,
+        // and hand over an accumulator, in both.
         for (int s = 0; s < STAGES; s++) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_empty[i], LT_EPI_WARPS);
+            mbar_init(&acc_empty[i], CTAS * LT_EPI_WARPS);
         }
         fence_barrier_init();
     }
-    if (warp == LT_EPI_WARPS + 1) tmem_alloc(tmem_slot, COLS);
+    if (warp == LT_EPI_WARPS + 1) {
+        if constexpr (CTAS == 2)
+            tmem_alloc_pair(tmem_slot, COLS);
+        else
+            tmem_alloc(tmem_slot, COLS);
+    }
     tc_fence_before();
     __syncthreads();
+    if constexpr (CTAS == 2) {
+        cluster_arrive();  // both CTAs' barriers are ready before either signals the other
+        cluster_wait();
+    }
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_wait();
@@ -323,10 +370,12 @@ __global__ void __launch_bounds__(LT_TC_THREADS, 1)
         if (lane == 0) {
             tma_prefetch_desc(&kp.map_a);
             tma_prefetch_desc(&kp.map_b);
+            const uint32_t leader = CTAS == 2 ? map_to_rank(smem_u32(full), 0) : 0;
             uint32_t it = 0;
             bool ok = true;
-            for (uint32_t i = blockIdx.x; ok && i < items; i += gridDim.x) {
-                const uint32_t t = i % tiles, z = i / tiles, n0 = t % p.tiles_n * BN, m0 = t / p.tiles_n * LT_BM;
+            for (uint32_t i = unit; ok && i < items; i += units) {
+                const uint32_t t = i % tiles, z = i / tiles;
+                const uint32_t n0 = t % p.tiles_n * BN + rank * (BN / CTAS), m0 = (t / p.tiles_n * CTAS + rank) * LT_BM;
                 const uint32_t k1 = (uint32_t)((uint64_t)blocks * (z + 1) / p.splits);
                 for (uint32_t kb = (uint32_t)((uint64_t)blocks * z / p.splits); kb < k1; kb++, it++) {
                     const uint32_t s = it % STAGES, round = it / STAGES;
@@ -334,23 +383,23 @@ __global__ void __launch_bounds__(LT_TC_THREADS, 1)
                         ok = false;
                         break;
                     }
-                    uint8_t *st = base + s * S::STAGE;
-                    mbar_arrive_expect_tx(&full[s], S::A_BYTES + S::B_BYTES);
-                    lt_tma<LT_BM, A_MN>(st, &kp.map_a, &full[s], m0, kb * LT_BK);
-                    lt_tma<BN, B_MN>(st + S::A_BYTES, &kp.map_b, &full[s], n0, kb * LT_BK);
+                    uint8_t *st = base + s * M::STAGE;
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], CTAS * M::STAGE);
+                    lt_tma<CTAS, LT_BM, A_MN>(st, &kp.map_a, &full[s], leader + s * 8, m0, kb * LT_BK);
+                    lt_tma<CTAS, BN / CTAS, B_MN>(st + M::A_BYTES, &kp.map_b, &full[s], leader + s * 8, n0, kb * LT_BK);
                 }
             }
-            // After a wait that gave up, the copies still in flight land before the CTA may leave.
-            if (!ok)
-                for (uint32_t j = it > STAGES ? it - STAGES : 0; j < it; j++)
-                    mbar_wait(&full[j % STAGES], (j / STAGES) & 1, JC_DEV_TIMEOUT_FULL);
+            // Every stage in use is released before the CTA may leave: all its copies have landed and
+            // (pairs) the leader's last commits have arrived.
+            for (uint32_t j = it > STAGES ? it - STAGES : 0; j < it; j++)
+                if (!mbar_wait(&empty[j % STAGES], (j / STAGES) & 1, JC_DEV_TIMEOUT_EMPTY)) break;
         }
     } else if (warp == LT_EPI_WARPS + 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = lt_idesc<T>(BN, A_MN, B_MN);
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = lt_idesc<T>(CTAS * LT_BM, BN, A_MN, B_MN);
             uint32_t it = 0, done = 0;
             bool ok = true;
-            for (uint32_t i = blockIdx.x; ok && i < items; i += gridDim.x, done++) {
+            for (uint32_t i = unit; ok && i < items; i += units, done++) {
                 const uint32_t z = i / tiles, buf = done & 1, use = done >> 1;
                 if (use > 0 && !mbar_wait(&acc_empty[buf], (use & 1) ^ 1, JC_DEV_TIMEOUT_MMA)) break;
                 tc_fence_after();
@@ -364,40 +413,65 @@ __global__ void __launch_bounds__(LT_TC_THREADS, 1)
                         break;
                     }
                     tc_fence_after();
-                    const uint64_t ad = lt_desc<A_MN>(smem_u32(base + s * S::STAGE));
-                    const uint64_t bd = lt_desc<B_MN>(smem_u32(base + s * S::STAGE + S::A_BYTES));
+                    const uint64_t ad = lt_desc<A_MN>(smem_u32(base + s * M::STAGE));
+                    const uint64_t bd = lt_desc<B_MN>(smem_u32(base + s * M::STAGE + M::A_BYTES));
 #pragma unroll
-                    for (int kk = 0; kk < LT_BK / 16; kk++)
-                        tc_mma_f16(acc, ad + kk * LT_STEP<A_MN>, bd + kk * LT_STEP<B_MN>, idesc, kb > k0 || kk > 0);
-                    tc_commit(&empty[s]);
+                    for (int kk = 0; kk < LT_BK / 16; kk++) {
+                        if constexpr (CTAS == 2)
+                            tc_mma_f16_pair(acc, ad + kk * LT_STEP<A_MN>, bd + kk * LT_STEP<B_MN>, idesc, kb > k0 || kk > 0);
+                        else
+                            tc_mma_f16(acc, ad + kk * LT_STEP<A_MN>, bd + kk * LT_STEP<B_MN>, idesc, kb > k0 || kk > 0);
+                    }
+                    if constexpr (CTAS == 2)
+                        tc_commit_pair(&empty[s]);
+                    else
+                        tc_commit(&empty[s]);
                 }
-                tc_commit(&acc_full[buf]);
+                if constexpr (CTAS == 2)
+                    tc_commit_pair(&acc_full[buf]);
+                else
+                    tc_commit(&acc_full[buf]);
             }
         }
     } else {
         uint8_t *buf = bufs + warp * LT_STAGE_BUF;
+        const uint32_t leader = CTAS == 2 ? map_to_rank(smem_u32(acc_empty), 0) : 0;
+        LtBias<S::CW> bias;
         LtRes<S::CW> res;
         uint32_t done = 0;
-        for (uint32_t i = blockIdx.x; i < items; i += gridDim.x, done++) {
-            const uint32_t t = i % tiles, n0 = t % p.tiles_n * BN, m0 = t / p.tiles_n * LT_BM;
-            // The first chunk's residual is on its way while the accumulator is still being summed.
+        for (uint32_t i = unit; i < items; i += units, done++) {
+            const uint32_t t = i % tiles, n0 = t % p.tiles_n * BN, m0 = (t / p.tiles_n * CTAS + rank) * LT_BM;
+            // The first chunk's bias and residual are on their way while the accumulator is being summed.
+            bias.load(p.bias, n0 + (warp >> 2) * (BN / 2), p.n);
             if (VEC && p.res && warp / 4 < (uint32_t)S::HALVES)
                 res.load(static_cast<const uint8_t *>(p.res), p.ldres, m0 + 32 * (warp & 3),
                          n0 + (warp >> 2) * (BN / 2), p.m, p.n);
             if (!mbar_wait_sleep(&acc_full[done & 1], (done >> 1) & 1, JC_DEV_TIMEOUT_MMA)) break;
             tc_fence_after();
-            lt_epilogue<T, BN, ACT, VEC>(p, tmem + (done & 1) * S::TMEM, buf, warp, m0, n0, i / tiles, res);
+            lt_epilogue<T, BN, ACT, VEC>(p, tmem + (done & 1) * S::TMEM, buf, warp, m0, n0, i / tiles, bias, res);
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[done & 1]);
+            if (lane == 0) {
+                if (rank == 0)
+                    mbar_arrive(&acc_empty[done & 1]);
+                else
+                    mbar_arrive_remote(leader + (done & 1) * 8);
+            }
         }
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if constexpr (CTAS == 2) {
+        cluster_arrive();  // every MMA into either CTA's accumulators is done and read
+        cluster_wait();
+    }
     if (warp == LT_EPI_WARPS + 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, COLS);
+        if constexpr (CTAS == 2)
+            tmem_dealloc_pair(tmem, COLS);
+        else
+            tmem_dealloc(tmem, COLS);
     }
 }
 
@@ -488,7 +562,7 @@ __global__ void __launch_bounds__(LT_ANY_THREADS, 1)
     const uint32_t count = (uint32_t)((uint64_t)blocks * (z + 1) / p.splits) - kb0;
     if (warp == LT_EPI_WARPS) {
         if (lane == 0) {
-            constexpr uint32_t idesc = lt_idesc<T>(BN, A_MN, B_MN);
+            constexpr uint32_t idesc = lt_idesc<T>(LT_BM, BN, A_MN, B_MN);
             for (uint32_t it = 0; it < count; it++) {
                 const uint32_t s = it % STAGES;
                 if (!mbar_wait(&full[s], (it / STAGES) & 1, JC_DEV_TIMEOUT_FULL)) break;
@@ -524,8 +598,10 @@ __global__ void __launch_bounds__(LT_ANY_THREADS, 1)
         ok = mbar_wait_sleep(acc_full, 0, JC_DEV_TIMEOUT_MMA);
         if (__all_sync(0xffffffffu, ok)) {
             tc_fence_after();
+            LtBias<S::CW> bias;
             LtRes<S::CW> res;
-            lt_epilogue<T, BN, ACT, false>(p, tmem, bufs + warp * LT_STAGE_BUF, warp, m0, n0, z, res);
+            bias.load(p.bias, n0 + (warp >> 2) * (BN / 2), p.n);
+            lt_epilogue<T, BN, ACT, false>(p, tmem, bufs + warp * LT_STAGE_BUF, warp, m0, n0, z, bias, res);
         }
     }
     __syncwarp();

@@ -220,19 +220,36 @@ static bool out_vec(const Product &q) {
            (!q.res || aligned16(q.res, q.ldres, 2));
 }
 
-template <class T, int BN, bool A_MN, bool B_MN, uint32_t ACT, bool VEC>
+template <class T, int BN, int CTAS, bool A_MN, bool B_MN, uint32_t ACT, bool VEC>
 static bool launch_tc(const Product &q, LinearTcParams &p, cudaStream_t s) {
     static std::atomic<uint64_t> smem_set{0};
-    auto kern = linear_tc_kernel<T, BN, A_MN, B_MN, ACT, VEC>;
+    auto kern = linear_tc_kernel<T, BN, CTAS, A_MN, B_MN, ACT, VEC>;
     LinearTcKernelParams kp;
     kp.p = p;
-    if (!ensure_smem(kern, LtTcSmem<BN>::BYTES, smem_set) ||
-        !make_operand_map<T>(&kp.map_a, q.a, q.m, q.k, A_MN, LT_BM) ||
-        !make_operand_map<T>(&kp.map_b, q.b, q.n, q.k, B_MN, BN))
+    kp.p.tiles_m = (q.m + CTAS * LT_BM - 1) / (CTAS * LT_BM);
+    kp.p.tiles_n = (q.n + BN - 1) / BN;
+    const uint64_t items = (uint64_t)kp.p.tiles_m * kp.p.tiles_n * p.splits;
+    if (items > 0x7FFFFFFFull) {
+        set_error("linear: too many tiles");
         return false;
-    const uint64_t items = (uint64_t)p.tiles_m * p.tiles_n * p.splits;
-    const uint32_t grid = (uint32_t)std::min<uint64_t>(items, (uint64_t)sm_count());
-    return launch_ex(kern, dim3(grid), dim3(LT_TC_THREADS), LtTcSmem<BN>::BYTES, s, true, "linear", kp);
+    }
+    using Mem = LtTcSmem<BN, CTAS>;
+    if (!ensure_smem(kern, Mem::BYTES, smem_set) || !make_operand_map<T>(&kp.map_a, q.a, q.m, q.k, A_MN, LT_BM) ||
+        !make_operand_map<T>(&kp.map_b, q.b, q.n, q.k, B_MN, BN / CTAS))
+        return false;
+    if constexpr (CTAS == 1) {
+        const uint32_t grid = (uint32_t)std::min<uint64_t>(items, (uint64_t)sm_count());
+        return launch_ex(kern, dim3(grid), dim3(LT_TC_THREADS), Mem::BYTES, s, true, "linear", kp);
+    } else {
+        static std::atomic<int> max_pairs{0};
+        int pairs = max_pairs.load();
+        if (pairs == 0) {
+            if (!max_clusters(kern, 2, LT_TC_THREADS, Mem::BYTES, &pairs)) return false;
+            max_pairs.store(pairs);
+        }
+        const uint32_t grid = 2 * (uint32_t)std::min<uint64_t>(items, (uint64_t)pairs);
+        return launch_ex_cluster(kern, dim3(grid), dim3(LT_TC_THREADS), Mem::BYTES, s, true, dim3(2, 1, 1), "linear", kp);
+    }
 }
 
 template <class T, int BN, bool A_MN, bool B_MN, uint32_t ACT>
@@ -244,19 +261,25 @@ static bool launch_any(const LinearTcParams &p, cudaStream_t s) {
                      true, "linear", p);
 }
 
-// Microseconds a product takes by the TMA kernel with BN-column tiles: the busiest CTA's items, each a
-// main loop of about 0.28 us per 64 contracted elements whatever BN is (one thread's MMAs complete in
-// order at about 130 cycles each) plus the part of its epilogue that nothing hides.
-static double tc_us(uint32_t m, uint32_t n, uint32_t k, uint32_t bn, uint32_t splits, uint32_t sms) {
-    const uint64_t items = (uint64_t)((m + LT_BM - 1) / LT_BM) * ((n + bn - 1) / bn) * splits;
-    const uint32_t blocks = ((k + LT_BK - 1) / LT_BK + splits - 1) / splits;
-    return (double)((items + sms - 1) / sms) * (0.28 * blocks + 0.5) + 2.0 + 0.008 * bn;
+// How the TMA kernel tiles a product: `ctas` x 128 rows by bn columns.
+struct Tiling {
+    uint32_t ctas, bn;
+};
+constexpr Tiling TILINGS[] = {{1, 64}, {1, 128}, {2, 128}, {2, 256}};
+
+// Microseconds a product takes with a tiling: the busiest unit's items, each a main loop of about 0.28
+// us per 64 contracted elements (one thread's MMAs complete in order at about 130 cycles each whatever
+// their width), plus the first loads and the last epilogue, which nothing hides.
+static double tc_us(uint32_t m, uint32_t n, uint32_t k, Tiling t, uint32_t splits, uint32_t sms) {
+    const uint64_t items = (uint64_t)((m + t.ctas * LT_BM - 1) / (t.ctas * LT_BM)) * ((n + t.bn - 1) / t.bn) * splits;
+    const uint32_t blocks = ((k + LT_BK - 1) / LT_BK + splits - 1) / splits, units = sms / t.ctas;
+    return (double)((items + units - 1) / units) * (0.28 * blocks + 0.5) + 2.0 + 0.008 * t.bn;
 }
 
-static uint32_t pick_bn(uint32_t m, uint32_t n, uint32_t k, uint32_t splits, uint32_t sms) {
-    uint32_t best = 64;
-    for (uint32_t bn : {128u, 256u})
-        if (tc_us(m, n, k, bn, splits, sms) <= tc_us(m, n, k, best, splits, sms)) best = bn;
+static Tiling pick_tiling(uint32_t m, uint32_t n, uint32_t k, uint32_t splits, uint32_t sms) {
+    Tiling best = TILINGS[0];
+    for (const Tiling &t : TILINGS)
+        if (tc_us(m, n, k, t, splits, sms) <= tc_us(m, n, k, best, splits, sms)) best = t;
     return best;
 }
 
@@ -288,16 +311,15 @@ static bool launch_product(const Product &q, cudaStream_t s) {
         return false;
     };
     if (tma_ok(q.a, A_MN) && tma_ok(q.b, B_MN)) {
-        const uint32_t bn = pick_bn(q.m, q.n, q.k, q.splits, (uint32_t)sm_count());
+        const Tiling t = pick_tiling(q.m, q.n, q.k, q.splits, (uint32_t)sm_count());
         const bool vec = out_vec(q);
-        if (!tiles(bn)) return false;
-        auto run = [&](auto w) {
-            constexpr int BN = decltype(w)::value;
-            // The gradients' outputs are as aligned as the operands they sit beside, or go the other way.
-            return vec ? launch_tc<T, BN, A_MN, B_MN, ACT, true>(q, p, s)
-                       : launch_tc<T, BN, A_MN, B_MN, ACT, false>(q, p, s);
+        auto run = [&](auto c, auto w) {
+            constexpr int CTAS = decltype(c)::value, BN = decltype(w)::value;
+            return vec ? launch_tc<T, BN, CTAS, A_MN, B_MN, ACT, true>(q, p, s)
+                       : launch_tc<T, BN, CTAS, A_MN, B_MN, ACT, false>(q, p, s);
         };
-        return bn == 256 ? run(Int<256>()) : bn == 128 ? run(Int<128>()) : run(Int<64>());
+        if (t.ctas == 2) return t.bn == 256 ? run(Int<2>(), Int<256>()) : run(Int<2>(), Int<128>());
+        return t.bn == 128 ? run(Int<1>(), Int<128>()) : run(Int<1>(), Int<64>());
     }
     if (q.n <= 16) return tiles(16) && launch_any<T, 16, A_MN, B_MN, ACT>(p, s);
     if (q.n <= 64) return tiles(64) && launch_any<T, 64, A_MN, B_MN, ACT>(p, s);
@@ -345,7 +367,7 @@ static LinearBwdPlan plan_linear_bwd(uint32_t m, uint32_t n, uint32_t k) {
     p.splits = 1;
     double best = 1e30;
     for (uint32_t s = 1; s <= std::min(32u, std::max(1u, blocks)); s++) {
-        const double us = tc_us(n, k, m, pick_bn(n, k, m, s, sms), s, sms) + (s > 1 ? 2.0 + 8e-6 * s * n * k / 3.0 : 0.0);
+        const double us = tc_us(n, k, m, pick_tiling(n, k, m, s, sms), s, sms) + (s > 1 ? 2.0 + 8e-6 * s * n * k / 3.0 : 0.0);
         if (us < best) {
             best = us;
             p.splits = s;
@@ -387,7 +409,6 @@ bool launch_linear_bwd(const LinearBwdArgs &a, cudaStream_t s) {
                 }))
                 return false;
         }
-        if (a.dbias && !launch_column_sum(part, a.m ? plan.dz_parts : 0, a.n, a.n, a.dbias, nullptr, s)) return false;
         if (a.dx && a.m > 0) {
             Product q;
             q.a = LinearOperand{dz, lddz, 1};
@@ -399,8 +420,8 @@ bool launch_linear_bwd(const LinearBwdArgs &a, cudaStream_t s) {
             q.ldc = a.lddx;
             if (!launch_product<T, false, true, 0>(q, s)) return false;
         }
+        LinearFinishParams f{};
         if (a.dw) {
-            float *parts = nullptr;
             if (a.m > 0) {
                 Product q;
                 q.a = LinearOperand{dz, 1, lddz};
@@ -411,18 +432,30 @@ bool launch_linear_bwd(const LinearBwdArgs &a, cudaStream_t s) {
                 q.c = a.dw;
                 q.ldc = a.lddw;
                 q.splits = plan.splits;
-                if (plan.splits > 1) q.ws = parts = reinterpret_cast<float *>(ws + plan.ws_at);
+                if (plan.splits > 1) f.ws = q.ws = reinterpret_cast<float *>(ws + plan.ws_at);
                 if (!launch_product<T, true, true, 0>(q, s)) return false;
             }
-            if (parts || a.m == 0) {
-                const size_t all = (size_t)a.n * a.k;
-                const uint32_t blocks = (uint32_t)std::min<size_t>((all + 255) / 256, 148 * 8);
-                if (!launch_ex(linear_join_kernel<T>, dim3(blocks), dim3(256), 0, s, true, "linear join",
-                               (const float *)parts, a.m ? plan.splits : 0u, a.n, a.k, static_cast<T *>(a.dw), a.lddw))
-                    return false;
+            if (f.ws || a.m == 0) {
+                f.splits = a.m ? plan.splits : 0;
+                f.m = a.n;
+                f.n = a.k;
+                f.c = a.dw;
+                f.ldc = a.lddw;
             }
         }
-        return true;
+        const bool vec = f.n % 8 == 0 && aligned16(f.c, f.ldc, 2);
+        const uint64_t threads = (uint64_t)f.m * (vec ? f.n / 8 : f.n);
+        f.join_blocks = (uint32_t)std::min<uint64_t>((threads + 255) / 256, 148 * 16);
+        if (a.dbias) {
+            f.part = part;
+            f.parts = a.m ? plan.dz_parts : 0;
+            f.bias_n = a.n;
+            f.dbias = a.dbias;
+        }
+        const dim3 grid(f.join_blocks + (f.bias_n + 31) / 32);
+        if (grid.x == 0) return true;
+        return vec ? launch_ex(linear_finish_kernel<T, 8>, grid, dim3(256), 0, s, true, "linear_backward", f)
+                   : launch_ex(linear_finish_kernel<T, 1>, grid, dim3(256), 0, s, true, "linear_backward", f);
     });
 }
 
