@@ -10,6 +10,7 @@
 
 #include "adamw.cuh"
 #include "launch.h"
+#include "linear_small.cuh"
 #include "linear_tc.cuh"
 #include "loss.cuh"
 #include "norm.cuh"
@@ -326,8 +327,43 @@ static bool launch_product(const Product &q, cudaStream_t s) {
     return tiles(128) && launch_any<T, 128, A_MN, B_MN, ACT>(p, s);
 }
 
+// Calls f(N) for the smallest instantiated number of columns a thin layer of n has.
+template <class F>
+static bool with_thin(uint32_t n, F &&f) {
+    if (n <= 1) return f(Int<1>());
+    if (n <= 2) return f(Int<2>());
+    if (n <= 4) return f(Int<4>());
+    return f(Int<8>());
+}
+
+// Up to this many rows the weights are read straight into mma.sync fragments (a 16-row block each);
+// beyond it the tensor tiles of 128 rows are faster.
+constexpr uint32_t LINEAR_ROWS = 16;
+
 bool launch_linear(const LinearArgs &a, cudaStream_t s) {
     if (a.m == 0) return true;
+    const LinearRowsParams rp{a.x, a.ldx, a.w, a.ldw, a.bias, a.res, a.ldres, a.y, a.ldy, a.z, a.ldz, a.m, a.n, a.k};
+    const bool vec = a.k % 8 == 0 && aligned16(a.x, a.ldx, 2) && aligned16(a.w, a.ldw, 2);
+    if (a.n <= LTHIN_MAX)
+        return with_half(a.type, [&](auto t) {
+            using T = decltype(t);
+            return with_act(a.act, [&](auto act) {
+                return with_thin(a.n, [&](auto n) {
+                    constexpr uint32_t ACT = decltype(act)::value;
+                    constexpr int N = decltype(n)::value;
+                    const dim3 grid((a.m + 8 * LTHIN_ROWS - 1) / (8 * LTHIN_ROWS));
+                    return vec ? launch_ex(linear_thin_kernel<T, N, true, ACT>, grid, dim3(256), 0, s, true, "linear", rp)
+                               : launch_ex(linear_thin_kernel<T, N, false, ACT>, grid, dim3(256), 0, s, true, "linear", rp);
+                });
+            });
+        });
+    if (a.m <= LINEAR_ROWS && vec)
+        return with_half(a.type, [&](auto t) {
+            return with_act(a.act, [&](auto act) {
+                return launch_ex(linear_rows_kernel<decltype(t), decltype(act)::value>, dim3((a.n + 7) / 8, (a.m + 15) / 16),
+                                 dim3(32 * LR_WARPS), 0, s, true, "linear", rp);
+            });
+        });
     Product q;
     q.a = LinearOperand{a.x, a.ldx, 1};
     q.b = LinearOperand{a.w, a.ldw, 1};
@@ -352,6 +388,7 @@ bool launch_linear(const LinearArgs &a, cudaStream_t s) {
 // partial products, each from a 256-byte boundary.
 struct LinearBwdPlan {
     uint32_t dz_parts, splits;
+    uint32_t thin_blocks;  // n <= LTHIN_MAX: blocks along the rows, each with its sums; nothing else used
     size_t lddz, part_at, ws_at, bytes;
 };
 
@@ -365,6 +402,11 @@ static LinearBwdPlan plan_linear_bwd(uint32_t m, uint32_t n, uint32_t k) {
     // dw's contraction runs over the rows: split so that its few tiles still fill the SMs.
     const uint32_t sms = 148, blocks = (m + LT_BK - 1) / LT_BK;
     p.splits = 1;
+    if (n <= LTHIN_MAX) {
+        p.thin_blocks = std::max(1u, std::min((m + 31) / 32, sms * 2));
+        p.bytes = up((size_t)p.thin_blocks * ((size_t)n * k + n) * 4);
+        return p;
+    }
     double best = 1e30;
     for (uint32_t s = 1; s <= std::min(32u, std::max(1u, blocks)); s++) {
         const double us = tc_us(n, k, m, pick_tiling(n, k, m, s, sms), s, sms) + (s > 1 ? 2.0 + 8e-6 * s * n * k / 3.0 : 0.0);
@@ -379,9 +421,41 @@ static LinearBwdPlan plan_linear_bwd(uint32_t m, uint32_t n, uint32_t k) {
 
 size_t linear_bwd_ws_bytes(uint32_t m, uint32_t n, uint32_t k) { return plan_linear_bwd(m, n, k).bytes; }
 
+static bool launch_linear_thin_bwd(const LinearBwdArgs &a, uint32_t blocks, cudaStream_t s) {
+    return with_half(a.type, [&](auto t) {
+        using T = decltype(t);
+        float *part = a.dw || a.dbias ? static_cast<float *>(a.ws) : nullptr;
+        if (a.m > 0) {
+            const LinearThinBwdParams p{a.dy, a.lddy, a.x, a.ldx, a.w, a.ldw, a.z, a.ldz, a.m, a.n, a.k,
+                                        a.dx, a.lddx, part, a.dw != nullptr};
+            const bool vec = a.k % 8 == 0 && (!a.dw || aligned16(a.x, a.ldx, 2)) &&
+                             (!a.dx || (aligned16(a.w, a.ldw, 2) && aligned16(a.dx, a.lddx, 2)));
+            const dim3 grid(blocks, (a.k + 255) / 256);
+            if (grid.y > 65535) {
+                set_error("linear_backward: k is too large");
+                return false;
+            }
+            if (!with_act(a.act, [&](auto act) {
+                    return with_thin(a.n, [&](auto n) {
+                        constexpr uint32_t ACT = decltype(act)::value;
+                        constexpr int N = decltype(n)::value;
+                        return vec ? launch_ex(linear_thin_bwd_kernel<T, N, true, ACT>, grid, dim3(256), 0, s, true, "linear_backward", p)
+                                   : launch_ex(linear_thin_bwd_kernel<T, N, false, ACT>, grid, dim3(256), 0, s, true, "linear_backward", p);
+                    });
+                }))
+                return false;
+        }
+        if (!part) return true;
+        return launch_ex(linear_thin_finish_kernel<T>, dim3((a.n * a.k + a.n + 31) / 32), dim3(256), 0, s, true,
+                         "linear_backward", (const float *)part, a.m ? blocks : 0u, a.n, a.k, static_cast<T *>(a.dw),
+                         a.lddw, a.dbias);
+    });
+}
+
 bool launch_linear_bwd(const LinearBwdArgs &a, cudaStream_t s) {
     const LinearBwdPlan plan = plan_linear_bwd(a.m, a.n, a.k);
     uint8_t *ws = static_cast<uint8_t *>(a.ws);
+    if (plan.thin_blocks) return launch_linear_thin_bwd(a, plan.thin_blocks, s);
     float *part = reinterpret_cast<float *>(ws + plan.part_at);
     return with_half(a.type, [&](auto t) {
         using T = decltype(t);
