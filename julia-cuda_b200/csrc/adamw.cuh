@@ -22,6 +22,7 @@ namespace jc {
 struct AdamwParams {
     const AdamwTensor *tensors;
     const uint2 *chunks;  // (tensor, chunk of it)
+    uint32_t n_chunks;
     const float *grad_scale;
     float beta1, beta2, one_minus_beta1, one_minus_beta2, lr, eps;
     float inv_bias1, inv_bias2;  // 1 / (1 - beta^t)
@@ -95,6 +96,12 @@ __device__ __forceinline__ void store_codes(uint8_t *p, uint32_t n, bool vec, co
 
 constexpr float FP8_MAX = 448.0f, FP8_MIN = 0.001953125f;  // e4m3: largest, smallest above 0
 
+__device__ __forceinline__ float sqrt_approx(float x) {
+    float y;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // x / s, given inv = 1 / s rounded to nearest: the product's remainder, exact in one fused
 // multiply-add, corrects it (Markstein, "Computation of elementary functions on the IBM RISC
 // System/6000 processor", 1990). The correctly rounded quotient wherever that remainder does not
@@ -104,75 +111,100 @@ __device__ __forceinline__ float div_by(float x, float s, float inv) {
     return __fmaf_rn(__fmaf_rn(-q, s, x), inv, q);
 }
 
-// One chunk a block, eight consecutive elements a thread: a warp holds the 256 elements that share
-// an 8-bit state's scale.
+// Blocks stay and walk the chunks, eight consecutive elements a thread (a warp holds the 256 elements
+// that share an 8-bit state's scale). The next chunk's tensor is looked up, into shared memory, while
+// the current one's data is on its way: looked up when needed, the two dependent reads in front of
+// every chunk left the memory idle for a third of the time.
+constexpr uint32_t ADAMW_WORDS = sizeof(AdamwTensor) / 4;
+
 template <int BITS>
 __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const AdamwParams p) {
+    __shared__ alignas(16) uint32_t desc[2][ADAMW_WORDS];
     pdl_wait();
     pdl_launch_dependents();
-    const uint2 ch = p.chunks[blockIdx.x];
-    const AdamwTensor &t = p.tensors[ch.x];
-    const uint64_t at = (uint64_t)ch.y * ADAMW_CHUNK + threadIdx.x * 8;
-    if ((at & ~uint64_t(255)) >= t.n) return;  // the whole warp is past the end
-    const uint32_t n = at >= t.n ? 0 : (uint32_t)min((uint64_t)8, t.n - at);
-    const bool vec = t.aligned && n == 8;
+    const uint32_t tid = threadIdx.x;
+    auto word = [&](uint32_t tensor) {
+        return __ldg(reinterpret_cast<const uint32_t *>(p.tensors + tensor) + tid);
+    };
+    uint2 ch = __ldg(p.chunks + blockIdx.x);  // the grid has no more blocks than chunks
+    uint2 next = make_uint2(0, 0);
+    if (blockIdx.x + gridDim.x < p.n_chunks) next = __ldg(p.chunks + blockIdx.x + gridDim.x);
+    if (tid < ADAMW_WORDS) desc[0][tid] = word(ch.x);
     const float gs = p.grad_scale ? *p.grad_scale : 1.0f;
-    float g[8], m[8], v[8], w[8];
-    if (t.grad_type == JC_F32)
-        load8(static_cast<const float *>(t.g) + at, n, vec, g);
-    else if (t.grad_type == JC_F16)
-        load8(static_cast<const __half *>(t.g) + at, n, vec, g);
-    else
-        load8(static_cast<const __nv_bfloat16 *>(t.g) + at, n, vec, g);
-    load8(t.p + at, n, vec, w);
-    if constexpr (BITS == 8) {
-        load_codes(static_cast<const uint8_t *>(t.m) + at, n, vec, t.m_scale[at / ADAMW_BLOCK], m);
-        load_codes(static_cast<const uint8_t *>(t.v) + at, n, vec, t.v_scale[at / ADAMW_BLOCK], v);
-    } else {
-        load8(static_cast<const float *>(t.m) + at, n, vec, m);
-        load8(static_cast<const float *>(t.v) + at, n, vec, v);
-    }
-    const float keep = 1.0f - p.lr * t.decay;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        // Each operation of the states rounded by itself, so that an 8-bit code does not depend on
-        // how a compiler contracts them.
-        const float gi = __fmul_rn(g[i], gs);
-        m[i] = __fadd_rn(__fmul_rn(p.beta1, m[i]), __fmul_rn(p.one_minus_beta1, gi));
-        v[i] = __fadd_rn(__fmul_rn(p.beta2, v[i]), __fmul_rn(__fmul_rn(p.one_minus_beta2, gi), gi));
-        w[i] = w[i] * keep - p.lr * (m[i] * p.inv_bias1) / (sqrtf(v[i] * p.inv_bias2) + p.eps);
-    }
-    store8(t.p + at, n, vec, w);
-    if (t.copy_type == JC_F16)
-        store8(static_cast<__half *>(t.copy) + at, n, vec, w);
-    else if (t.copy_type == JC_BF16)
-        store8(static_cast<__nv_bfloat16 *>(t.copy) + at, n, vec, w);
-    if constexpr (BITS == 8) {
-        float mm = 0.0f, vm = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            mm = fmaxf(mm, fabsf(m[i]));
-            vm = fmaxf(vm, v[i]);
+    __syncthreads();
+    uint32_t buf = 0;
+    for (uint32_t i = blockIdx.x; i < p.n_chunks; i += gridDim.x, buf ^= 1) {
+        const AdamwTensor &t = *reinterpret_cast<const AdamwTensor *>(desc[buf]);
+        const uint64_t at = (uint64_t)ch.y * ADAMW_CHUNK + tid * 8;
+        const bool some = (at & ~uint64_t(255)) < t.n;  // of this warp
+        const uint32_t n = at >= t.n ? 0 : (uint32_t)min((uint64_t)8, t.n - at);
+        const bool vec = t.aligned && n == 8;
+        float g[8], m[8], v[8], w[8];
+        if (some) {
+            if (t.grad_type == JC_F32)
+                load8(static_cast<const float *>(t.g) + at, n, vec, g);
+            else if (t.grad_type == JC_F16)
+                load8(static_cast<const __half *>(t.g) + at, n, vec, g);
+            else
+                load8(static_cast<const __nv_bfloat16 *>(t.g) + at, n, vec, g);
+            load8(t.p + at, n, vec, w);
+            if constexpr (BITS == 8) {
+                load_codes(static_cast<const uint8_t *>(t.m) + at, n, vec, t.m_scale[at / ADAMW_BLOCK], m);
+                load_codes(static_cast<const uint8_t *>(t.v) + at, n, vec, t.v_scale[at / ADAMW_BLOCK], v);
+            } else {
+                load8(static_cast<const float *>(t.m) + at, n, vec, m);
+                load8(static_cast<const float *>(t.v) + at, n, vec, v);
+            }
         }
-        mm = __fmul_rn(warp_max(mm), 1.0f / FP8_MAX);
-        vm = __fmul_rn(warp_max(vm), 1.0f / FP8_MAX);
-        const float sm = mm > 0.0f ? mm : 1.0f, sv = vm > 0.0f ? vm : 1.0f;
-        const float im = __frcp_rn(sm), iv = __frcp_rn(sv);
+        if (i + gridDim.x < p.n_chunks && tid < ADAMW_WORDS) desc[buf ^ 1][tid] = word(next.x);
+        ch = next;
+        if (i + 2ull * gridDim.x < p.n_chunks) next = __ldg(p.chunks + i + 2 * gridDim.x);
+        if (some) {
+            const float keep = 1.0f - p.lr * t.decay;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float q = div_by(v[i], sv, iv);
-            v[i] = v[i] > 0.0f ? fmaxf(q, FP8_MIN) : v[i];
-            m[i] = div_by(m[i], sm, im);
+            for (int j = 0; j < 8; j++) {
+                // Each operation of the states rounded by itself, so that an 8-bit code does not
+                // depend on how a compiler contracts them.
+                const float gi = __fmul_rn(g[j], gs);
+                m[j] = __fadd_rn(__fmul_rn(p.beta1, m[j]), __fmul_rn(p.one_minus_beta1, gi));
+                v[j] = __fadd_rn(__fmul_rn(p.beta2, v[j]), __fmul_rn(__fmul_rn(p.one_minus_beta2, gi), gi));
+                // The quotient and root to a few ulp: their error is far below the parameter's own.
+                w[j] = w[j] * keep - __fdividef(p.lr * (m[j] * p.inv_bias1), sqrt_approx(v[j] * p.inv_bias2) + p.eps);
+            }
+            store8(t.p + at, n, vec, w);
+            if (t.copy_type == JC_F16)
+                store8(static_cast<__half *>(t.copy) + at, n, vec, w);
+            else if (t.copy_type == JC_BF16)
+                store8(static_cast<__nv_bfloat16 *>(t.copy) + at, n, vec, w);
+            if constexpr (BITS == 8) {
+                float mm = 0.0f, vm = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    mm = fmaxf(mm, fabsf(m[j]));
+                    vm = fmaxf(vm, v[j]);
+                }
+                mm = __fmul_rn(warp_max(mm), 1.0f / FP8_MAX);
+                vm = __fmul_rn(warp_max(vm), 1.0f / FP8_MAX);
+                const float sm = mm > 0.0f ? mm : 1.0f, sv = vm > 0.0f ? vm : 1.0f;
+                const float im = __frcp_rn(sm), iv = __frcp_rn(sv);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float q = div_by(v[j], sv, iv);
+                    v[j] = v[j] > 0.0f ? fmaxf(q, FP8_MIN) : v[j];
+                    m[j] = div_by(m[j], sm, im);
+                }
+                store_codes(static_cast<uint8_t *>(t.m) + at, n, vec, m);
+                store_codes(static_cast<uint8_t *>(t.v) + at, n, vec, v);
+                if ((tid & 31) == 0) {
+                    t.m_scale[at / ADAMW_BLOCK] = mm;
+                    t.v_scale[at / ADAMW_BLOCK] = vm;
+                }
+            } else {
+                store8(static_cast<float *>(t.m) + at, n, vec, m);
+                store8(static_cast<float *>(t.v) + at, n, vec, v);
+            }
         }
-        store_codes(static_cast<uint8_t *>(t.m) + at, n, vec, m);
-        store_codes(static_cast<uint8_t *>(t.v) + at, n, vec, v);
-        if ((threadIdx.x & 31) == 0) {
-            t.m_scale[at / ADAMW_BLOCK] = mm;
-            t.v_scale[at / ADAMW_BLOCK] = vm;
-        }
-    } else {
-        store8(static_cast<float *>(t.m) + at, n, vec, m);
-        store8(static_cast<float *>(t.v) + at, n, vec, v);
+        __syncthreads();  // the next tensor is there, and nobody reads this one any more
     }
 }
 

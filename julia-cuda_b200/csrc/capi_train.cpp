@@ -121,7 +121,7 @@ int jc_layer_norm_backward(uint32_t type, const void *dy, size_t lddy, const voi
             !check_matrix(op, "dx", dx, lddx, d, size, any) || !check_vector(op, "gamma", gamma, 4, true) ||
             !check_vector(op, "stats", stats, 8, any) || !check_vector(op, "dgamma", dgamma, 4, false) ||
             !check_vector(op, "dbeta", dbeta, 4, false) ||
-            !check_vector(op, "ws", ws, 16, any && (dgamma || dbeta)))
+            !check_vector(op, "ws", ws, 16, (dgamma || dbeta) && jc::norm_bwd_ws_floats(rows, d) > 0))
             return -1;
         jc::NormBwdArgs a;
         a.type = type;

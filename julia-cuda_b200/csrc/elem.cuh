@@ -77,6 +77,27 @@ struct Elem<float, 4> {
     }
 };
 
+// Two f32 operations in one instruction (each rounded as its scalar form): a pair is two neighbours of
+// an array of even length.
+__device__ __forceinline__ void add2(float *d, const float *a, const float *b) {
+    asm("{.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+        "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;}"
+        : "=f"(d[0]), "=f"(d[1])
+        : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]));
+}
+__device__ __forceinline__ void mul2(float *d, const float *a, const float *b) {
+    asm("{.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+        "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;}"
+        : "=f"(d[0]), "=f"(d[1])
+        : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]));
+}
+__device__ __forceinline__ void fma2(float *d, const float *a, const float *b, const float *c) {
+    asm("{.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;}"
+        : "=f"(d[0]), "=f"(d[1])
+        : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]), "f"(c[0]), "f"(c[1]));
+}
+
 // Elements of a 16-byte access.
 template <class T>
 constexpr int VEC = 16 / (int)sizeof(T);

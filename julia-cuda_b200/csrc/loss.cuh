@@ -89,15 +89,15 @@ __device__ __forceinline__ void loss_group(const LossParams &p, uint32_t r, uint
     if (top == -INFINITY) top = 0.0f;
     float sum = 0.0f;
 #pragma unroll
-    for (int k = 0; k < LOSS_KEEP; k++) sum += expf(v[k] - top);
-    for (uint32_t i = LOSS_KEEP * G + t; i < b - a; i += G) sum += expf(p.logits[a + i] - top);
+    for (int k = 0; k < LOSS_KEEP; k++) sum += __expf(v[k] - top);
+    for (uint32_t i = LOSS_KEEP * G + t; i < b - a; i += G) sum += __expf(p.logits[a + i] - top);
     sum = loss_sum<G>(sum, part);
     const bool counts = gold >= 0 && w != 0.0f && sum != 0.0f;
     if (t == 0) p.loss[r] = counts ? w * (top + logf(sum) - right) : 0.0f;
     if (!p.dlogits) return;
     const float inv = 1.0f / sum;
     auto grad = [&](uint32_t i, float l) {
-        p.dlogits[a + i] = counts ? w * (expf(l - top) * inv - (i == (uint32_t)gold ? 1.0f : 0.0f)) : 0.0f;
+        p.dlogits[a + i] = counts ? w * (__expf(l - top) * inv - (i == (uint32_t)gold ? 1.0f : 0.0f)) : 0.0f;
     };
 #pragma unroll
     for (int k = 0; k < LOSS_KEEP; k++)
@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) loss_group_kernel(const Los
 // whatever their lengths, and moves them through shared memory in whole lines; a thread works on a
 // request there. A block whose logits do not fit (a long request among short ones) or lie out of
 // order takes them a warp at a time instead.
-constexpr int LOSS_BLOCK = 128, LOSS_SMEM = 4096;
+constexpr int LOSS_BLOCK = 128, LOSS_SMEM = 4096, LOSS_REGS = 16;
 
 __global__ void __launch_bounds__(LOSS_BLOCK) loss_short_kernel(const LossParams p) {
     __shared__ float s[LOSS_SMEM];
@@ -145,19 +145,49 @@ __global__ void __launch_bounds__(LOSS_BLOCK) loss_short_kernel(const LossParams
     }
     for (uint32_t i = t; i < hi - lo; i += LOSS_BLOCK) s[i] = p.logits[lo + i];
     __syncthreads();
-    if (t < n) {
-        float *l = s + (a - lo);
-        const uint32_t len = b - a;
+    const uint32_t len = b - a, longest = __reduce_max_sync(0xffffffffu, len);
+    float *l = s + (a - lo);
+    if (longest <= LOSS_REGS) {
+        // Read once into registers, written back once: these accesses hit random banks.
+        float v[LOSS_REGS], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < LOSS_REGS; i += 4)
+            if (i < longest)
+#pragma unroll
+                for (int j = i; j < i + 4; j++) {
+                    v[j] = j < len ? l[j] : -INFINITY;
+                    top = fmaxf(top, v[j]);
+                }
+        const float right = gold >= 0 ? l[gold] : 0.0f;
+        if (top == -INFINITY) top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < LOSS_REGS; i += 4)
+            if (i < longest)
+#pragma unroll
+                for (int j = i; j < i + 4; j++) {
+                    v[j] = __expf(v[j] - top);
+                    sum += v[j];
+                }
+        const bool counts = gold >= 0 && w != 0.0f && sum != 0.0f;
+        if (t < n) p.loss[r0 + t] = counts ? w * (top + logf(sum) - right) : 0.0f;
+        const float f = counts ? w / sum : 0.0f;
+#pragma unroll
+        for (int i = 0; i < LOSS_REGS; i += 4)
+            if (i < longest)
+#pragma unroll
+                for (int j = i; j < i + 4; j++)
+                    if (j < len) l[j] = counts ? (j == gold ? v[j] * f - w : v[j] * f) : 0.0f;
+    } else {
         float top = -INFINITY, sum = 0.0f;
         for (uint32_t i = 0; i < len; i++) top = fmaxf(top, l[i]);
         if (top == -INFINITY) top = 0.0f;
         const float right = gold >= 0 ? l[gold] : 0.0f;
         for (uint32_t i = 0; i < len; i++) {
-            l[i] = expf(l[i] - top);
+            l[i] = __expf(l[i] - top);
             sum += l[i];
         }
         const bool counts = gold >= 0 && w != 0.0f && sum != 0.0f;
-        p.loss[r0 + t] = counts ? w * (top + logf(sum) - right) : 0.0f;
+        if (t < n) p.loss[r0 + t] = counts ? w * (top + logf(sum) - right) : 0.0f;
         const float f = counts ? w / sum : 0.0f;
         for (uint32_t i = 0; i < len; i++) l[i] = counts ? l[i] * f : 0.0f;
         if (counts) l[gold] -= w;

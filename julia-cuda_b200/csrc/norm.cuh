@@ -35,36 +35,43 @@ constexpr int NORM_BLOCK = G > 128 ? G : 128;
 template <class T, int V, int G, int E>
 constexpr int NORM_BWD_BLOCK = G > 256 ? G : sizeof(T) == 2 && V > 1 && E <= 24 ? 384 : 256;
 
-// Sums of a and b over the G threads of a row's group, in a fixed order. `part`: two floats a warp in
-// shared memory; G > 32: every thread of the block calls it.
-template <int G>
-__device__ __forceinline__ void norm_sum2(float &a, float &b, float2 *part) {
+// Sums over the G threads of a row's group, in a fixed order: K values at once. `part`: K floats a warp
+// in shared memory; G > 32: every thread of the block calls it.
+template <int G, int K>
+__device__ __forceinline__ void norm_sum(float (&v)[K], float *part) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        b += __shfl_xor_sync(0xffffffffu, b, o);
-    }
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < K; k++) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
     if constexpr (G > 32) {
         const uint32_t warp = threadIdx.x >> 5, first = warp / (G / 32) * (G / 32);
         __syncthreads();
-        if ((threadIdx.x & 31) == 0) part[warp] = make_float2(a, b);
-        __syncthreads();
-        a = b = 0.0f;
+        if ((threadIdx.x & 31) == 0)
 #pragma unroll
-        for (int w = 0; w < G / 32; w++) {
-            a += part[first + w].x;
-            b += part[first + w].y;
+            for (int k = 0; k < K; k++) part[warp * K + k] = v[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            v[k] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < G / 32; w++) v[k] += part[(first + w) * K + k];
         }
     }
 }
 
 // Thread t's share of a row of d elements that starts `shift` elements into its first chunk: chunk c
-// holds elements first(c) .. first(c) + V.
+// holds elements first(c) .. first(c) + V. What lies outside the row is masked in the chunks that need
+// it (`edges`, the same for a whole warp and for every row).
 template <class T, int V, int G, int E>
 struct NormRow {
     static constexpr int N = E / V;
     using Raw = std::conditional_t<V == 1, T, uint4>;
-    uint32_t t, shift, d;
+    uint32_t t, shift, d, edges;
+    __device__ __forceinline__ NormRow(uint32_t t_, uint32_t shift_, uint32_t d_) : t(t_), shift(shift_), d(d_), edges(0) {
+#pragma unroll
+        for (int c = 0; c < N; c++)
+            if (__any_sync(0xffffffffu, !whole(c))) edges |= 1u << c;
+    }
     __device__ __forceinline__ uint32_t place(int c) const { return (c * G + t) * V; }
     __device__ __forceinline__ int first(int c) const { return (int)place(c) - (int)shift; }
     __device__ __forceinline__ bool whole(int c) const {
@@ -76,33 +83,50 @@ struct NormRow {
     __device__ __forceinline__ bool has(int c, int i) const {
         return (uint32_t)(first(c) + i) < d;  // below 0 wraps past d
     }
-    // Requests the row; places outside it are 0.
-    __device__ __forceinline__ void load(const T *row, Raw *q) const {
+    __device__ __forceinline__ bool edge(int c) const { return edges >> c & 1; }
+    // Whether row r's outer chunks may reach past the tensor's first or last element.
+    __device__ __forceinline__ bool ends(uint64_t r, uint32_t rows) const {
+        return V > 1 && (r * d < V || (rows - 1 - r) * d < V);
+    }
+    // Requests the row. A chunk that it shares with a neighbouring row is read whole and masked later,
+    // or, where it may reach past the tensor (`ends`), element by element.
+    __device__ __forceinline__ void load(const T *row, bool ends, Raw *q) const {
 #pragma unroll
         for (int c = 0; c < N; c++) {
             if constexpr (V == 1) {
-                q[c] = whole(c) ? row[place(c)] : T(0.0f);
+                q[c] = place(c) < d ? row[place(c)] : T(0.0f);
             } else {
-                q[c] = make_uint4(0, 0, 0, 0);
-                if (whole(c)) {
+                if (!edge(c) || (ends ? whole(c) : some(c))) {
                     q[c] = *reinterpret_cast<const uint4 *>(row + first(c));
-                } else if (some(c)) {
-                    T e[V];
+                } else {
+                    q[c] = make_uint4(0, 0, 0, 0);
+                    if (some(c)) {
+                        T e[V];
 #pragma unroll
-                    for (int i = 0; i < V; i++) e[i] = has(c, i) ? row[first(c) + i] : T(0.0f);
-                    memcpy(&q[c], e, 16);
+                        for (int i = 0; i < V; i++) e[i] = has(c, i) ? row[first(c) + i] : T(0.0f);
+                        memcpy(&q[c], e, 16);
+                    }
                 }
             }
         }
     }
-    static __device__ __forceinline__ void unpack(const Raw &q, float *v) {
-        if constexpr (V == 1)
+    // Chunk c as f32, 0 outside the row.
+    __device__ __forceinline__ void unpack(const Raw &q, int c, float *v) const {
+        if constexpr (V == 1) {
             v[0] = static_cast<float>(q);
-        else
+        } else {
             Elem<T, V>::load(reinterpret_cast<const T *>(&q), v);
+            mask(c, v);
+        }
+    }
+    // 0 outside the row.
+    __device__ __forceinline__ void mask(int c, float *v) const {
+        if (edge(c))
+#pragma unroll
+            for (int i = 0; i < V; i++) v[i] = has(c, i) ? v[i] : 0.0f;
     }
     __device__ __forceinline__ void store(T *row, int c, const float *v) const {
-        if (whole(c)) {
+        if (!edge(c) || whole(c)) {
             Elem<T, V>::store(row + first(c), v);
         } else if (V > 1 && some(c)) {
 #pragma unroll
@@ -111,6 +135,15 @@ struct NormRow {
         }
     }
 };
+
+// The sum of v[0..E), two running sums side by side.
+template <int E>
+__device__ __forceinline__ float norm_add_up(const float *v) {
+    float s[2] = {v[0], v[1]};
+#pragma unroll
+    for (int i = 2; i < E; i += 2) add2(s, s, v + i);
+    return s[0] + s[1];
+}
 
 // gamma or beta in shared memory at the places the rows' elements have, 0 outside the row. Eight a
 // chunk are kept as two arrays of four, so that a warp's 16-byte reads are free of bank conflicts.
@@ -152,71 +185,78 @@ template <class T, int V, int G, int E>
 __global__ void __launch_bounds__(NORM_BLOCK<G>) norm_kernel(const NormParams p) {
     constexpr int THREADS = NORM_BLOCK<G>, GROUPS = THREADS / G;
     using Row = NormRow<T, V, G, E>;
-    __shared__ float2 part[THREADS / 32];
+    __shared__ float part[THREADS / 32];
     extern __shared__ float params[];  // gamma, beta: G x E each
     pdl_wait();
     pdl_launch_dependents();
     const uint32_t g = threadIdx.x / G, cls = blockIdx.x % p.period, step = gridDim.x / p.period * GROUPS;
     const T *x = static_cast<const T *>(p.x);
-    Row row;
-    row.t = threadIdx.x % G;
-    row.d = p.d;
-    row.shift = V == 1 ? 0 : (uint32_t)(reinterpret_cast<uintptr_t>(x + (size_t)cls * p.ldx) % 16 / sizeof(T));
+    const Row row(threadIdx.x % G,
+                  V == 1 ? 0 : (uint32_t)(reinterpret_cast<uintptr_t>(x + (size_t)cls * p.ldx) % 16 / sizeof(T)), p.d);
     // Row i of this group is row cls + i period; a group that is out of rows keeps its block's company.
     uint32_t i = blockIdx.x / p.period * GROUPS + g;
     auto at = [&](uint32_t k) { return (uint64_t)cls + (uint64_t)k * p.period; };
+    auto fetch = [&](uint64_t r, typename Row::Raw *q) {
+        if (r < p.rows) row.load(x + r * p.ldx, row.ends(r, p.rows), q);
+    };
     typename Row::Raw raw[Row::N];
-    if (at(i) < p.rows) row.load(x + at(i) * p.ldx, raw);
+    fetch(at(i), raw);
     float *gs = params, *bs = params + G * E;
     norm_stage_param<V, G, E>(gs, p.gamma, row.shift, p.d, THREADS);
     norm_stage_param<V, G, E>(bs, p.beta, row.shift, p.d, THREADS);
     __syncthreads();
     const float inv_d = 1.0f / (float)p.d;
     for (uint32_t k = blockIdx.x / p.period * GROUPS; at(k) < p.rows; k += step, i += step) {
-        const bool mine = at(i) < p.rows;
+        const uint64_t r = at(i);
+        const bool mine = r < p.rows;
         if (G == 32 && !mine) break;  // a warp by itself
         float v[E];
-        float s = 0.0f, none = 0.0f;
 #pragma unroll
-        for (int c = 0; c < Row::N; c++) {
-            Row::unpack(raw[c], v + c * V);
+        for (int c = 0; c < Row::N; c++) row.unpack(raw[c], c, v + c * V);
+        fetch(at(i + step), raw);
+        float s[1] = {norm_add_up<E>(v)};
+        norm_sum<G>(s, part);
+        const float mean = s[0] * inv_d, off[2] = {-mean, -mean};
+        float q[2] = {0.0f, 0.0f};
+        if constexpr (V == 1) {
 #pragma unroll
-            for (int e = 0; e < V; e++) s += v[c * V + e];
-        }
-        if (at(i + step) < p.rows) row.load(x + at(i + step) * p.ldx, raw);
-        norm_sum2<G>(s, none, part);
-        const float mean = s * inv_d;
-        s = 0.0f;
+            for (int c = 0; c < E; c++) {
+                v[c] = row.place(c) < p.d ? v[c] - mean : 0.0f;
+                q[c & 1] = fmaf(v[c], v[c], q[c & 1]);
+            }
+        } else {
 #pragma unroll
-        for (int c = 0; c < Row::N; c++) {
-            if (row.whole(c)) {
+            for (int c = 0; c < Row::N; c++) {
 #pragma unroll
-                for (int e = 0; e < V; e++) {
-                    const float u = v[c * V + e] - mean;
-                    s = fmaf(u, u, s);
-                }
-            } else if (V > 1 && row.some(c)) {
+                for (int e = 0; e < V; e += 2) add2(v + c * V + e, v + c * V + e, off);
+                row.mask(c, v + c * V);
 #pragma unroll
-                for (int e = 0; e < V; e++) {
-                    const float u = row.has(c, e) ? v[c * V + e] - mean : 0.0f;
-                    s = fmaf(u, u, s);
-                }
+                for (int e = 0; e < V; e += 2) fma2(q, v + c * V + e, v + c * V + e, q);
             }
         }
-        norm_sum2<G>(s, none, part);
-        const float rstd = rsqrtf(s * inv_d + p.eps);
+        s[0] = q[0] + q[1];
+        norm_sum<G>(s, part);
+        const float rstd = rsqrtf(s[0] * inv_d + p.eps), by[2] = {rstd, rstd};
         if (!mine) continue;
-        T *out = static_cast<T *>(p.y) + at(i) * p.ldy;
+        T *out = static_cast<T *>(p.y) + r * p.ldy;
 #pragma unroll
         for (int c = 0; c < Row::N; c++) {
             float ga[V], be[V];
             norm_param<V, G, E>(gs, row.place(c), ga);
             norm_param<V, G, E>(bs, row.place(c), be);
+            if constexpr (V == 1) {
+                v[c] = fmaf(v[c] * rstd, ga[0], be[0]);
+                if (row.place(c) < p.d) out[row.place(c)] = static_cast<T>(v[c]);
+            } else {
 #pragma unroll
-            for (int e = 0; e < V; e++) v[c * V + e] = fmaf((v[c * V + e] - mean) * rstd, ga[e], be[e]);
-            row.store(out, c, v + c * V);
+                for (int e = 0; e < V; e += 2) {
+                    mul2(v + c * V + e, v + c * V + e, by);
+                    fma2(v + c * V + e, v + c * V + e, ga + e, be + e);
+                }
+                row.store(out, c, v + c * V);
+            }
         }
-        if (p.stats && row.t == 0) *reinterpret_cast<float2 *>(p.stats + 2 * at(i)) = make_float2(mean, rstd);
+        if (p.stats && row.t == 0) *reinterpret_cast<float2 *>(p.stats + 2 * r) = make_float2(mean, rstd);
     }
 }
 
@@ -231,35 +271,37 @@ struct NormBwdParams {
     uint32_t rows, d, period;
     void *dx;
     size_t lddx;
-    float *ws;  // [gridDim.x][2][d]: each block's sums for dgamma and dbeta (nullptr: neither is wanted)
+    float *ws;  // [gridDim.x][2][d]: each block's sums for dgamma and dbeta
+    float *dgamma, *dbeta;  // either may be nullptr
 };
 
 // A block's groups keep their sums for dgamma and dbeta in registers over all their rows and add them
-// up in shared memory once, group after group; one row of sums a block goes to ws.
+// up in shared memory once, group after group; one row of sums a block goes to ws, or, from a block
+// alone, to dgamma and dbeta themselves.
 template <class T, int V, int G, int E>
 __global__ void __launch_bounds__(NORM_BWD_BLOCK<T, V, G, E>, 1) norm_bwd_kernel(const NormBwdParams p) {
     constexpr int THREADS = NORM_BWD_BLOCK<T, V, G, E>, GROUPS = THREADS / G;
     using Row = NormRow<T, V, G, E>;
-    __shared__ float2 part[THREADS / 32];
+    __shared__ float part[2 * THREADS / 32];
     extern __shared__ float smem[];  // gamma [G E], then the groups' sums [GROUPS][2][G E]
     pdl_wait();
     pdl_launch_dependents();
     const uint32_t g = threadIdx.x / G, cls = blockIdx.x % p.period, step = gridDim.x / p.period * GROUPS;
     const T *x = static_cast<const T *>(p.x), *dy = static_cast<const T *>(p.dy);
-    Row row;
-    row.t = threadIdx.x % G;
-    row.d = p.d;
-    row.shift = V == 1 ? 0 : (uint32_t)(reinterpret_cast<uintptr_t>(x + (size_t)cls * p.ldx) % 16 / sizeof(T));
+    const Row row(threadIdx.x % G,
+                  V == 1 ? 0 : (uint32_t)(reinterpret_cast<uintptr_t>(x + (size_t)cls * p.ldx) % 16 / sizeof(T)), p.d);
     uint32_t i = blockIdx.x / p.period * GROUPS + g;
     auto at = [&](uint32_t k) { return (uint64_t)cls + (uint64_t)k * p.period; };
     typename Row::Raw rx[Row::N], rdy[Row::N], radd[Row::N];
     float2 st = make_float2(0.0f, 0.0f);
     auto fetch = [&](uint64_t r) {
-        row.load(x + r * p.ldx, rx);
-        row.load(dy + r * p.lddy, rdy);
+        if (r >= p.rows) return;
+        const bool ends = row.ends(r, p.rows);
+        row.load(x + r * p.ldx, ends, rx);
+        row.load(dy + r * p.lddy, ends, rdy);
         st = *reinterpret_cast<const float2 *>(p.stats + 2 * r);
     };
-    if (at(i) < p.rows) fetch(at(i));
+    fetch(at(i));
     norm_stage_param<V, G, E>(smem, p.gamma, row.shift, p.d, THREADS);
     __syncthreads();
     float dg[E], db[E];
@@ -267,57 +309,73 @@ __global__ void __launch_bounds__(NORM_BWD_BLOCK<T, V, G, E>, 1) norm_bwd_kernel
     for (int e = 0; e < E; e++) dg[e] = db[e] = 0.0f;
     const float inv_d = 1.0f / (float)p.d;
     for (uint32_t k = blockIdx.x / p.period * GROUPS; at(k) < p.rows; k += step, i += step) {
-        const bool mine = at(i) < p.rows;
-        if (G == 32 && !mine) break;  // a warp by itself
         const uint64_t r = at(i);
-        const float mean = st.x, rstd = st.y;
+        const bool mine = r < p.rows;
+        if (G == 32 && !mine) break;  // a warp by itself
+        const float rstd = st.y, by[2] = {rstd, rstd}, off[2] = {-st.x * rstd, -st.x * rstd};
         float xh[E], u[E];
-        float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int c = 0; c < Row::N; c++) {
-            Row::unpack(rx[c], xh + c * V);
-            Row::unpack(rdy[c], u + c * V);
+            row.unpack(rx[c], c, xh + c * V);
+            row.unpack(rdy[c], c, u + c * V);
         }
-        if (mine && p.add) row.load(static_cast<const T *>(p.add) + r * p.ldadd, radd);
-        if (at(i + step) < p.rows) fetch(at(i + step));
+        if (mine && p.add) row.load(static_cast<const T *>(p.add) + r * p.ldadd, row.ends(r, p.rows), radd);
+        fetch(at(i + step));
+        float s[2] = {0.0f, 0.0f}, s2[2] = {0.0f, 0.0f};
         if (mine) {
 #pragma unroll
-            for (int c = 0; c < Row::N; c++) {
-                float ga[V];
+            for (int c = 0; c < Row::N; c += V == 1 ? 2 : 1) {
+                constexpr int W = V == 1 ? 2 : V;  // elements worked on together
+                float ga[W];
                 norm_param<V, G, E>(smem, row.place(c), ga);
+                if constexpr (V == 1) norm_param<V, G, E>(smem, row.place(c + 1), ga + 1);
 #pragma unroll
-                for (int e = 0; e < V; e++) {
+                for (int e = 0; e < W; e += 2) {
                     // Outside the row dy and gamma are 0: nothing is added there.
                     const int j = c * V + e;
-                    xh[j] = (xh[j] - mean) * rstd;
-                    dg[j] = fmaf(u[j], xh[j], dg[j]);
-                    db[j] += u[j];
-                    u[j] *= ga[e];
-                    s1 += u[j];
-                    s2 = fmaf(u[j], xh[j], s2);
+                    fma2(xh + j, xh + j, by, off);
+                    fma2(dg + j, u + j, xh + j, dg + j);
+                    add2(db + j, db + j, u + j);
+                    mul2(u + j, u + j, ga + e);
+                    add2(s, s, u + j);
+                    fma2(s2, u + j, xh + j, s2);
                 }
             }
         }
-        norm_sum2<G>(s1, s2, part);
+        float both[2] = {s[0] + s[1], s2[0] + s2[1]};
+        norm_sum<G>(both, part);
         if (!mine) continue;
-        s1 *= inv_d;
-        s2 *= inv_d;
+        // dx = rstd u - rstd (s1 + xh s2) [+ add]
+        const float m1 = -both[0] * inv_d * rstd, m2 = -both[1] * inv_d * rstd, a1[2] = {m1, m1}, a2[2] = {m2, m2};
         T *out = static_cast<T *>(p.dx) + r * p.lddx;
 #pragma unroll
-        for (int c = 0; c < Row::N; c++) {
-            float o[V];
-#pragma unroll
-            for (int e = 0; e < V; e++) o[e] = rstd * (u[c * V + e] - s1 - xh[c * V + e] * s2);
+        for (int c = 0; c < Row::N; c += V == 1 ? 2 : 1) {
+            constexpr int W = V == 1 ? 2 : V;
+            float o[W];
             if (p.add) {
-                float a[V];
-                Row::unpack(radd[c], a);
-#pragma unroll
-                for (int e = 0; e < V; e++) o[e] += a[e];
+                row.unpack(radd[c], c, o);
+                if constexpr (V == 1) row.unpack(radd[c + 1], c + 1, o + 1);
             }
-            row.store(out, c, o);
+#pragma unroll
+            for (int e = 0; e < W; e += 2) {
+                const int j = c * V + e;
+                float h[2];
+                fma2(h, xh + j, a2, a1);
+                fma2(h, u + j, by, h);
+                if (p.add)
+                    add2(o + e, o + e, h);
+                else
+                    o[e] = h[0], o[e + 1] = h[1];
+            }
+            if constexpr (V == 1) {
+                if (row.place(c) < p.d) out[row.place(c)] = static_cast<T>(o[0]);
+                if (row.place(c + 1) < p.d) out[row.place(c + 1)] = static_cast<T>(o[1]);
+            } else {
+                row.store(out, c, o);
+            }
         }
     }
-    if (!p.ws) return;
+    if (!p.dgamma && !p.dbeta) return;
     // Every group's sums into shared memory (chunk order, conflict-free), then one thread a column.
     float *sums = smem + G * E;
 #pragma unroll
@@ -336,7 +394,8 @@ __global__ void __launch_bounds__(NORM_BWD_BLOCK<T, V, G, E>, 1) norm_bwd_kernel
         }
     }
     __syncthreads();
-    float *out = p.ws + (size_t)blockIdx.x * 2 * p.d;
+    const bool alone = gridDim.x == 1;
+    float *og = alone ? p.dgamma : p.ws + (size_t)blockIdx.x * 2 * p.d, *ob = alone ? p.dbeta : og + p.d;
     for (uint32_t j = threadIdx.x; j < p.d; j += THREADS) {
         const uint32_t k = norm_param_at<V, G, E>(j + row.shift);
         float a = 0.0f, b = 0.0f;
@@ -345,8 +404,8 @@ __global__ void __launch_bounds__(NORM_BWD_BLOCK<T, V, G, E>, 1) norm_bwd_kernel
             a += sums[(size_t)(2 * q) * G * E + k];
             b += sums[(size_t)(2 * q + 1) * G * E + k];
         }
-        out[j] = a;
-        out[p.d + j] = b;
+        if (og) og[j] = a;
+        if (ob) ob[j] = b;
     }
 }
 

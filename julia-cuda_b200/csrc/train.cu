@@ -18,10 +18,27 @@
 namespace jc {
 
 static int sm_count() {
+    static std::atomic<int> known[64];
     int dev = 0, sms = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess)
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (cudaGetDevice(&dev) != cudaSuccess) return sms;
+    const int k = known[dev & 63].load();
+    if (k > 0) return k;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) known[dev & 63].store(sms);
     return sms;
+}
+
+// Blocks of a kernel that an SM holds (asked once: the kernels run on one architecture).
+template <class K>
+static bool blocks_per_sm(K kern, int threads, int smem, std::atomic<int> &known, int *n) {
+    *n = known.load();
+    if (*n > 0) return true;
+    if (!cuda_ok(cudaOccupancyMaxActiveBlocksPerMultiprocessor(n, kern, threads, (size_t)smem), "occupancy")) return false;
+    if (*n <= 0) {
+        set_error("a kernel does not fit an SM");
+        return false;
+    }
+    known.store(*n);
+    return true;
 }
 
 static bool aligned16(const void *p, size_t ld, size_t size) {
@@ -101,12 +118,8 @@ bool launch_norm(const NormArgs &a, cudaStream_t s) {
             const int smem = 2 * G * E * (int)sizeof(float);
             auto go = [&](auto kern, std::atomic<uint64_t> &set, std::atomic<int> &resident) {
                 if (!ensure_smem(kern, smem, set)) return false;
-                int per_sm = resident.load();
-                if (per_sm == 0) {
-                    if (!cuda_ok(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, THREADS, smem), "occupancy"))
-                        return false;
-                    resident.store(per_sm);
-                }
+                int per_sm = 0;
+                if (!blocks_per_sm(kern, THREADS, smem, resident, &per_sm)) return false;
                 const dim3 grid(norm_blocks(a.rows, THREADS / G, l.period, (uint32_t)(sm_count() * per_sm)));
                 return launch_ex(kern, grid, dim3(THREADS), smem, s, true, "layer_norm", p);
             };
@@ -121,8 +134,12 @@ bool launch_norm(const NormArgs &a, cudaStream_t s) {
 // blocks more than rows: a multiple of the period).
 constexpr uint32_t NORM_BWD_BLOCKS = 148;
 
+// A few rows take one block, which then writes dgamma and dbeta without a second kernel: 3 us less
+// of launches than it costs to have a group take NORM_BWD_ALONE rows one after the other.
+constexpr uint32_t NORM_BWD_ALONE = 8;
+
 size_t norm_bwd_ws_floats(uint32_t rows, uint32_t d) {
-    return rows ? (size_t)std::min(rows + 7, NORM_BWD_BLOCKS) * 2 * d : 0;
+    return rows > NORM_BWD_ALONE ? (size_t)std::min(rows + 7, NORM_BWD_BLOCKS) * 2 * d : 0;
 }
 
 static bool launch_column_sum(const float *ws, uint32_t parts, uint32_t n, uint32_t columns, float *a,
@@ -137,14 +154,15 @@ bool launch_norm_bwd(const NormBwdArgs &a, cudaStream_t s) {
     if (a.rows > 0) {
         const bool ok = with_type(a.type, [&](auto t) {
             using T = decltype(t);
-            const NormLayout l = norm_layout(a.d, sizeof(T), {{a.x, a.ldx}, {a.dy, a.lddy}, {a.dx, a.lddx}, {a.add, a.ldadd}});
+            NormLayout l = norm_layout(a.d, sizeof(T), {{a.x, a.ldx}, {a.dy, a.lddy}, {a.dx, a.lddx}, {a.add, a.ldadd}});
+            if (a.rows <= NORM_BWD_ALONE && l.period > 1) l = NormLayout{false, 1, a.d};  // one class of rows only
             return with_group(l.span, [&](auto g, auto e) {
                 constexpr int G = g, E = e;
                 const NormBwdParams p{a.dy, a.lddy, a.x, a.ldx, a.gamma, a.stats, a.add, a.ldadd, a.rows,
-                                      a.d, l.period, a.dx, a.lddx, sums ? a.ws : nullptr};
+                                      a.d, l.period, a.dx, a.lddx, a.ws, a.dgamma, a.dbeta};
                 auto go = [&](auto kern, std::atomic<uint64_t> &set, int threads) {
                     const int groups = threads / G, smem = (1 + 2 * groups) * G * E * (int)sizeof(float);
-                    blocks = norm_blocks(a.rows, groups, l.period, NORM_BWD_BLOCKS);
+                    blocks = a.rows <= NORM_BWD_ALONE ? 1 : norm_blocks(a.rows, groups, l.period, NORM_BWD_BLOCKS);
                     return ensure_smem(kern, smem, set) &&
                            launch_ex(kern, dim3(blocks), dim3(threads), smem, s, true, "layer_norm_backward", p);
                 };
@@ -155,7 +173,7 @@ bool launch_norm_bwd(const NormBwdArgs &a, cudaStream_t s) {
         });
         if (!ok) return false;
     }
-    return !sums || launch_column_sum(a.ws, blocks, a.d, 2 * a.d, a.dgamma, a.dbeta, s);
+    return !sums || blocks == 1 || launch_column_sum(a.ws, blocks, a.d, 2 * a.d, a.dgamma, a.dbeta, s);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -566,8 +584,15 @@ bool launch_adamw(const AdamwStep &a, cudaStream_t s) {
     p.eps = a.eps;
     p.inv_bias1 = (float)(1.0 / (1.0 - std::pow(a.beta1, (double)a.step)));
     p.inv_bias2 = (float)(1.0 / (1.0 - std::pow(a.beta2, (double)a.step)));
-    return a.bits == 8 ? launch_ex(adamw_kernel<8>, dim3(a.n_chunks), dim3(ADAMW_THREADS), 0, s, true, "adamw", p)
-                       : launch_ex(adamw_kernel<32>, dim3(a.n_chunks), dim3(ADAMW_THREADS), 0, s, true, "adamw", p);
+    p.n_chunks = a.n_chunks;
+    auto go = [&](auto kern, std::atomic<int> &resident) {
+        int per_sm = 0;
+        if (!blocks_per_sm(kern, ADAMW_THREADS, 0, resident, &per_sm)) return false;
+        const uint32_t grid = std::min(a.n_chunks, (uint32_t)(sm_count() * per_sm));
+        return launch_ex(kern, dim3(grid), dim3(ADAMW_THREADS), 0, s, true, "adamw", p);
+    };
+    static std::atomic<int> res_8{0}, res_32{0};
+    return a.bits == 8 ? go(adamw_kernel<8>, res_8) : go(adamw_kernel<32>, res_32);
 }
 
 }  // namespace jc

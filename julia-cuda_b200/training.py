@@ -56,7 +56,7 @@ def _type(op: str, t, halves: bool = False) -> int:
 
 def _scratch(n: int, dtype, like, stream):
     """Scratch of the allocator's own, which must not reuse it before `stream` is done with it."""
-    ws = torch.empty(max(n, 1), dtype=dtype, device=like.device)
+    ws = torch.empty(n, dtype=dtype, device=like.device)
     if stream is not None:
         ws.record_stream(stream if isinstance(stream, torch.cuda.Stream)
                          else torch.cuda.ExternalStream(stream))
@@ -90,14 +90,15 @@ def layer_norm_backward(dy, x, gamma, stats, dx, dgamma=None, dbeta=None, add=No
     dxp, lddx = _matrix(op, "dx", dx, rows, d, x.dtype)
     ap, ldadd = _matrix(op, "add", add, rows, d, x.dtype)
     need = lib().jc_layer_norm_ws_floats(rows, d) if dgamma is not None or dbeta is not None else 0
-    if ws is None:
+    if need and ws is None:
         ws = _scratch(need, torch.float32, x, stream)
-    elif ws.numel() < need:
+    elif need and ws.numel() < need:
         _fail(f"{op}: ws needs {need} floats")
     _check(lib().jc_layer_norm_backward(t, dyp, lddy, xp, ldx, _vector(op, "gamma", gamma, d),
                                         _vector(op, "stats", stats, 2 * rows), ap, ldadd, rows, d,
                                         dxp, lddx, _vector(op, "dgamma", dgamma, d),
-                                        _vector(op, "dbeta", dbeta, d), ws.data_ptr(),
+                                        _vector(op, "dbeta", dbeta, d),
+                                        ws.data_ptr() if need else None,
                                         _stream(stream)), "jc_layer_norm_backward")
 
 
@@ -141,12 +142,12 @@ def linear_backward(dy, x, w, *, z=None, act: str = "none", dx=None, dw=None, db
     dxp, lddx = _matrix(op, "dx", dx, m, k, x.dtype)
     dwp, lddw = _matrix(op, "dw", dw, n, k, x.dtype)
     need = lib().jc_linear_ws_bytes(m, n, k)
-    if ws is None:
+    if need and ws is None:
         ws = _scratch(need, torch.uint8, x, stream)
-    elif ws.numel() * ws.element_size() < need:
+    elif need and ws.numel() * ws.element_size() < need:
         _fail(f"{op}: ws needs {need} bytes")
     _check(lib().jc_linear_backward(t, a, dyp, lddy, xp, ldx, wp, ldw, zp, ldz, m, n, k, dxp, lddx,
-                                    dwp, lddw, _vector(op, "dbias", dbias, n), ws.data_ptr(),
+                                    dwp, lddw, _vector(op, "dbias", dbias, n), ws.data_ptr() if need else None,
                                     _stream(stream)), "jc_linear_backward")
 
 

@@ -36,7 +36,7 @@ def test_layer_norm_backward_refusals(jc, buf):
                                         None)
     for kw, why in ((dict(type=9), "element type"), (dict(dy=None), "dy is null"), (dict(x=None), "x is null"),
                     (dict(stats=None), "stats is null"), (dict(dx=None), "dx is null"), (dict(lddx=4), "overlap"),
-                    (dict(add=p, ldadd=3), "add"), (dict(ws=None), "ws is null"), (dict(dg=p + 1), "dgamma")):
+                    (dict(add=p, ldadd=3), "add"), (dict(ws=None, rows=100), "ws is null"), (dict(dg=p + 1), "dgamma")):
         assert call(**kw) == -1 and why in jc.last_error(), (kw, jc.last_error())
     assert L.jc_layer_norm_ws_floats(100000, 768) >= 2 * 768
 
