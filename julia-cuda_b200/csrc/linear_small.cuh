@@ -250,11 +250,11 @@ __global__ void __launch_bounds__(256) linear_thin_bwd_kernel(const LinearThinBw
     }
 }
 
-// dw [n][k] and dbias [n] from the blocks' sums: 32 columns a block, eight threads a column.
+// dw [n][k] and dbias [n] from the blocks' sums: 32 columns a block, 32 threads a column.
 template <class T>
-__global__ void __launch_bounds__(256) linear_thin_finish_kernel(const float *part, uint32_t parts, uint32_t n,
+__global__ void __launch_bounds__(1024) linear_thin_finish_kernel(const float *part, uint32_t parts, uint32_t n,
                                                                  uint32_t k, T *dw, size_t lddw, float *dbias) {
-    __shared__ float s[8][32];
+    __shared__ float s[32][32];
     pdl_wait();
     pdl_launch_dependents();
     const uint32_t c = threadIdx.x & 31, g = threadIdx.x >> 5, j = blockIdx.x * 32 + c, all = n * k + n;
@@ -262,12 +262,12 @@ __global__ void __launch_bounds__(256) linear_thin_finish_kernel(const float *pa
     float v = 0.0f;
     if (want)
 #pragma unroll 4
-        for (uint32_t i = g; i < parts; i += 8) v += part[(size_t)i * all + j];
+        for (uint32_t i = g; i < parts; i += 32) v += part[(size_t)i * all + j];
     s[g][c] = v;
     __syncthreads();
     if (g != 0 || !want) return;
 #pragma unroll
-    for (int i = 1; i < 8; i++) v += s[i][c];
+    for (int i = 1; i < 32; i++) v += s[i][c];
     if (j < n * k)
         dw[(size_t)(j / k) * lddw + j % k] = static_cast<T>(v);
     else

@@ -28,12 +28,13 @@ namespace jc {
 
 constexpr int NORM_MAX_D = 16384;
 
-// Threads of a block whose rows take G threads each. Backward: as many as the registers of a row's
-// four f32 copies (x, dy and the two sums) and the next row's raw elements allow on one SM.
+// Threads of a forward block whose rows take G threads each.
 template <int G>
 constexpr int NORM_BLOCK = G > 128 ? G : 128;
-template <class T, int V, int G, int E>
-constexpr int NORM_BWD_BLOCK = G > 256 ? G : sizeof(T) == 2 && V > 1 && E <= 24 ? 384 : 256;
+// Forward blocks an SM should hold: what the registers of a row (f32, and the next row's raw elements)
+// allow; left to itself the compiler takes more registers than it needs.
+template <int V, int G, int E>
+constexpr int NORM_RESIDENT = G >= 256 ? 1 : E == 8 ? 10 : E == 16 ? 8 : E == 24 ? (V == 1 ? 5 : 6) : V == 1 ? 4 : 5;
 
 // Sums over the G threads of a row's group, in a fixed order: K values at once. `part`: K floats a warp
 // in shared memory; G > 32: every thread of the block calls it.
@@ -110,6 +111,16 @@ struct NormRow {
             }
         }
     }
+    // Chunk c of a row in global memory as f32, 0 outside the row.
+    __device__ __forceinline__ void chunk(const T *row, int c, bool ends, float *v) const {
+        if (!edge(c) || (ends ? whole(c) : some(c))) {
+            Elem<T, V>::load(row + first(c), v);
+            mask(c, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; i++) v[i] = has(c, i) ? static_cast<float>(row[first(c) + i]) : 0.0f;
+        }
+    }
     // Chunk c as f32, 0 outside the row.
     __device__ __forceinline__ void unpack(const Raw &q, int c, float *v) const {
         if constexpr (V == 1) {
@@ -182,7 +193,7 @@ struct NormParams {
 };
 
 template <class T, int V, int G, int E>
-__global__ void __launch_bounds__(NORM_BLOCK<G>) norm_kernel(const NormParams p) {
+__global__ void __launch_bounds__(NORM_BLOCK<G>, NORM_RESIDENT<V, G, E>) norm_kernel(const NormParams p) {
     constexpr int THREADS = NORM_BLOCK<G>, GROUPS = THREADS / G;
     using Row = NormRow<T, V, G, E>;
     __shared__ float part[THREADS / 32];
@@ -273,110 +284,194 @@ struct NormBwdParams {
     size_t lddx;
     float *ws;  // [gridDim.x][2][d]: each block's sums for dgamma and dbeta
     float *dgamma, *dbeta;  // either may be nullptr
+    unsigned int *err;
 };
+
+// How a block of the backward kernel is made up. Rows of x, dy and add come into shared memory by bulk
+// copies, STAGES rows ahead, each group its own; a row is then read twice from there, which leaves the
+// registers to the two running sums. Held in registers instead, with the next row's raw elements, a
+// row cost 170 registers a thread, and twelve warps a SM moved 4.1 TB/s at 1000 elements a row.
+// STAGES 0 (V = 1, and f32 rows too wide for the ring): each pass reads global memory.
+template <class T, int V, int G, int E>
+struct NormBwdShape {
+    static constexpr int ROW = G * E * (int)sizeof(T);  // bytes
+    static constexpr int STAGES = V == 1 || ROW > 32768 ? 0 : ROW * 2 > 32768 ? 1 : 2;
+    static constexpr int THREADS = G > 512 ? G : STAGES && ROW * (512 / G) * STAGES * 3 > 200000 ? (G > 256 ? G : 256) : 512;
+    static constexpr int GROUPS = THREADS / G;
+    static constexpr int RING = GROUPS * STAGES * 3 * ROW, SUMS = GROUPS * 2 * G * E * 4;
+    static constexpr int SMEM = G * E * 4 + (RING > SUMS ? RING : SUMS);  // gamma, then the ring, later the sums
+    static_assert(SMEM <= 227 * 1024 - 1024, "shared memory");
+};
+
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
 
 // A block's groups keep their sums for dgamma and dbeta in registers over all their rows and add them
 // up in shared memory once, group after group; one row of sums a block goes to ws, or, from a block
 // alone, to dgamma and dbeta themselves.
 template <class T, int V, int G, int E>
-__global__ void __launch_bounds__(NORM_BWD_BLOCK<T, V, G, E>, 1) norm_bwd_kernel(const NormBwdParams p) {
-    constexpr int THREADS = NORM_BWD_BLOCK<T, V, G, E>, GROUPS = THREADS / G;
+__global__ void __launch_bounds__(NormBwdShape<T, V, G, E>::THREADS, 1) norm_bwd_kernel(const NormBwdParams p) {
+    using S = NormBwdShape<T, V, G, E>;
     using Row = NormRow<T, V, G, E>;
+    constexpr int THREADS = S::THREADS, GROUPS = S::GROUPS, STAGES = S::STAGES;
     __shared__ float part[2 * THREADS / 32];
-    extern __shared__ float smem[];  // gamma [G E], then the groups' sums [GROUPS][2][G E]
-    pdl_wait();
-    pdl_launch_dependents();
+    __shared__ uint64_t bars[GROUPS * (STAGES ? STAGES : 1)];
+    extern __shared__ __align__(16) float smem[];
+    dev_err_bind(p.err);
     const uint32_t g = threadIdx.x / G, cls = blockIdx.x % p.period, step = gridDim.x / p.period * GROUPS;
-    const T *x = static_cast<const T *>(p.x), *dy = static_cast<const T *>(p.dy);
+    const T *x = static_cast<const T *>(p.x), *dy = static_cast<const T *>(p.dy), *add = static_cast<const T *>(p.add);
     const Row row(threadIdx.x % G,
                   V == 1 ? 0 : (uint32_t)(reinterpret_cast<uintptr_t>(x + (size_t)cls * p.ldx) % 16 / sizeof(T)), p.d);
     uint32_t i = blockIdx.x / p.period * GROUPS + g;
     auto at = [&](uint32_t k) { return (uint64_t)cls + (uint64_t)k * p.period; };
-    typename Row::Raw rx[Row::N], rdy[Row::N], radd[Row::N];
-    float2 st = make_float2(0.0f, 0.0f);
-    auto fetch = [&](uint64_t r) {
-        if (r >= p.rows) return;
-        const bool ends = row.ends(r, p.rows);
-        row.load(x + r * p.ldx, ends, rx);
-        row.load(dy + r * p.lddy, ends, rdy);
-        st = *reinterpret_cast<const float2 *>(p.stats + 2 * r);
+    uint8_t *ring = reinterpret_cast<uint8_t *>(smem + G * E) + g * (STAGES * 3 * S::ROW);
+    uint64_t *bar = bars + g * STAGES;
+    if (STAGES && row.t == 0) {
+        for (int k = 0; k < STAGES; k++) mbar_init(&bar[k], 1);
+        fence_barrier_init();
+    }
+    pdl_wait();
+    pdl_launch_dependents();
+    // One thread of a group requests a row's chunks of every tensor. Rows whose outer chunks may reach
+    // past the tensor are copied by the group itself, element by element, when their turn comes.
+    auto whole_chunks = [&](uint64_t r) { return p.period == 1 || !row.ends(r, p.rows); };
+    auto request = [&](uint64_t r, uint32_t st) {
+        if (STAGES == 0 || row.t != 0 || r >= p.rows || !whole_chunks(r)) return;
+        const uint32_t bytes = (row.shift + p.d + V - 1) / V * 16;
+        uint8_t *to = ring + st * (3 * S::ROW);
+        mbar_arrive_expect_tx(&bar[st], (p.add ? 3 : 2) * bytes);
+        bulk_load(to, x + r * p.ldx - row.shift, bytes, &bar[st]);
+        bulk_load(to + S::ROW, dy + r * p.lddy - row.shift, bytes, &bar[st]);
+        if (p.add) bulk_load(to + 2 * S::ROW, add + r * p.ldadd - row.shift, bytes, &bar[st]);
     };
-    fetch(at(i));
+#pragma unroll
+    for (int k = 0; k < STAGES; k++) request(at(i + k * step), k);
     norm_stage_param<V, G, E>(smem, p.gamma, row.shift, p.d, THREADS);
-    __syncthreads();
+    float2 next_st = at(i) < p.rows ? *reinterpret_cast<const float2 *>(p.stats + 2 * at(i)) : make_float2(0.0f, 0.0f);
+    __syncthreads();  // gamma, and the barriers
     float dg[E], db[E];
 #pragma unroll
     for (int e = 0; e < E; e++) dg[e] = db[e] = 0.0f;
     const float inv_d = 1.0f / (float)p.d;
+    uint32_t st = 0, phases = 0;  // the stage, and a bit a stage: its barrier's parity
     for (uint32_t k = blockIdx.x / p.period * GROUPS; at(k) < p.rows; k += step, i += step) {
         const uint64_t r = at(i);
         const bool mine = r < p.rows;
         if (G == 32 && !mine) break;  // a warp by itself
-        const float rstd = st.y, by[2] = {rstd, rstd}, off[2] = {-st.x * rstd, -st.x * rstd};
-        float xh[E], u[E];
-#pragma unroll
-        for (int c = 0; c < Row::N; c++) {
-            row.unpack(rx[c], c, xh + c * V);
-            row.unpack(rdy[c], c, u + c * V);
+        T *stage = reinterpret_cast<T *>(ring + st * (3 * S::ROW));
+        constexpr int ELEMS = S::ROW / (int)sizeof(T);
+        if constexpr (STAGES > 0) {
+            const bool copied = mine && whole_chunks(r);
+            if (copied) {
+                mbar_wait(&bar[st], phases >> st & 1, JC_DEV_TIMEOUT_FULL);
+                phases ^= 1u << st;
+            } else if (mine) {
+                for (uint32_t j = row.t; j < p.d; j += G) {
+                    stage[row.shift + j] = x[r * p.ldx + j];
+                    stage[ELEMS + row.shift + j] = dy[r * p.lddy + j];
+                    if (p.add) stage[2 * ELEMS + row.shift + j] = add[r * p.ldadd + j];
+                }
+            }
+            if (G == 32)
+                __syncwarp();
+            else if (p.period > 1)
+                __syncthreads();
         }
-        if (mine && p.add) row.load(static_cast<const T *>(p.add) + r * p.ldadd, row.ends(r, p.rows), radd);
-        fetch(at(i + step));
+        // Chunk c of a tensor as f32, 0 outside the row.
+        auto get = [&](int which, const T *global, int c, float *v) {
+            if constexpr (STAGES > 0) {
+                Elem<T, V>::load(stage + which * ELEMS + row.place(c), v);
+                row.mask(c, v);
+            } else if constexpr (V == 1) {
+                v[0] = row.place(c) < p.d ? static_cast<float>(global[row.place(c)]) : 0.0f;
+            } else {
+                const bool ends = p.period > 1 && row.ends(r, p.rows);
+                row.chunk(global, c, ends, v);
+            }
+        };
+        const T *xr = x + r * p.ldx, *dyr = dy + r * p.lddy, *ar = add + r * p.ldadd;
+        const float rstd = next_st.y, by[2] = {rstd, rstd}, off[2] = {-next_st.x * rstd, -next_st.x * rstd};
+        if (at(i + step) < p.rows) next_st = *reinterpret_cast<const float2 *>(p.stats + 2 * at(i + step));
+        constexpr int PER = V == 1 ? 2 : 1, W = V == 1 ? 2 : V;  // chunks, elements worked on together
         float s[2] = {0.0f, 0.0f}, s2[2] = {0.0f, 0.0f};
         if (mine) {
 #pragma unroll
-            for (int c = 0; c < Row::N; c += V == 1 ? 2 : 1) {
-                constexpr int W = V == 1 ? 2 : V;  // elements worked on together
-                float ga[W];
-                norm_param<V, G, E>(smem, row.place(c), ga);
-                if constexpr (V == 1) norm_param<V, G, E>(smem, row.place(c + 1), ga + 1);
+            for (int c = 0; c < Row::N; c += PER) {
+                float xh[W], u[W], ga[W];
+#pragma unroll
+                for (int q = 0; q < PER; q++) {
+                    get(0, xr, c + q, xh + q);
+                    get(1, dyr, c + q, u + q);
+                    norm_param<V, G, E>(smem, row.place(c + q), ga + q);
+                }
 #pragma unroll
                 for (int e = 0; e < W; e += 2) {
                     // Outside the row dy and gamma are 0: nothing is added there.
                     const int j = c * V + e;
-                    fma2(xh + j, xh + j, by, off);
-                    fma2(dg + j, u + j, xh + j, dg + j);
-                    add2(db + j, db + j, u + j);
-                    mul2(u + j, u + j, ga + e);
-                    add2(s, s, u + j);
-                    fma2(s2, u + j, xh + j, s2);
+                    fma2(xh + e, xh + e, by, off);
+                    fma2(dg + j, u + e, xh + e, dg + j);
+                    add2(db + j, db + j, u + e);
+                    mul2(u + e, u + e, ga + e);
+                    add2(s, s, u + e);
+                    fma2(s2, u + e, xh + e, s2);
                 }
             }
         }
         float both[2] = {s[0] + s[1], s2[0] + s2[1]};
         norm_sum<G>(both, part);
-        if (!mine) continue;
-        // dx = rstd u - rstd (s1 + xh s2) [+ add]
-        const float m1 = -both[0] * inv_d * rstd, m2 = -both[1] * inv_d * rstd, a1[2] = {m1, m1}, a2[2] = {m2, m2};
-        T *out = static_cast<T *>(p.dx) + r * p.lddx;
+        if (G == 32) __syncwarp();  // or the compiler keeps the first pass's f32 values, and spills
+        if (mine) {
+            // dx = rstd u - rstd (s1 + xh s2) [+ add]
+            const float m1 = -both[0] * inv_d * rstd, m2 = -both[1] * inv_d * rstd, a1[2] = {m1, m1}, a2[2] = {m2, m2};
+            T *out = static_cast<T *>(p.dx) + r * p.lddx;
 #pragma unroll
-        for (int c = 0; c < Row::N; c += V == 1 ? 2 : 1) {
-            constexpr int W = V == 1 ? 2 : V;
-            float o[W];
-            if (p.add) {
-                row.unpack(radd[c], c, o);
-                if constexpr (V == 1) row.unpack(radd[c + 1], c + 1, o + 1);
-            }
+            for (int c = 0; c < Row::N; c += PER) {
+                float o[W], xh[W], u[W], ga[W];
 #pragma unroll
-            for (int e = 0; e < W; e += 2) {
-                const int j = c * V + e;
-                float h[2];
-                fma2(h, xh + j, a2, a1);
-                fma2(h, u + j, by, h);
-                if (p.add)
-                    add2(o + e, o + e, h);
-                else
-                    o[e] = h[0], o[e + 1] = h[1];
+                for (int q = 0; q < PER; q++) {
+                    get(0, xr, c + q, xh + q);
+                    get(1, dyr, c + q, u + q);
+                    norm_param<V, G, E>(smem, row.place(c + q), ga + q);
+                    if (p.add) get(2, ar, c + q, o + q);
+                }
+#pragma unroll
+                for (int e = 0; e < W; e += 2) {
+                    float h[2];
+                    fma2(xh + e, xh + e, by, off);
+                    mul2(u + e, u + e, ga + e);
+                    fma2(h, xh + e, a2, a1);
+                    fma2(h, u + e, by, h);
+                    if (p.add)
+                        add2(o + e, o + e, h);
+                    else
+                        o[e] = h[0], o[e + 1] = h[1];
+                }
+                if constexpr (V == 1) {
+                    if (row.place(c) < p.d) out[row.place(c)] = static_cast<T>(o[0]);
+                    if (row.place(c + 1) < p.d) out[row.place(c + 1)] = static_cast<T>(o[1]);
+                } else {
+                    row.store(out, c, o);
+                }
             }
-            if constexpr (V == 1) {
-                if (row.place(c) < p.d) out[row.place(c)] = static_cast<T>(o[0]);
-                if (row.place(c + 1) < p.d) out[row.place(c + 1)] = static_cast<T>(o[1]);
-            } else {
-                row.store(out, c, o);
-            }
+        }
+        if constexpr (STAGES > 0) {
+            // The group has read the stage; the row STAGES further on may take it.
+            if (G == 32)
+                __syncwarp();
+            else
+                __syncthreads();
+            request(at(i + STAGES * step), st);
+            st = st + 1 == STAGES ? 0 : st + 1;
         }
     }
     if (!p.dgamma && !p.dbeta) return;
-    // Every group's sums into shared memory (chunk order, conflict-free), then one thread a column.
+    // Every group's sums into shared memory (chunk order, conflict-free; the rings are empty), then one
+    // thread a column.
+    __syncthreads();
     float *sums = smem + G * E;
 #pragma unroll
     for (int c = 0; c < Row::N; c++) {
@@ -399,7 +494,7 @@ __global__ void __launch_bounds__(NORM_BWD_BLOCK<T, V, G, E>, 1) norm_bwd_kernel
     for (uint32_t j = threadIdx.x; j < p.d; j += THREADS) {
         const uint32_t k = norm_param_at<V, G, E>(j + row.shift);
         float a = 0.0f, b = 0.0f;
-#pragma unroll 1
+#pragma unroll 4
         for (int q = 0; q < GROUPS; q++) {
             a += sums[(size_t)(2 * q) * G * E + k];
             b += sums[(size_t)(2 * q + 1) * G * E + k];
@@ -410,21 +505,23 @@ __global__ void __launch_bounds__(NORM_BWD_BLOCK<T, V, G, E>, 1) norm_bwd_kernel
 }
 
 // out_a[j] = sum over parts of ws[part][j], j < n, and out_b[j] the same of ws[part][n + j] (either
-// may be nullptr): 32 columns a block, eight threads a column each summing every eighth part.
-__global__ void __launch_bounds__(256) column_sum_kernel(const float *ws, uint32_t parts, uint32_t n,
+// may be nullptr): 32 columns a block, 32 threads a column each summing every 32nd part, so that all of
+// a column's reads are in flight at once.
+__global__ void __launch_bounds__(1024) column_sum_kernel(const float *ws, uint32_t parts, uint32_t n,
                                                          uint32_t columns, float *out_a, float *out_b) {
-    __shared__ float s[8][32];
+    __shared__ float s[32][32];
     pdl_wait();
     pdl_launch_dependents();
     const uint32_t c = threadIdx.x & 31, k = threadIdx.x >> 5, j = blockIdx.x * 32 + c;
     float v = 0.0f;
     if (j < columns)
-        for (uint32_t i = k; i < parts; i += 8) v += ws[(size_t)i * columns + j];
+#pragma unroll 5
+        for (uint32_t i = k; i < parts; i += 32) v += ws[(size_t)i * columns + j];
     s[k][c] = v;
     __syncthreads();
     if (k == 0 && j < columns) {
 #pragma unroll
-        for (int i = 1; i < 8; i++) v += s[i][c];
+        for (int i = 1; i < 32; i++) v += s[i][c];
         if (j < n) {
             if (out_a) out_a[j] = v;
         } else if (out_b) {

@@ -144,13 +144,15 @@ size_t norm_bwd_ws_floats(uint32_t rows, uint32_t d) {
 
 static bool launch_column_sum(const float *ws, uint32_t parts, uint32_t n, uint32_t columns, float *a,
                               float *b, cudaStream_t s) {
-    return launch_ex(column_sum_kernel, dim3((columns + 31) / 32), dim3(256), 0, s, true, "column sums", ws,
+    return launch_ex(column_sum_kernel, dim3((columns + 31) / 32), dim3(1024), 0, s, true, "column sums", ws,
                      parts, n, columns, a, b);
 }
 
 bool launch_norm_bwd(const NormBwdArgs &a, cudaStream_t s) {
     const bool sums = a.dgamma || a.dbeta;
     uint32_t blocks = 0;
+    unsigned int *err = module_error_word();
+    if (!err) return false;
     if (a.rows > 0) {
         const bool ok = with_type(a.type, [&](auto t) {
             using T = decltype(t);
@@ -159,16 +161,16 @@ bool launch_norm_bwd(const NormBwdArgs &a, cudaStream_t s) {
             return with_group(l.span, [&](auto g, auto e) {
                 constexpr int G = g, E = e;
                 const NormBwdParams p{a.dy, a.lddy, a.x, a.ldx, a.gamma, a.stats, a.add, a.ldadd, a.rows,
-                                      a.d, l.period, a.dx, a.lddx, a.ws, a.dgamma, a.dbeta};
-                auto go = [&](auto kern, std::atomic<uint64_t> &set, int threads) {
-                    const int groups = threads / G, smem = (1 + 2 * groups) * G * E * (int)sizeof(float);
-                    blocks = a.rows <= NORM_BWD_ALONE ? 1 : norm_blocks(a.rows, groups, l.period, NORM_BWD_BLOCKS);
-                    return ensure_smem(kern, smem, set) &&
-                           launch_ex(kern, dim3(blocks), dim3(threads), smem, s, true, "layer_norm_backward", p);
+                                      a.d, l.period, a.dx, a.lddx, a.ws, a.dgamma, a.dbeta, err};
+                auto go = [&](auto kern, std::atomic<uint64_t> &set, auto shape) {
+                    using S = decltype(shape);
+                    blocks = a.rows <= NORM_BWD_ALONE ? 1 : norm_blocks(a.rows, S::GROUPS, l.period, NORM_BWD_BLOCKS);
+                    return ensure_smem(kern, S::SMEM, set) &&
+                           launch_ex(kern, dim3(blocks), dim3(S::THREADS), S::SMEM, s, true, "layer_norm_backward", p);
                 };
                 static std::atomic<uint64_t> set_v{0}, set_1{0};
-                return l.chunks ? go(norm_bwd_kernel<T, VEC<T>, G, E>, set_v, NORM_BWD_BLOCK<T, VEC<T>, G, E>)
-                                : go(norm_bwd_kernel<T, 1, G, E>, set_1, NORM_BWD_BLOCK<T, 1, G, E>);
+                return l.chunks ? go(norm_bwd_kernel<T, VEC<T>, G, E>, set_v, NormBwdShape<T, VEC<T>, G, E>())
+                                : go(norm_bwd_kernel<T, 1, G, E>, set_1, NormBwdShape<T, 1, G, E>());
             });
         });
         if (!ok) return false;
@@ -464,7 +466,7 @@ static bool launch_linear_thin_bwd(const LinearBwdArgs &a, uint32_t blocks, cuda
                 return false;
         }
         if (!part) return true;
-        return launch_ex(linear_thin_finish_kernel<T>, dim3((a.n * a.k + a.n + 31) / 32), dim3(256), 0, s, true,
+        return launch_ex(linear_thin_finish_kernel<T>, dim3((a.n * a.k + a.n + 31) / 32), dim3(1024), 0, s, true,
                          "linear_backward", (const float *)part, a.m ? blocks : 0u, a.n, a.k, static_cast<T *>(a.dw),
                          a.lddw, a.dbias);
     });
