@@ -28,10 +28,9 @@ struct AdamwParams {
     float inv_bias1, inv_bias2;  // 1 / (1 - beta^t)
 };
 
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
+// The largest of a warp's values, none below 0: their bits order as they do.
+__device__ __forceinline__ float warp_max_positive(float v) {
+    return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
 }
 
 // Eight consecutive values at p[0..n) (n up to 8; `vec`: 16-byte aligned and all eight there).
@@ -73,8 +72,8 @@ __device__ __forceinline__ void load_codes(const uint8_t *p, uint32_t n, bool ve
         const uint32_t w = (i < 2 ? q.x : q.y) >> (16 * (i & 1));
         const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xFFFF), __NV_E4M3);
         const float2 f = __half22float2(__half2(h));
-        v[2 * i] = f.x * scale;
-        v[2 * i + 1] = f.y * scale;
+        const float s[2] = {scale, scale}, c[2] = {f.x, f.y};
+        mul2(v + 2 * i, c, s);
     }
 }
 
@@ -102,13 +101,15 @@ __device__ __forceinline__ float sqrt_approx(float x) {
     return y;
 }
 
-// x / s, given inv = 1 / s rounded to nearest: the product's remainder, exact in one fused
-// multiply-add, corrects it (Markstein, "Computation of elementary functions on the IBM RISC
+// x / s for a pair, given -s and inv = 1 / s rounded to nearest: the product's remainder, exact in one
+// fused multiply-add, corrects it (Markstein, "Computation of elementary functions on the IBM RISC
 // System/6000 processor", 1990). The correctly rounded quotient wherever that remainder does not
 // underflow, at a fifth of a division's instructions; below that a code is 0 either way.
-__device__ __forceinline__ float div_by(float x, float s, float inv) {
-    const float q = __fmul_rn(x, inv);
-    return __fmaf_rn(__fmaf_rn(-q, s, x), inv, q);
+__device__ __forceinline__ void div2(float *x, const float *minus_s, const float *inv) {
+    float q[2], r[2];
+    mul2(q, x, inv);
+    fma2(r, q, minus_s, x);
+    fma2(x, r, inv, q);
 }
 
 // Blocks stay and walk the chunks, eight consecutive elements a thread (a warp holds the 256 elements
@@ -160,16 +161,33 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const AdamwParams 
         ch = next;
         if (i + 2ull * gridDim.x < p.n_chunks) next = __ldg(p.chunks + i + 2 * gridDim.x);
         if (some) {
-            const float keep = 1.0f - p.lr * t.decay;
+            const float k = 1.0f - p.lr * t.decay, up = -p.lr * p.inv_bias1;
+            const float keep[2] = {k, k}, rate[2] = {up, up}, gs2[2] = {gs, gs}, b1[2] = {p.beta1, p.beta1},
+                        b2[2] = {p.beta2, p.beta2}, c1[2] = {p.one_minus_beta1, p.one_minus_beta1},
+                        c2[2] = {p.one_minus_beta2, p.one_minus_beta2}, ib2[2] = {p.inv_bias2, p.inv_bias2},
+                        eps[2] = {p.eps, p.eps};
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
+            for (int j = 0; j < 8; j += 2) {
                 // Each operation of the states rounded by itself, so that an 8-bit code does not
                 // depend on how a compiler contracts them.
-                const float gi = __fmul_rn(g[j], gs);
-                m[j] = __fadd_rn(__fmul_rn(p.beta1, m[j]), __fmul_rn(p.one_minus_beta1, gi));
-                v[j] = __fadd_rn(__fmul_rn(p.beta2, v[j]), __fmul_rn(__fmul_rn(p.one_minus_beta2, gi), gi));
+                float a[2], b[2];
+                mul2(g + j, g + j, gs2);
+                mul2(m + j, m + j, b1);
+                mul2(a, g + j, c1);
+                add2(m + j, m + j, a);
+                mul2(v + j, v + j, b2);
+                mul2(a, g + j, c2);
+                mul2(a, a, g + j);
+                add2(v + j, v + j, a);
                 // The quotient and root to a few ulp: their error is far below the parameter's own.
-                w[j] = w[j] * keep - __fdividef(p.lr * (m[j] * p.inv_bias1), sqrt_approx(v[j] * p.inv_bias2) + p.eps);
+                mul2(a, v + j, ib2);
+                a[0] = sqrt_approx(a[0]);
+                a[1] = sqrt_approx(a[1]);
+                add2(a, a, eps);
+                mul2(b, m + j, rate);
+                b[0] = __fdividef(b[0], a[0]);
+                b[1] = __fdividef(b[1], a[1]);
+                fma2(w + j, w + j, keep, b);
             }
             store8(t.p + at, n, vec, w);
             if (t.copy_type == JC_F16)
@@ -183,15 +201,18 @@ __global__ void __launch_bounds__(ADAMW_THREADS) adamw_kernel(const AdamwParams 
                     mm = fmaxf(mm, fabsf(m[j]));
                     vm = fmaxf(vm, v[j]);
                 }
-                mm = __fmul_rn(warp_max(mm), 1.0f / FP8_MAX);
-                vm = __fmul_rn(warp_max(vm), 1.0f / FP8_MAX);
+                mm = __fmul_rn(warp_max_positive(mm), 1.0f / FP8_MAX);
+                vm = __fmul_rn(warp_max_positive(vm), 1.0f / FP8_MAX);
                 const float sm = mm > 0.0f ? mm : 1.0f, sv = vm > 0.0f ? vm : 1.0f;
                 const float im = __frcp_rn(sm), iv = __frcp_rn(sv);
+                const float nsm[2] = {-sm, -sm}, nsv[2] = {-sv, -sv}, im2[2] = {im, im}, iv2[2] = {iv, iv};
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float q = div_by(v[j], sv, iv);
-                    v[j] = v[j] > 0.0f ? fmaxf(q, FP8_MIN) : v[j];
-                    m[j] = div_by(m[j], sm, im);
+                for (int j = 0; j < 8; j += 2) {
+                    const bool a = v[j] > 0.0f, b = v[j + 1] > 0.0f;
+                    div2(m + j, nsm, im2);
+                    div2(v + j, nsv, iv2);
+                    v[j] = a ? fmaxf(v[j], FP8_MIN) : v[j];
+                    v[j + 1] = b ? fmaxf(v[j + 1], FP8_MIN) : v[j + 1];
                 }
                 store_codes(static_cast<uint8_t *>(t.m) + at, n, vec, m);
                 store_codes(static_cast<uint8_t *>(t.v) + at, n, vec, v);

@@ -6,10 +6,9 @@
 //             dx = rstd (u - sum(u) / d - xh sum(u xh) / d) [+ add]
 //             dgamma = sum over rows of dy xh, dbeta = sum over rows of dy
 //
-// Both are bound by memory: each row is read once, held by G threads with E of its elements in each
-// one's registers as f32, so the mean is known before the squared deviations are summed, from the
-// same registers; the next row is requested before the current one is worked on. Blocks stay and
-// walk rows, with gamma and beta in shared memory.
+// Both are bound by memory: each row is read from it once, by bulk copies into shared memory a row or
+// two ahead, and worked on by G threads with E elements each. The mean is known before the squared
+// deviations are summed. Blocks stay and walk rows, with gamma and beta in shared memory.
 //
 // Rows are read in 16-byte chunks whatever their width: a row that starts `shift` elements into a
 // 16-byte chunk is worked on as the chunks that cover it, the first and last element by element.
@@ -17,24 +16,12 @@
 // block b takes rows that are b modulo P and one shifted copy of gamma and beta serves it. Tensors
 // whose rows start differently from each other are read element by element (V = 1).
 #pragma once
-#include <string.h>
-
-#include <type_traits>
-
 #include "common.cuh"
 #include "elem.cuh"
 
 namespace jc {
 
 constexpr int NORM_MAX_D = 16384;
-
-// Threads of a forward block whose rows take G threads each.
-template <int G>
-constexpr int NORM_BLOCK = G > 128 ? G : 128;
-// Forward blocks an SM should hold: what the registers of a row (f32, and the next row's raw elements)
-// allow; left to itself the compiler takes more registers than it needs.
-template <int V, int G, int E>
-constexpr int NORM_RESIDENT = G >= 256 ? 1 : E == 8 ? 10 : E == 16 ? 8 : E == 24 ? (V == 1 ? 5 : 6) : V == 1 ? 4 : 5;
 
 // Sums over the G threads of a row's group, in a fixed order: K values at once. `part`: K floats a warp
 // in shared memory; G > 32: every thread of the block calls it.
@@ -66,7 +53,6 @@ __device__ __forceinline__ void norm_sum(float (&v)[K], float *part) {
 template <class T, int V, int G, int E>
 struct NormRow {
     static constexpr int N = E / V;
-    using Raw = std::conditional_t<V == 1, T, uint4>;
     uint32_t t, shift, d, edges;
     __device__ __forceinline__ NormRow(uint32_t t_, uint32_t shift_, uint32_t d_) : t(t_), shift(shift_), d(d_), edges(0) {
 #pragma unroll
@@ -89,28 +75,6 @@ struct NormRow {
     __device__ __forceinline__ bool ends(uint64_t r, uint32_t rows) const {
         return V > 1 && (r * d < V || (rows - 1 - r) * d < V);
     }
-    // Requests the row. A chunk that it shares with a neighbouring row is read whole and masked later,
-    // or, where it may reach past the tensor (`ends`), element by element.
-    __device__ __forceinline__ void load(const T *row, bool ends, Raw *q) const {
-#pragma unroll
-        for (int c = 0; c < N; c++) {
-            if constexpr (V == 1) {
-                q[c] = place(c) < d ? row[place(c)] : T(0.0f);
-            } else {
-                if (!edge(c) || (ends ? whole(c) : some(c))) {
-                    q[c] = *reinterpret_cast<const uint4 *>(row + first(c));
-                } else {
-                    q[c] = make_uint4(0, 0, 0, 0);
-                    if (some(c)) {
-                        T e[V];
-#pragma unroll
-                        for (int i = 0; i < V; i++) e[i] = has(c, i) ? row[first(c) + i] : T(0.0f);
-                        memcpy(&q[c], e, 16);
-                    }
-                }
-            }
-        }
-    }
     // Chunk c of a row in global memory as f32, 0 outside the row.
     __device__ __forceinline__ void chunk(const T *row, int c, bool ends, float *v) const {
         if (!edge(c) || (ends ? whole(c) : some(c))) {
@@ -119,15 +83,6 @@ struct NormRow {
         } else {
 #pragma unroll
             for (int i = 0; i < V; i++) v[i] = has(c, i) ? static_cast<float>(row[first(c) + i]) : 0.0f;
-        }
-    }
-    // Chunk c as f32, 0 outside the row.
-    __device__ __forceinline__ void unpack(const Raw &q, int c, float *v) const {
-        if constexpr (V == 1) {
-            v[0] = static_cast<float>(q);
-        } else {
-            Elem<T, V>::load(reinterpret_cast<const T *>(&q), v);
-            mask(c, v);
         }
     }
     // 0 outside the row.
@@ -181,6 +136,15 @@ __device__ __forceinline__ void norm_param(const float *s, uint32_t place, float
     }
 }
 
+// `bytes` (a multiple of 16, both addresses on 16-byte boundaries) of global into shared memory,
+// completing on `bar`.
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
 struct NormParams {
     const void *x;
     size_t ldx;
@@ -190,16 +154,32 @@ struct NormParams {
     void *y;
     size_t ldy;
     float *stats;
+    unsigned int *err;
+};
+
+// How a block of the forward kernel is made up: rows of x come into shared memory by bulk copies, STAGES
+// rows ahead, each group its own. STAGES 0 (V = 1): read where they are used.
+template <class T, int V, int G, int E>
+struct NormShape {
+    static constexpr int ROW = G * E * (int)sizeof(T);  // bytes
+    static constexpr int STAGES = V == 1 ? 0 : ROW > 32768 ? 1 : 2;
+    static constexpr int THREADS = G > 256 ? G : 256, GROUPS = THREADS / G;
+    static constexpr int SMEM = 2 * G * E * 4 + GROUPS * STAGES * ROW;  // gamma, beta, the rings
+    // Blocks an SM should hold: what the registers of a row allow.
+    static constexpr int RESIDENT = G > 256 ? 1 : E == 8 ? 6 : E <= 24 ? 4 : G < 256 ? 3 : sizeof(T) == 4 ? 1 : 2;
+    static_assert(SMEM <= 227 * 1024 - 1024, "shared memory");
 };
 
 template <class T, int V, int G, int E>
-__global__ void __launch_bounds__(NORM_BLOCK<G>, NORM_RESIDENT<V, G, E>) norm_kernel(const NormParams p) {
-    constexpr int THREADS = NORM_BLOCK<G>, GROUPS = THREADS / G;
+__global__ void __launch_bounds__(NormShape<T, V, G, E>::THREADS, NormShape<T, V, G, E>::RESIDENT)
+    norm_kernel(const NormParams p) {
+    using S = NormShape<T, V, G, E>;
     using Row = NormRow<T, V, G, E>;
+    constexpr int THREADS = S::THREADS, GROUPS = S::GROUPS, STAGES = S::STAGES;
     __shared__ float part[THREADS / 32];
-    extern __shared__ float params[];  // gamma, beta: G x E each
-    pdl_wait();
-    pdl_launch_dependents();
+    __shared__ uint64_t bars[GROUPS * (STAGES ? STAGES : 1)];
+    extern __shared__ __align__(16) float smem[];
+    dev_err_bind(p.err);
     const uint32_t g = threadIdx.x / G, cls = blockIdx.x % p.period, step = gridDim.x / p.period * GROUPS;
     const T *x = static_cast<const T *>(p.x);
     const Row row(threadIdx.x % G,
@@ -207,26 +187,67 @@ __global__ void __launch_bounds__(NORM_BLOCK<G>, NORM_RESIDENT<V, G, E>) norm_ke
     // Row i of this group is row cls + i period; a group that is out of rows keeps its block's company.
     uint32_t i = blockIdx.x / p.period * GROUPS + g;
     auto at = [&](uint32_t k) { return (uint64_t)cls + (uint64_t)k * p.period; };
-    auto fetch = [&](uint64_t r, typename Row::Raw *q) {
-        if (r < p.rows) row.load(x + r * p.ldx, row.ends(r, p.rows), q);
+    float *gs = smem, *bs = smem + G * E;
+    T *ring = reinterpret_cast<T *>(smem + 2 * G * E) + g * (STAGES * G * E);
+    uint64_t *bar = bars + g * STAGES;
+    if (STAGES && row.t == 0) {
+        for (int k = 0; k < STAGES; k++) mbar_init(&bar[k], 1);
+        fence_barrier_init();
+    }
+    pdl_wait();
+    pdl_launch_dependents();
+    // One thread of a group requests a row's chunks. Rows whose outer chunks may reach past the tensor
+    // are copied by the group itself, element by element, when their turn comes.
+    auto whole_chunks = [&](uint64_t r) { return p.period == 1 || !row.ends(r, p.rows); };
+    auto request = [&](uint64_t r, uint32_t st) {
+        if (STAGES == 0 || row.t != 0 || r >= p.rows || !whole_chunks(r)) return;
+        const uint32_t bytes = (row.shift + p.d + V - 1) / V * 16;
+        mbar_arrive_expect_tx(&bar[st], bytes);
+        bulk_load(ring + st * (G * E), x + r * p.ldx - row.shift, bytes, &bar[st]);
     };
-    typename Row::Raw raw[Row::N];
-    fetch(at(i), raw);
-    float *gs = params, *bs = params + G * E;
+#pragma unroll
+    for (int k = 0; k < STAGES; k++) request(at(i + k * step), k);
     norm_stage_param<V, G, E>(gs, p.gamma, row.shift, p.d, THREADS);
     norm_stage_param<V, G, E>(bs, p.beta, row.shift, p.d, THREADS);
     __syncthreads();
     const float inv_d = 1.0f / (float)p.d;
+    uint32_t st = 0, phases = 0;  // the stage, and a bit a stage: its barrier's parity
     for (uint32_t k = blockIdx.x / p.period * GROUPS; at(k) < p.rows; k += step, i += step) {
         const uint64_t r = at(i);
         const bool mine = r < p.rows;
         if (G == 32 && !mine) break;  // a warp by itself
         float v[E];
+        if constexpr (STAGES > 0) {
+            T *stage = ring + st * (G * E);
+            if (mine && whole_chunks(r)) {
+                mbar_wait(&bar[st], phases >> st & 1, JC_DEV_TIMEOUT_FULL);
+                phases ^= 1u << st;
+            } else if (mine) {
+                for (uint32_t j = row.t; j < p.d; j += G) stage[row.shift + j] = x[r * p.ldx + j];
+            }
+            if (G == 32)
+                __syncwarp();
+            else if (p.period > 1)
+                __syncthreads();
 #pragma unroll
-        for (int c = 0; c < Row::N; c++) row.unpack(raw[c], c, v + c * V);
-        fetch(at(i + step), raw);
+            for (int c = 0; c < Row::N; c++) {
+                Elem<T, V>::load(stage + row.place(c), v + c * V);
+                row.mask(c, v + c * V);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < E; c++)
+                v[c] = mine && row.place(c) < p.d ? static_cast<float>(x[r * p.ldx + row.place(c)]) : 0.0f;
+        }
         float s[1] = {norm_add_up<E>(v)};
         norm_sum<G>(s, part);
+        if constexpr (STAGES > 0) {
+            // The group has read the stage (every lane has added into the sum): the row STAGES further on
+            // may take it.
+            if (G == 32) __syncwarp();
+            request(at(i + STAGES * step), st);
+            st = st + 1 == STAGES ? 0 : st + 1;
+        }
         const float mean = s[0] * inv_d, off[2] = {-mean, -mean};
         float q[2] = {0.0f, 0.0f};
         if constexpr (V == 1) {
@@ -302,13 +323,6 @@ struct NormBwdShape {
     static constexpr int SMEM = G * E * 4 + (RING > SUMS ? RING : SUMS);  // gamma, then the ring, later the sums
     static_assert(SMEM <= 227 * 1024 - 1024, "shared memory");
 };
-
-__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                     smem_u32(dst)),
-                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
-                 : "memory");
-}
 
 // A block's groups keep their sums for dgamma and dbeta in registers over all their rows and add them
 // up in shared memory once, group after group; one row of sums a block goes to ws, or, from a block

@@ -109,23 +109,26 @@ static uint32_t norm_blocks(uint32_t rows, uint32_t groups, uint32_t period, uin
 
 bool launch_norm(const NormArgs &a, cudaStream_t s) {
     if (a.rows == 0) return true;
+    unsigned int *err = module_error_word();
+    if (!err) return false;
     return with_type(a.type, [&](auto t) {
         using T = decltype(t);
         const NormLayout l = norm_layout(a.d, sizeof(T), {{a.x, a.ldx}, {a.y, a.ldy}});
         return with_group(l.span, [&](auto g, auto e) {
-            constexpr int G = g, E = e, THREADS = NORM_BLOCK<G>;
-            const NormParams p{a.x, a.ldx, a.gamma, a.beta, a.eps, a.rows, a.d, l.period, a.y, a.ldy, a.stats};
-            const int smem = 2 * G * E * (int)sizeof(float);
-            auto go = [&](auto kern, std::atomic<uint64_t> &set, std::atomic<int> &resident) {
-                if (!ensure_smem(kern, smem, set)) return false;
+            constexpr int G = g, E = e;
+            const NormParams p{a.x, a.ldx, a.gamma, a.beta, a.eps, a.rows, a.d, l.period, a.y, a.ldy, a.stats, err};
+            auto go = [&](auto kern, std::atomic<uint64_t> &set, std::atomic<int> &resident, auto shape) {
+                using S = decltype(shape);
                 int per_sm = 0;
-                if (!blocks_per_sm(kern, THREADS, smem, resident, &per_sm)) return false;
-                const dim3 grid(norm_blocks(a.rows, THREADS / G, l.period, (uint32_t)(sm_count() * per_sm)));
-                return launch_ex(kern, grid, dim3(THREADS), smem, s, true, "layer_norm", p);
+                if (!ensure_smem(kern, S::SMEM, set) || !blocks_per_sm(kern, S::THREADS, S::SMEM, resident, &per_sm))
+                    return false;
+                const dim3 grid(norm_blocks(a.rows, S::GROUPS, l.period, (uint32_t)(sm_count() * per_sm)));
+                return launch_ex(kern, grid, dim3(S::THREADS), S::SMEM, s, true, "layer_norm", p);
             };
             static std::atomic<uint64_t> set_v{0}, set_1{0};
             static std::atomic<int> res_v{0}, res_1{0};
-            return l.chunks ? go(norm_kernel<T, VEC<T>, G, E>, set_v, res_v) : go(norm_kernel<T, 1, G, E>, set_1, res_1);
+            return l.chunks ? go(norm_kernel<T, VEC<T>, G, E>, set_v, res_v, NormShape<T, VEC<T>, G, E>())
+                            : go(norm_kernel<T, 1, G, E>, set_1, res_1, NormShape<T, 1, G, E>());
         });
     });
 }
@@ -556,7 +559,7 @@ bool launch_linear_bwd(const LinearBwdArgs &a, cudaStream_t s) {
 // ---------------------------------------------------------------------------------------------
 // loss and optimizer
 
-// Requests of up to this many logits on average go a thread each.
+// Requests of up to this many logits on average go a lane each (a warp's 32 must fit LOSS_SMEM).
 constexpr uint32_t LOSS_SHORT = 24;
 
 bool launch_choice_loss(const LossArgs &a, cudaStream_t s) {
@@ -566,8 +569,8 @@ bool launch_choice_loss(const LossArgs &a, cudaStream_t s) {
     const LossParams p{a.logits, a.n_logits, a.offsets, a.gold, a.weight, a.requests, a.loss, a.dlogits, err};
     const uint32_t mean = a.n_logits / a.requests;
     if (mean <= LOSS_SHORT)
-        return launch_ex(loss_short_kernel, dim3((a.requests + LOSS_BLOCK - 1) / LOSS_BLOCK), dim3(LOSS_BLOCK), 0, s, true,
-                         "choice_loss", p);
+        return launch_ex(loss_short_kernel, dim3((a.requests + 32 * LOSS_WARPS - 1) / (32 * LOSS_WARPS)),
+                         dim3(32 * LOSS_WARPS), 0, s, true, "choice_loss", p);
     if (mean <= 512) return launch_ex(loss_group_kernel<32>, dim3((a.requests + 3) / 4), dim3(128), 0, s, true, "choice_loss", p);
     return launch_ex(loss_group_kernel<256>, dim3(a.requests), dim3(256), 0, s, true, "choice_loss", p);
 }
