@@ -117,87 +117,96 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) loss_group_kernel(const Los
     if (r < p.requests) loss_group<G>(p, r, threadIdx.x % G, part);
 }
 
-// Requests of a few markers: a warp takes 32 consecutive requests, whose logits lie together whatever
-// their lengths, and moves them through its own part of shared memory in whole lines; a lane works on a
-// request there. A warp whose logits do not fit (a long request among short ones) or lie out of order
-// takes its requests one by one instead. Warps do not wait for each other: with a block's 128 requests
-// behind barriers, a million requests took 31 us.
+// Requests of a few markers: a lane takes a request, a warp 32 consecutive ones. A lane reads its logits
+// where they are (neighbours share the lines, so the first reads bring the others into L1) and keeps up
+// to LOSS_REGS of them in registers; the gradients go out through the warp's part of shared memory in
+// whole lines. Warps stay and walk the requests, the next ones' spans requested ahead. A warp whose
+// gradients do not fit (a long request among short ones), or whose requests lie out of order, takes them
+// one by one instead.
 constexpr int LOSS_WARPS = 4, LOSS_SMEM = 768, LOSS_REGS = 16;
 
-__global__ void __launch_bounds__(32 * LOSS_WARPS, 12) loss_short_kernel(const LossParams p) {
+__global__ void __launch_bounds__(32 * LOSS_WARPS, 8) loss_short_kernel(const LossParams p) {
     __shared__ float smem[LOSS_WARPS][LOSS_SMEM];
     dev_err_bind(p.err);
     pdl_wait();
     pdl_launch_dependents();
-    const uint32_t t = threadIdx.x & 31, r0 = (blockIdx.x * LOSS_WARPS + threadIdx.x / 32) * 32;
-    if (r0 >= p.requests) return;
-    const uint32_t n = min(32u, p.requests - r0);
+    const uint32_t t = threadIdx.x & 31, step = gridDim.x * LOSS_WARPS * 32;
     float *s = smem[threadIdx.x / 32];
-    uint32_t a = 0, b = 0;
-    int32_t gold = -1;
-    float w = 0.0f;
-    const bool ok = t >= n || loss_request(p, r0 + t, a, b, gold, w);
-    const uint32_t lo = __shfl_sync(0xffffffffu, a, 0), hi = __shfl_sync(0xffffffffu, b, n - 1);
-    const bool inside = t >= n || (a >= lo && b <= hi);
-    if (!__all_sync(0xffffffffu, ok && inside && hi >= lo && hi - lo <= LOSS_SMEM)) {
-        for (uint32_t k = 0; k < n; k++) loss_group<32>(p, r0 + k, t, nullptr);
-        return;
-    }
-#pragma unroll 8
-    for (uint32_t i = t; i < hi - lo; i += 32) s[i] = p.logits[lo + i];
-    __syncwarp();
-    const uint32_t len = b - a, longest = __reduce_max_sync(0xffffffffu, len);
-    float *l = s + (t < n ? a - lo : 0);
-    float top = -INFINITY, sum = 0.0f, v[LOSS_REGS];
-    const bool regs = longest <= LOSS_REGS;
-    if (regs) {
-        // Read once into registers, written back once: these accesses hit random banks.
-#pragma unroll
-        for (int i = 0; i < LOSS_REGS; i += 4)
-            if (i < longest)
-#pragma unroll
-                for (int j = i; j < i + 4; j++) {
-                    v[j] = j < len ? l[j] : -INFINITY;
-                    top = fmaxf(top, v[j]);
-                }
-    } else {
-        for (uint32_t i = 0; i < len; i++) top = fmaxf(top, l[i]);
-    }
-    const float right = gold >= 0 ? l[gold] : 0.0f;
-    if (top == -INFINITY) top = 0.0f;
-    if (regs) {
-#pragma unroll
-        for (int i = 0; i < LOSS_REGS; i += 4)
-            if (i < longest)
-#pragma unroll
-                for (int j = i; j < i + 4; j++) {
-                    v[j] = __expf(v[j] - top);
-                    sum += v[j];
-                }
-    } else {
-        for (uint32_t i = 0; i < len; i++) {
-            l[i] = __expf(l[i] - top);
-            sum += l[i];
+    // A request's span, right marker and weight; none past the last request.
+    struct Request {
+        uint32_t a, b;
+        int32_t gold;
+        float w;
+        bool ok;
+    };
+    auto look_up = [&](uint64_t r) {
+        Request q{0, 0, -1, 0.0f, true};
+        if (r < p.requests) q.ok = loss_request(p, (uint32_t)r, q.a, q.b, q.gold, q.w);
+        return q;
+    };
+    uint64_t r0 = ((uint64_t)blockIdx.x * LOSS_WARPS + threadIdx.x / 32) * 32;
+    Request next = look_up(r0 + t);
+    for (; r0 < p.requests; r0 += step) {
+        const Request q = next;
+        next = look_up(r0 + step + t);
+        const uint32_t n = (uint32_t)min((uint64_t)32, p.requests - r0), len = q.b - q.a;
+        const uint32_t lo = __shfl_sync(0xffffffffu, q.a, 0), hi = __shfl_sync(0xffffffffu, q.b, n - 1);
+        const bool fits = q.ok && (t >= n || (q.a >= lo && q.b <= hi)) && hi >= lo && hi - lo <= LOSS_SMEM;
+        if (!__all_sync(0xffffffffu, fits)) {
+            for (uint32_t k = 0; k < n; k++) loss_group<32>(p, (uint32_t)(r0 + k), t, nullptr);
+            continue;
         }
-    }
-    const bool counts = gold >= 0 && w != 0.0f && sum != 0.0f;
-    if (t < n) p.loss[r0 + t] = counts ? w * (top + logf(sum) - right) : 0.0f;
-    if (!p.dlogits) return;
-    const float f = counts ? w / sum : 0.0f;
-    if (regs) {
+        const float *l = p.logits + q.a;
+        float *out = s + (t < n ? q.a - lo : 0);
+        const uint32_t longest = __reduce_max_sync(0xffffffffu, len);
+        const bool regs = longest <= LOSS_REGS;
+        float top = -INFINITY, sum = 0.0f, v[LOSS_REGS];
+        const float right = q.gold >= 0 ? l[q.gold] : 0.0f;
+        if (regs) {
 #pragma unroll
-        for (int i = 0; i < LOSS_REGS; i += 4)
-            if (i < longest)
+            for (int i = 0; i < LOSS_REGS; i += 4)
+                if (i < longest)
 #pragma unroll
-                for (int j = i; j < i + 4; j++)
-                    if (j < len) l[j] = counts ? v[j] * f : 0.0f;
-    } else {
-        for (uint32_t i = 0; i < len; i++) l[i] = counts ? l[i] * f : 0.0f;
-    }
-    if (counts) l[gold] -= w;
-    __syncwarp();
+                    for (int j = i; j < i + 4; j++) v[j] = j < len ? l[j] : -INFINITY;
+#pragma unroll
+            for (int i = 0; i < LOSS_REGS; i += 4)
+                if (i < longest) top = fmaxf(top, fmaxf(fmaxf(v[i], v[i + 1]), fmaxf(v[i + 2], v[i + 3])));
+        } else {
+            for (uint32_t i = 0; i < len; i++) top = fmaxf(top, l[i]);
+        }
+        if (top == -INFINITY) top = 0.0f;
+        if (regs) {
+#pragma unroll
+            for (int i = 0; i < LOSS_REGS; i += 4)
+                if (i < longest)
+#pragma unroll
+                    for (int j = i; j < i + 4; j++) {
+                        v[j] = __expf(v[j] - top);
+                        sum += v[j];
+                    }
+        } else {
+            for (uint32_t i = 0; i < len; i++) sum += __expf(l[i] - top);
+        }
+        const bool counts = q.gold >= 0 && q.w != 0.0f && sum != 0.0f;
+        if (t < n) p.loss[r0 + t] = counts ? q.w * (top + logf(sum) - right) : 0.0f;
+        if (!p.dlogits) continue;
+        const float f = q.w / sum;
+        if (regs) {
+#pragma unroll
+            for (int i = 0; i < LOSS_REGS; i += 4)
+                if (i < longest)
+#pragma unroll
+                    for (int j = i; j < i + 4; j++)
+                        if (j < len) out[j] = counts ? v[j] * f : 0.0f;
+        } else {
+            for (uint32_t i = 0; i < len; i++) out[i] = counts ? __expf(l[i] - top) * f : 0.0f;
+        }
+        if (counts) out[q.gold] -= q.w;
+        __syncwarp();
 #pragma unroll 8
-    for (uint32_t i = t; i < hi - lo; i += 32) p.dlogits[lo + i] = s[i];
+        for (uint32_t i = t; i < hi - lo; i += 32) p.dlogits[lo + i] = s[i];
+        __syncwarp();
+    }
 }
 
 }  // namespace jc

@@ -568,9 +568,14 @@ bool launch_choice_loss(const LossArgs &a, cudaStream_t s) {
     if (!err) return false;
     const LossParams p{a.logits, a.n_logits, a.offsets, a.gold, a.weight, a.requests, a.loss, a.dlogits, err};
     const uint32_t mean = a.n_logits / a.requests;
-    if (mean <= LOSS_SHORT)
-        return launch_ex(loss_short_kernel, dim3((a.requests + 32 * LOSS_WARPS - 1) / (32 * LOSS_WARPS)),
-                         dim3(32 * LOSS_WARPS), 0, s, true, "choice_loss", p);
+    if (mean <= LOSS_SHORT) {
+        static std::atomic<int> resident{0};
+        int per_sm = 0;
+        if (!blocks_per_sm(loss_short_kernel, 32 * LOSS_WARPS, 0, resident, &per_sm)) return false;
+        const uint32_t blocks = (a.requests + 32 * LOSS_WARPS - 1) / (32 * LOSS_WARPS);
+        return launch_ex(loss_short_kernel, dim3(std::min(blocks, (uint32_t)(sm_count() * per_sm))), dim3(32 * LOSS_WARPS),
+                         0, s, true, "choice_loss", p);
+    }
     if (mean <= 512) return launch_ex(loss_group_kernel<32>, dim3((a.requests + 3) / 4), dim3(128), 0, s, true, "choice_loss", p);
     return launch_ex(loss_group_kernel<256>, dim3(a.requests), dim3(256), 0, s, true, "choice_loss", p);
 }
