@@ -422,20 +422,25 @@ size_t jc_layer_norm_ws_floats(uint32_t rows, uint32_t d);
 /* z = x w^T + bias, y = act(z) + res: x [m][k], w [n][k], y, z, res [m][n] of `type` (JC_F16 or
  * JC_BF16), bias [n] f32; bias, res and z may be NULL. act: 0, JC_EPI_RELU or JC_EPI_GELU. z, when
  * given, keeps the values before the activation, which the backward pass reads. Unlike jc_gemm, any
- * m, n and k, both 16-bit types, strided rows. y may be res. */
+ * m, n and k, both 16-bit types, strided rows. y may be res. ws: jc_linear_ws_bytes(x, ldx, w, ldw, m,
+ * n, k) bytes of scratch, 256-byte aligned: 0 (ws may be NULL) where the rows of x and w start on
+ * 16-byte boundaries; others are copied there first. */
 int jc_linear(uint32_t type, uint32_t act, const void *x, size_t ldx, const void *w, size_t ldw,
               const float *bias, const void *res, size_t ldres, void *y, size_t ldy, void *z,
-              size_t ldz, uint32_t m, uint32_t n, uint32_t k, void *stream);
+              size_t ldz, uint32_t m, uint32_t n, uint32_t k, void *ws, void *stream);
+size_t jc_linear_ws_bytes(const void *x, size_t ldx, const void *w, size_t ldw, uint32_t m,
+                          uint32_t n, uint32_t k);
 /* The gradients of jc_linear: dz = dy act'(z), dx = dz w [m][k], dw = dz^T x [n][k], dbias = sum over
  * rows of dz ([n] f32); each of dx, dw and dbias may be NULL. (res's gradient is dy itself.) z is
  * read when act is not 0. dz is rounded to `type` before the products, as every tensor-core
  * operand is; dbias sums it unrounded. With f16 a gradient below 6e-8 becomes 0: scale the loss.
- * ws: jc_linear_ws_bytes(m, n, k) bytes of scratch, 256-byte aligned. */
+ * ws: jc_linear_backward_ws_bytes(x, ldx, w, ldw, m, n, k) bytes of scratch, 256-byte aligned. */
 int jc_linear_backward(uint32_t type, uint32_t act, const void *dy, size_t lddy, const void *x,
                        size_t ldx, const void *w, size_t ldw, const void *z, size_t ldz, uint32_t m,
                        uint32_t n, uint32_t k, void *dx, size_t lddx, void *dw, size_t lddw,
                        float *dbias, void *ws, void *stream);
-size_t jc_linear_ws_bytes(uint32_t m, uint32_t n, uint32_t k);
+size_t jc_linear_backward_ws_bytes(const void *x, size_t ldx, const void *w, size_t ldw, uint32_t m,
+                                   uint32_t n, uint32_t k);
 
 /* The loss of requests that each pick one of their markers: request r's logits are
  * [offsets[r], offsets[r + 1]) of `logits` (n_logits in all; offsets int32 [requests + 1]) and its

@@ -145,10 +145,11 @@ def lib():
         "jc_layer_norm_backward": ([u32, P, sz, P, sz, P, P, P, sz, u32, u32, P, sz, P, P, P, P],
                                    i32),
         "jc_layer_norm_ws_floats": ([u32, u32], sz),
-        "jc_linear": ([u32, u32, P, sz, P, sz, P, P, sz, P, sz, P, sz, u32, u32, u32, P], i32),
+        "jc_linear": ([u32, u32, P, sz, P, sz, P, P, sz, P, sz, P, sz, u32, u32, u32, P, P], i32),
         "jc_linear_backward": ([u32, u32, P, sz, P, sz, P, sz, P, sz, u32, u32, u32, P, sz, P, sz, P,
                                 P, P], i32),
-        "jc_linear_ws_bytes": ([u32, u32, u32], sz),
+        "jc_linear_ws_bytes": ([P, sz, P, sz, u32, u32, u32], sz),
+        "jc_linear_backward_ws_bytes": ([P, sz, P, sz, u32, u32, u32], sz),
         "jc_choice_loss": ([P, u32, P, P, P, u32, P, P, P], i32),
         "jc_adamw_create": ([P, sz, u32], P),
         "jc_adamw_step": ([P, u64, f32, ctypes.c_double, ctypes.c_double, f32, P, P], i32),

@@ -146,7 +146,7 @@ int jc_layer_norm_backward(uint32_t type, const void *dy, size_t lddy, const voi
 
 int jc_linear(uint32_t type, uint32_t act, const void *x, size_t ldx, const void *w, size_t ldw,
               const float *bias, const void *res, size_t ldres, void *y, size_t ldy, void *z, size_t ldz,
-              uint32_t m, uint32_t n, uint32_t k, void *stream) {
+              uint32_t m, uint32_t n, uint32_t k, void *ws, void *stream) {
     return guarded(nullptr, 0, [&]() -> int {
         const char *op = "linear";
         const bool any = m > 0;
@@ -154,9 +154,11 @@ int jc_linear(uint32_t type, uint32_t act, const void *x, size_t ldx, const void
         if (n == 0 || k == 0) return fail("linear: n and k must not be 0");
         if (!check_matrix(op, "x", x, ldx, k, 2, any) || !check_matrix(op, "w", w, ldw, k, 2, true) ||
             !check_vector(op, "bias", bias, 4, false) || !check_matrix(op, "res", res, ldres, n, 2, false) ||
-            !check_matrix(op, "y", y, ldy, n, 2, any) || !check_matrix(op, "z", z, ldz, n, 2, false))
+            !check_matrix(op, "y", y, ldy, n, 2, any) || !check_matrix(op, "z", z, ldz, n, 2, false) ||
+            !check_vector(op, "ws", ws, 256, any && jc::linear_ws_bytes(x, ldx, w, ldw, m, n, k) > 0))
             return -1;
         jc::LinearArgs a;
+        a.ws = ws;
         a.type = type;
         a.act = act;
         a.x = x;
@@ -177,8 +179,13 @@ int jc_linear(uint32_t type, uint32_t act, const void *x, size_t ldx, const void
     });
 }
 
-size_t jc_linear_ws_bytes(uint32_t m, uint32_t n, uint32_t k) {
-    return n && k ? jc::linear_bwd_ws_bytes(m, n, k) : 0;
+size_t jc_linear_ws_bytes(const void *x, size_t ldx, const void *w, size_t ldw, uint32_t m, uint32_t n, uint32_t k) {
+    return n && k ? jc::linear_ws_bytes(x, ldx, w, ldw, m, n, k) : 0;
+}
+
+size_t jc_linear_backward_ws_bytes(const void *x, size_t ldx, const void *w, size_t ldw, uint32_t m, uint32_t n,
+                                   uint32_t k) {
+    return n && k ? jc::linear_bwd_ws_bytes(x, ldx, w, ldw, m, n, k) : 0;
 }
 
 int jc_linear_backward(uint32_t type, uint32_t act, const void *dy, size_t lddy, const void *x, size_t ldx,
@@ -195,7 +202,7 @@ int jc_linear_backward(uint32_t type, uint32_t act, const void *dy, size_t lddy,
             !check_matrix(op, "z", z, ldz, n, 2, any && act) ||
             !check_matrix(op, "dx", dx, lddx, k, 2, false) || !check_matrix(op, "dw", dw, lddw, k, 2, false) ||
             !check_vector(op, "dbias", dbias, 4, false) ||
-            !check_vector(op, "ws", ws, 256, any && jc::linear_bwd_ws_bytes(m, n, k) > 0))
+            !check_vector(op, "ws", ws, 256, any && jc::linear_bwd_ws_bytes(dw ? x : nullptr, ldx, dx ? w : nullptr, ldw, m, n, k) > 0))
             return -1;
         jc::LinearBwdArgs a;
         a.type = type;

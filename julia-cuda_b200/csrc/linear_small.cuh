@@ -47,13 +47,24 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Eight elements, of which `left` exist (VEC: all, on a 16-byte boundary).
+template <bool VEC, class T>
+__device__ __forceinline__ uint4 eight(const T *p, uint32_t left) {
+    if constexpr (VEC) return *reinterpret_cast<const uint4 *>(p);
+    const uint16_t *s = reinterpret_cast<const uint16_t *>(p);
+    uint32_t v[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = j < (int)min(left, 8u) ? s[j] : 0;
+    return make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+}
+
 constexpr int LR_WARPS = 8, LR_AHEAD = 4;
 
 // A block computes 16 rows x 8 columns; its warps take every eighth group of 32 contracted elements and
 // their sums meet in shared memory, in order. The contraction's order is free, so a lane loads the 16
 // bytes (8 elements) that make its fragments of two MMAs: lane 4 g + q holds elements 8 q .. 8 q + 7 of
 // column g of w, and of rows g and g + 8 of x, and takes them in pairs as the MMA's k places 2 q, 2 q + 8.
-template <class T, uint32_t ACT>
+template <class T, uint32_t ACT, bool VEC>
 __global__ void __launch_bounds__(32 * LR_WARPS) linear_rows_kernel(const LinearRowsParams p) {
     __shared__ float sums[LR_WARPS][128];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
@@ -70,10 +81,10 @@ __global__ void __launch_bounds__(32 * LR_WARPS) linear_rows_kernel(const Linear
 #pragma unroll
         for (int i = 0; i < LR_AHEAD; i++) {
             const uint32_t k = k0 + i * LR_WARPS * 32 + 8 * q;
-            const bool in = k < p.k;  // k is a multiple of 8
-            b[i] = in && col ? __ldg(reinterpret_cast<const uint4 *>(w + k)) : none;
-            a0[i] = in && ra ? *reinterpret_cast<const uint4 *>(xa + k) : none;
-            a1[i] = in && rb ? *reinterpret_cast<const uint4 *>(xb + k) : none;
+            const bool in = k < p.k;
+            b[i] = in && col ? eight<VEC>(w + k, p.k - k) : none;
+            a0[i] = in && ra ? eight<VEC>(xa + k, p.k - k) : none;
+            a1[i] = in && rb ? eight<VEC>(xb + k, p.k - k) : none;
         }
 #pragma unroll
         for (int i = 0; i < LR_AHEAD; i++) {

@@ -9,16 +9,12 @@
 // as it lies, in blocks of 64 (contiguous) x 64 (contracted), and its shared-memory descriptor says
 // so ("MN-major").
 //
-// Two kernels share the tiles, the epilogue and the roles:
-//   linear_tc_kernel   TMA loads; the operands' rows on 16-byte boundaries. One CTA per SM walks the
-//                      tiles; the epilogue of one runs under the main loop of the next (two
-//                      accumulators). CTAS 2: pairs of CTAs on 256 x BN tiles (cta_group::2), each
-//                      with 128 rows of a and half of the rows of b, for a third fewer operand bytes
-//                      per SM than a 128 x 256 tile: alone, such a tile asks an SM for 48 KB per 512
-//                      tensor cycles, more than the 64 bytes a cycle it can take in.
-//   linear_any_kernel  any strides and alignment: eight warps load elements and write them into the
-//                      same swizzled tiles. One tile a CTA.
-// Both: one warp issues the MMAs, eight run the epilogue.
+// Operands come by TMA, whose rows start on 16-byte boundaries; others are laid out so first
+// (linear_pad_kernel). One CTA per SM walks the tiles: a warp loads, one issues the MMAs, eight run the
+// epilogue of one tile under the main loop of the next (two accumulators). CTAS 2: pairs of CTAs on 256 x
+// BN tiles (cta_group::2), each with 128 rows of a and half of the rows of b, for a third fewer operand
+// bytes per SM than a 128 x 256 tile: alone, such a tile asks an SM for 48 KB per 512 tensor cycles, more
+// than the 64 bytes a cycle it can take in.
 #pragma once
 #include <type_traits>
 
@@ -57,7 +53,6 @@ constexpr uint32_t LT_STEP = MN ? (16 * 128) >> 4 : 32 >> 4;
 
 struct LinearTcParams {
     uint32_t m, n, k;
-    LinearOperand a, b;  // linear_any_kernel; linear_tc_kernel's come as tensor maps
     const float *bias;
     const void *res;
     size_t ldres;
@@ -78,12 +73,8 @@ struct LinearTcKernelParams {
 
 template <int BN>
 struct LtShape {
-    static constexpr int HALVES = BN >= 64 ? 2 : 1;        // column halves the eight warps split
-    static constexpr int CW = BN / HALVES < 64 ? BN / HALVES : 64;  // columns of an epilogue chunk
-    static constexpr int CHUNKS = BN / HALVES / CW;
-    static constexpr int B_ROWS = BN < 64 ? 64 : BN;       // an MN-major block is 64 wide
-    static constexpr int A_BYTES = LT_BM * 128, B_BYTES = B_ROWS * 128, STAGE = A_BYTES + B_BYTES;
-    static constexpr int TMEM = BN < 32 ? 32 : BN;         // columns of one accumulator
+    static constexpr int CW = BN / 2 < 64 ? BN / 2 : 64;  // columns of an epilogue chunk
+    static constexpr int CHUNKS = BN / 2 / CW;            // chunks of a warp: half of the columns
 };
 
 // ---------------------------------------------------------------------------------------------
@@ -213,12 +204,8 @@ __device__ __forceinline__ void lt_add_row(const uint8_t *buf, float *v) {
 // CW columns of this lane's accumulator row.
 template <int CW>
 __device__ __forceinline__ void lt_acc(uint32_t taddr, float *v) {
-    if constexpr (CW == 16) {
-        tmem_ld<16>(taddr, v);
-    } else {
 #pragma unroll
-        for (int i = 0; i < CW; i += 32) tmem_ld32(taddr + i, *reinterpret_cast<float(*)[32]>(v + i));
-    }
+    for (int i = 0; i < CW; i += 32) tmem_ld32(taddr + i, *reinterpret_cast<float(*)[32]>(v + i));
     tc_wait_ld();
 }
 
@@ -231,7 +218,6 @@ __device__ __forceinline__ void lt_epilogue(const LinearTcParams &p, uint32_t ac
                                             LtBias<LtShape<BN>::CW> &bias, LtRes<LtShape<BN>::CW> &res) {
     using S = LtShape<BN>;
     constexpr int CW = S::CW;
-    if (warp / 4 >= (uint32_t)S::HALVES) return;
     const uint32_t r0 = m0 + 32 * (warp & 3);
     const uint32_t lane_acc = acc + ((32 * (warp & 3)) << 16);
 #pragma unroll 1
@@ -242,7 +228,7 @@ __device__ __forceinline__ void lt_epilogue(const LinearTcParams &p, uint32_t ac
         if (p.ws) {
             // Partial sums, f32, 32 columns (128 bytes) at a time.
             uint8_t *ws = reinterpret_cast<uint8_t *>(p.ws + (size_t)split * p.m * p.n);
-            constexpr int PW = CW < 32 ? CW : 32;
+            constexpr int PW = 32;
 #pragma unroll
             for (int h = 0; h < CW / PW; h++) {
                 const uint32_t r = threadIdx.x & 31;
@@ -333,7 +319,7 @@ __global__ void __launch_bounds__(LT_TC_THREADS, 1)
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = CTAS == 2 ? cluster_rank() : 0, unit = blockIdx.x / CTAS, units = gridDim.x / CTAS;
-    constexpr uint32_t COLS = 2 * S::TMEM;
+    constexpr uint32_t COLS = 2 * BN;
     if (threadIdx.x == 0) {
         // Pairs: the leader's producer arms a stage for both CTAs' bytes, and its commits release it,
         // and hand over an accumulator, in both.
@@ -403,7 +389,7 @@ __global__ void __launch_bounds__(LT_TC_THREADS, 1)
                 const uint32_t z = i / tiles, buf = done & 1, use = done >> 1;
                 if (use > 0 && !mbar_wait(&acc_empty[buf], (use & 1) ^ 1, JC_DEV_TIMEOUT_MMA)) break;
                 tc_fence_after();
-                const uint32_t acc = tmem + buf * S::TMEM;
+                const uint32_t acc = tmem + buf * BN;
                 const uint32_t k0 = (uint32_t)((uint64_t)blocks * z / p.splits);
                 const uint32_t k1 = (uint32_t)((uint64_t)blocks * (z + 1) / p.splits);
                 for (uint32_t kb = k0; kb < k1; kb++, it++) {
@@ -443,12 +429,12 @@ __global__ void __launch_bounds__(LT_TC_THREADS, 1)
             const uint32_t t = i % tiles, n0 = t % p.tiles_n * BN, m0 = (t / p.tiles_n * CTAS + rank) * LT_BM;
             // The first chunk's bias and residual are on their way while the accumulator is being summed.
             bias.load(p.bias, n0 + (warp >> 2) * (BN / 2), p.n);
-            if (VEC && p.res && warp / 4 < (uint32_t)S::HALVES)
+            if (VEC && p.res)
                 res.load(static_cast<const uint8_t *>(p.res), p.ldres, m0 + 32 * (warp & 3),
                          n0 + (warp >> 2) * (BN / 2), p.m, p.n);
             if (!mbar_wait_sleep(&acc_full[done & 1], (done >> 1) & 1, JC_DEV_TIMEOUT_MMA)) break;
             tc_fence_after();
-            lt_epilogue<T, BN, ACT, VEC>(p, tmem + (done & 1) * S::TMEM, buf, warp, m0, n0, i / tiles, bias, res);
+            lt_epilogue<T, BN, ACT, VEC>(p, tmem + (done & 1) * BN, buf, warp, m0, n0, i / tiles, bias, res);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
@@ -472,144 +458,6 @@ __global__ void __launch_bounds__(LT_TC_THREADS, 1)
             tmem_dealloc_pair(tmem, COLS);
         else
             tmem_dealloc(tmem, COLS);
-    }
-}
-
-// ---------------------------------------------------------------------------------------------
-// any strides and alignment
-
-// ROWS x 64 of an operand from (row0, k0) into a stage's tile by eight warps, zeros past (rows, k1). A
-// warp reads along the contiguous axis, two elements a lane; `pairs`: every row starts on a 4-byte
-// boundary.
-template <int ROWS, bool MN>
-__device__ __forceinline__ void lt_gather(uint8_t *dst, const LinearOperand &o, uint32_t row0, uint32_t rows,
-                                          uint32_t k0, uint32_t k1, bool pairs) {
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint16_t *g = static_cast<const uint16_t *>(o.p);
-    constexpr int LINES = MN ? 64 * ((ROWS + 63) / 64) : ROWS;  // 128-byte lines of the tile
-    constexpr int BATCH = LINES / 8 < 16 ? LINES / 8 : 16;
-#pragma unroll 1
-    for (int l0 = 0; l0 < LINES / 8; l0 += BATCH) {
-        uint32_t v[BATCH];
-#pragma unroll
-        for (int j = 0; j < BATCH; j++) {
-            const uint32_t line = warp + 8 * (l0 + j);
-            // The line's place, and how many of this lane's two elements exist.
-            const uint32_t across = MN ? row0 + line / 64 * 64 + 2 * lane : k0 + 2 * lane;
-            const uint32_t end = MN ? min(rows, row0 + ROWS) : k1;
-            const uint32_t other = MN ? k0 + line % 64 : row0 + line;
-            const bool there = other < (MN ? k1 : rows);
-            const uint16_t *s = g + (size_t)other * (MN ? o.sk : o.si) + across;
-            uint32_t lo = 0, hi = 0;
-            if (there && across + 1 < end && pairs) {
-                lo = *reinterpret_cast<const uint32_t *>(s);
-            } else if (there) {
-                if (across < end) lo = s[0];
-                if (across + 1 < end) hi = s[1];
-            }
-            v[j] = lo | hi << 16;
-        }
-#pragma unroll
-        for (int j = 0; j < BATCH; j++) {
-            const uint32_t line = warp + 8 * (l0 + j), r = line & 7;
-            *reinterpret_cast<uint32_t *>(dst + line * 128 + (((lane >> 2) ^ r) << 4) + (lane & 3) * 4) = v[j];
-        }
-    }
-}
-
-template <int BN>
-struct LtAnySmem {
-    using S = LtShape<BN>;
-    static constexpr int STAGES = 3;
-    static constexpr int BYTES = STAGES * S::STAGE + LT_EPI_WARPS * LT_STAGE_BUF + 256 + 1024;
-};
-
-constexpr int LT_ANY_THREADS = 32 * (LT_EPI_WARPS + 1);
-
-template <class T, int BN, bool A_MN, bool B_MN, uint32_t ACT>
-__global__ void __launch_bounds__(LT_ANY_THREADS, 1)
-    linear_any_kernel(const __grid_constant__ LinearTcParams p) {
-    using S = LtShape<BN>;
-    constexpr int STAGES = LtAnySmem<BN>::STAGES;
-    dev_err_bind(p.err);
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *bufs = base + STAGES * S::STAGE;
-    uint64_t *full = reinterpret_cast<uint64_t *>(bufs + LT_EPI_WARPS * LT_STAGE_BUF);
-    uint64_t *empty = full + STAGES, *acc_full = empty + STAGES;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_full + 1);
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; s++) {
-            mbar_init(&full[s], LT_EPI_WARPS);
-            mbar_init(&empty[s], 1);
-        }
-        mbar_init(acc_full, 1);
-        fence_barrier_init();
-    }
-    if (warp == LT_EPI_WARPS) tmem_alloc(tmem_slot, S::TMEM);
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
-    pdl_wait();
-    pdl_launch_dependents();
-
-    const uint32_t tiles = p.tiles_m * p.tiles_n, t = blockIdx.x % tiles, z = blockIdx.x / tiles;
-    const uint32_t n0 = t % p.tiles_n * BN, m0 = t / p.tiles_n * LT_BM;
-    const uint32_t blocks = (p.k + LT_BK - 1) / LT_BK;
-    const uint32_t kb0 = (uint32_t)((uint64_t)blocks * z / p.splits);
-    const uint32_t count = (uint32_t)((uint64_t)blocks * (z + 1) / p.splits) - kb0;
-    if (warp == LT_EPI_WARPS) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = lt_idesc<T>(LT_BM, BN, A_MN, B_MN);
-            for (uint32_t it = 0; it < count; it++) {
-                const uint32_t s = it % STAGES;
-                if (!mbar_wait(&full[s], (it / STAGES) & 1, JC_DEV_TIMEOUT_FULL)) break;
-                tc_fence_after();
-                const uint64_t ad = lt_desc<A_MN>(smem_u32(base + s * S::STAGE));
-                const uint64_t bd = lt_desc<B_MN>(smem_u32(base + s * S::STAGE + S::A_BYTES));
-#pragma unroll
-                for (int kk = 0; kk < LT_BK / 16; kk++)
-                    tc_mma_f16(tmem, ad + kk * LT_STEP<A_MN>, bd + kk * LT_STEP<B_MN>, idesc, it > 0 || kk > 0);
-                tc_commit(&empty[s]);
-            }
-            tc_commit(acc_full);
-        }
-    } else {
-        auto pairs = [](const LinearOperand &o, bool mn) {
-            return (reinterpret_cast<uintptr_t>(o.p) % 4 == 0) && (mn ? o.sk : o.si) % 2 == 0;
-        };
-        const bool pa = pairs(p.a, A_MN), pb = pairs(p.b, B_MN);
-        bool ok = true;
-        for (uint32_t it = 0; it < count; it++) {
-            const uint32_t s = it % STAGES, round = it / STAGES;
-            // All lanes wait: each writes into the stage.
-            if (round > 0 && !mbar_wait(&empty[s], (round & 1) ^ 1, JC_DEV_TIMEOUT_EMPTY)) ok = false;
-            if (!__all_sync(0xffffffffu, ok)) break;
-            const uint32_t k0 = (kb0 + it) * LT_BK;
-            uint8_t *st = base + s * S::STAGE;
-            lt_gather<LT_BM, A_MN>(st, p.a, m0, p.m, k0, p.k, pa);
-            lt_gather<BN, B_MN>(st + S::A_BYTES, p.b, n0, p.n, k0, p.k, pb);
-            fence_proxy_async();  // the MMAs read shared memory through the async proxy
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&full[s]);
-        }
-        ok = mbar_wait_sleep(acc_full, 0, JC_DEV_TIMEOUT_MMA);
-        if (__all_sync(0xffffffffu, ok)) {
-            tc_fence_after();
-            LtBias<S::CW> bias;
-            LtRes<S::CW> res;
-            bias.load(p.bias, n0 + (warp >> 2) * (BN / 2), p.n);
-            lt_epilogue<T, BN, ACT, false>(p, tmem, bufs + warp * LT_STAGE_BUF, warp, m0, n0, z, bias, res);
-        }
-    }
-    __syncwarp();
-    tc_fence_before();
-    __syncthreads();
-    if (warp == LT_EPI_WARPS) {
-        tc_fence_after();
-        tmem_dealloc(tmem, S::TMEM);
     }
 }
 

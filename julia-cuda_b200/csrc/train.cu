@@ -233,10 +233,47 @@ static bool make_operand_map(CUtensorMap *map, const LinearOperand &o, uint32_t 
     return false;
 }
 
-// Whether TMA can load an operand: its rows on 16-byte boundaries (and a row distance it can hold).
-static bool tma_ok(const LinearOperand &o, bool mn) {
-    const size_t ld = mn ? o.sk : o.si;
-    return aligned16(o.p, ld, 2) && ld * 2 < ((size_t)1 << 40);
+// Whether TMA can load a matrix: its rows on 16-byte boundaries (and a row distance it can hold).
+static bool tma_ok(const void *p, size_t ld) { return aligned16(p, ld, 2) && ld * 2 < ((size_t)1 << 40); }
+
+static size_t round_up(size_t v, size_t to) { return (v + to - 1) / to * to; }
+
+// A matrix argument's copy for TMA, if it needs one: where in the workspace, and how long.
+struct Pad {
+    bool need = false;
+    size_t at = 0, ld = 0, bytes = 0;
+};
+static Pad plan_pad(const void *p, size_t ld, uint32_t rows, uint32_t cols, size_t at) {
+    Pad d;
+    d.need = p && !tma_ok(p, ld);
+    d.at = at;
+    d.ld = round_up(cols, 8);
+    d.bytes = d.need ? round_up((size_t)rows * d.ld * 2, 256) : 0;
+    return d;
+}
+
+// Queues the copies of two matrices that need them and points the arguments at them.
+static bool launch_pads(uint8_t *ws, const Pad &a, const void **pa, size_t *lda, uint32_t rows_a, uint32_t cols_a,
+                        const Pad &b, const void **pb, size_t *ldb, uint32_t rows_b, uint32_t cols_b, cudaStream_t s) {
+    PadParams p{};
+    uint32_t blocks[2] = {0, 0};
+    auto add = [&](int i, const Pad &d, const void **src, size_t *ld, uint32_t rows, uint32_t cols) {
+        if (!d.need || rows == 0) return;
+        p.src[i] = static_cast<const uint16_t *>(*src);
+        p.ld[i] = *ld;
+        p.rows[i] = rows;
+        p.cols[i] = cols;
+        p.dst[i] = reinterpret_cast<uint16_t *>(ws + d.at);
+        p.ldd[i] = d.ld;
+        blocks[i] = (uint32_t)std::min<uint64_t>(((uint64_t)rows * (d.ld / 8) + 255) / 256, 148 * 16);
+        *src = ws + d.at;
+        *ld = d.ld;
+    };
+    add(0, a, pa, lda, rows_a, cols_a);
+    add(1, b, pb, ldb, rows_b, cols_b);
+    p.first = blocks[0];
+    if (blocks[0] + blocks[1] == 0) return true;
+    return launch_ex(linear_pad_kernel, dim3(blocks[0] + blocks[1]), dim3(256), 0, s, true, "linear", p);
 }
 
 static bool out_vec(const Product &q) {
@@ -276,15 +313,6 @@ static bool launch_tc(const Product &q, LinearTcParams &p, cudaStream_t s) {
     }
 }
 
-template <class T, int BN, bool A_MN, bool B_MN, uint32_t ACT>
-static bool launch_any(const LinearTcParams &p, cudaStream_t s) {
-    static std::atomic<uint64_t> smem_set{0};
-    auto kern = linear_any_kernel<T, BN, A_MN, B_MN, ACT>;
-    if (!ensure_smem(kern, LtAnySmem<BN>::BYTES, smem_set)) return false;
-    return launch_ex(kern, dim3(p.tiles_m * p.tiles_n * p.splits), dim3(LT_ANY_THREADS), LtAnySmem<BN>::BYTES, s,
-                     true, "linear", p);
-}
-
 // How the TMA kernel tiles a product: `ctas` x 128 rows by bn columns.
 struct Tiling {
     uint32_t ctas, bn;
@@ -314,8 +342,6 @@ static bool launch_product(const Product &q, cudaStream_t s) {
     p.m = q.m;
     p.n = q.n;
     p.k = q.k;
-    p.a = q.a;
-    p.b = q.b;
     p.bias = q.bias;
     p.res = q.res;
     p.ldres = q.ldres;
@@ -327,27 +353,15 @@ static bool launch_product(const Product &q, cudaStream_t s) {
     p.splits = q.splits;
     p.err = module_error_word();
     if (!p.err) return false;
-    p.tiles_m = (q.m + LT_BM - 1) / LT_BM;
-    auto tiles = [&](uint32_t bn) {
-        p.tiles_n = (q.n + bn - 1) / bn;
-        if ((uint64_t)p.tiles_m * p.tiles_n * p.splits <= 0x7FFFFFFFull) return true;
-        set_error("linear: too many tiles");
-        return false;
+    const Tiling t = pick_tiling(q.m, q.n, q.k, q.splits, (uint32_t)sm_count());
+    const bool vec = out_vec(q);
+    auto run = [&](auto c, auto w) {
+        constexpr int CTAS = decltype(c)::value, BN = decltype(w)::value;
+        return vec ? launch_tc<T, BN, CTAS, A_MN, B_MN, ACT, true>(q, p, s)
+                   : launch_tc<T, BN, CTAS, A_MN, B_MN, ACT, false>(q, p, s);
     };
-    if (tma_ok(q.a, A_MN) && tma_ok(q.b, B_MN)) {
-        const Tiling t = pick_tiling(q.m, q.n, q.k, q.splits, (uint32_t)sm_count());
-        const bool vec = out_vec(q);
-        auto run = [&](auto c, auto w) {
-            constexpr int CTAS = decltype(c)::value, BN = decltype(w)::value;
-            return vec ? launch_tc<T, BN, CTAS, A_MN, B_MN, ACT, true>(q, p, s)
-                       : launch_tc<T, BN, CTAS, A_MN, B_MN, ACT, false>(q, p, s);
-        };
-        if (t.ctas == 2) return t.bn == 256 ? run(Int<2>(), Int<256>()) : run(Int<2>(), Int<128>());
-        return t.bn == 128 ? run(Int<1>(), Int<128>()) : run(Int<1>(), Int<64>());
-    }
-    if (q.n <= 16) return tiles(16) && launch_any<T, 16, A_MN, B_MN, ACT>(p, s);
-    if (q.n <= 64) return tiles(64) && launch_any<T, 64, A_MN, B_MN, ACT>(p, s);
-    return tiles(128) && launch_any<T, 128, A_MN, B_MN, ACT>(p, s);
+    if (t.ctas == 2) return t.bn == 256 ? run(Int<2>(), Int<256>()) : run(Int<2>(), Int<128>());
+    return t.bn == 128 ? run(Int<1>(), Int<128>()) : run(Int<1>(), Int<64>());
 }
 
 // Calls f(N) for the smallest instantiated number of columns a thin layer of n has.
@@ -380,16 +394,23 @@ bool launch_linear(const LinearArgs &a, cudaStream_t s) {
                 });
             });
         });
-    if (a.m <= LINEAR_ROWS && vec)
+    if (a.m <= LINEAR_ROWS)
         return with_half(a.type, [&](auto t) {
             return with_act(a.act, [&](auto act) {
-                return launch_ex(linear_rows_kernel<decltype(t), decltype(act)::value>, dim3((a.n + 7) / 8, (a.m + 15) / 16),
-                                 dim3(32 * LR_WARPS), 0, s, true, "linear", rp);
+                using T = decltype(t);
+                constexpr uint32_t ACT = decltype(act)::value;
+                const dim3 grid((a.n + 7) / 8, (a.m + 15) / 16);
+                return vec ? launch_ex(linear_rows_kernel<T, ACT, true>, grid, dim3(32 * LR_WARPS), 0, s, true, "linear", rp)
+                           : launch_ex(linear_rows_kernel<T, ACT, false>, grid, dim3(32 * LR_WARPS), 0, s, true, "linear", rp);
             });
         });
+    const void *x = a.x, *w = a.w;
+    size_t ldx = a.ldx, ldw = a.ldw;
+    const Pad px = plan_pad(x, ldx, a.m, a.k, 0), pw = plan_pad(w, ldw, a.n, a.k, px.bytes);
+    if (!launch_pads(static_cast<uint8_t *>(a.ws), px, &x, &ldx, a.m, a.k, pw, &w, &ldw, a.n, a.k, s)) return false;
     Product q;
-    q.a = LinearOperand{a.x, a.ldx, 1};
-    q.b = LinearOperand{a.w, a.ldw, 1};
+    q.a = LinearOperand{x, ldx, 1};
+    q.b = LinearOperand{w, ldw, 1};
     q.m = a.m;
     q.n = a.n;
     q.k = a.k;
@@ -407,17 +428,24 @@ bool launch_linear(const LinearArgs &a, cudaStream_t s) {
     });
 }
 
+size_t linear_ws_bytes(const void *x, size_t ldx, const void *w, size_t ldw, uint32_t m, uint32_t n, uint32_t k) {
+    if (n <= LTHIN_MAX || m <= LINEAR_ROWS) return 0;
+    return plan_pad(x, ldx, m, k, 0).bytes + plan_pad(w, ldw, n, k, 0).bytes;
+}
+
 // The backward pass's workspace: dz (16 bits, rows padded to 16 bytes), the column sums' parts, dw's
-// partial products, each from a 256-byte boundary.
+// partial products, the copies of w and x where TMA cannot load them, each from a 256-byte boundary.
 struct LinearBwdPlan {
     uint32_t dz_parts, splits;
     uint32_t thin_blocks;  // n <= LTHIN_MAX: blocks along the rows, each with its sums; nothing else used
     size_t lddz, part_at, ws_at, bytes;
+    Pad w, x;
 };
 
-static LinearBwdPlan plan_linear_bwd(uint32_t m, uint32_t n, uint32_t k) {
+static LinearBwdPlan plan_linear_bwd(const void *x, size_t ldx, const void *w, size_t ldw, uint32_t m, uint32_t n,
+                                     uint32_t k) {
     LinearBwdPlan p{};
-    auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+    auto up = [](size_t v) { return round_up(v, 256); };
     p.dz_parts = (m + DZ_ROWS - 1) / DZ_ROWS;
     p.lddz = (n + 7) / 8 * 8;
     p.part_at = up((size_t)m * p.lddz * 2);
@@ -439,10 +467,15 @@ static LinearBwdPlan plan_linear_bwd(uint32_t m, uint32_t n, uint32_t k) {
         }
     }
     p.bytes = p.ws_at + (p.splits > 1 ? up((size_t)p.splits * n * k * 4) : 0);
+    p.w = plan_pad(w, ldw, n, k, p.bytes);
+    p.x = plan_pad(x, ldx, m, k, p.bytes + p.w.bytes);
+    p.bytes += p.w.bytes + p.x.bytes;
     return p;
 }
 
-size_t linear_bwd_ws_bytes(uint32_t m, uint32_t n, uint32_t k) { return plan_linear_bwd(m, n, k).bytes; }
+size_t linear_bwd_ws_bytes(const void *x, size_t ldx, const void *w, size_t ldw, uint32_t m, uint32_t n, uint32_t k) {
+    return plan_linear_bwd(x, ldx, w, ldw, m, n, k).bytes;
+}
 
 static bool launch_linear_thin_bwd(const LinearBwdArgs &a, uint32_t blocks, cudaStream_t s) {
     return with_half(a.type, [&](auto t) {
@@ -476,7 +509,7 @@ static bool launch_linear_thin_bwd(const LinearBwdArgs &a, uint32_t blocks, cuda
 }
 
 bool launch_linear_bwd(const LinearBwdArgs &a, cudaStream_t s) {
-    const LinearBwdPlan plan = plan_linear_bwd(a.m, a.n, a.k);
+    const LinearBwdPlan plan = plan_linear_bwd(a.dw ? a.x : nullptr, a.ldx, a.dx ? a.w : nullptr, a.ldw, a.m, a.n, a.k);
     uint8_t *ws = static_cast<uint8_t *>(a.ws);
     if (plan.thin_blocks) return launch_linear_thin_bwd(a, plan.thin_blocks, s);
     float *part = reinterpret_cast<float *>(ws + plan.part_at);
@@ -506,10 +539,13 @@ bool launch_linear_bwd(const LinearBwdArgs &a, cudaStream_t s) {
                 }))
                 return false;
         }
+        const void *x = a.x, *w = a.w;
+        size_t ldx = a.ldx, ldw = a.ldw;
+        if (a.m > 0 && !launch_pads(ws, plan.w, &w, &ldw, a.n, a.k, plan.x, &x, &ldx, a.m, a.k, s)) return false;
         if (a.dx && a.m > 0) {
             Product q;
             q.a = LinearOperand{dz, lddz, 1};
-            q.b = LinearOperand{a.w, 1, a.ldw};
+            q.b = LinearOperand{w, 1, ldw};
             q.m = a.m;
             q.n = a.k;
             q.k = a.n;
@@ -522,7 +558,7 @@ bool launch_linear_bwd(const LinearBwdArgs &a, cudaStream_t s) {
             if (a.m > 0) {
                 Product q;
                 q.a = LinearOperand{dz, 1, lddz};
-                q.b = LinearOperand{a.x, 1, a.ldx};
+                q.b = LinearOperand{x, 1, ldx};
                 q.m = a.n;
                 q.n = a.k;
                 q.k = a.m;

@@ -55,7 +55,9 @@ struct LinearArgs {
     void *z = nullptr;
     size_t ldz = 0;
     uint32_t m = 0, n = 0, k = 0;
+    void *ws = nullptr;
 };
+size_t linear_ws_bytes(const void *x, size_t ldx, const void *w, size_t ldw, uint32_t m, uint32_t n, uint32_t k);
 bool launch_linear(const LinearArgs &a, cudaStream_t s);
 
 struct LinearBwdArgs {
@@ -76,7 +78,7 @@ struct LinearBwdArgs {
     float *dbias = nullptr;
     void *ws = nullptr;
 };
-size_t linear_bwd_ws_bytes(uint32_t m, uint32_t n, uint32_t k);
+size_t linear_bwd_ws_bytes(const void *x, size_t ldx, const void *w, size_t ldw, uint32_t m, uint32_t n, uint32_t k);
 bool launch_linear_bwd(const LinearBwdArgs &a, cudaStream_t s);
 
 struct LossArgs {

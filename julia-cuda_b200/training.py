@@ -109,9 +109,11 @@ def _act(op: str, act: str) -> int:
     return code
 
 
-def linear(x, w, y, *, bias=None, act: str = "none", res=None, z=None, stream=None) -> None:
+def linear(x, w, y, *, bias=None, act: str = "none", res=None, z=None, ws=None, stream=None) -> None:
     """y = act(x w^T + bias) + res (jc_linear): x [m, k], w [n, k], y, res [m, n] of one 16-bit type,
-    bias [n] f32. z, if given, keeps the values before the activation for the backward pass."""
+    bias [n] f32. z, if given, keeps the values before the activation for the backward pass. ws:
+    jc_linear_ws_bytes(...) bytes, needed where rows of x or w start off 16-byte boundaries (allocated
+    here when not given)."""
     t = _type("linear", x, halves=True)
     m, k = x.shape
     n = w.shape[0]
@@ -120,16 +122,24 @@ def linear(x, w, y, *, bias=None, act: str = "none", res=None, z=None, stream=No
     rp, ldres = _matrix("linear", "res", res, m, n, x.dtype)
     yp, ldy = _matrix("linear", "y", y, m, n, x.dtype)
     zp, ldz = _matrix("linear", "z", z, m, n, x.dtype)
+    wsp = None
+    if (xp | wp | 2 * ldx | 2 * ldw) % 16:
+        need = lib().jc_linear_ws_bytes(xp, ldx, wp, ldw, m, n, k)
+        if need and ws is None:
+            ws = _scratch(need, torch.uint8, x, stream)
+        elif need and ws.numel() * ws.element_size() < need:
+            _fail(f"linear: ws needs {need} bytes")
+        wsp = ws.data_ptr() if need else None
     _check(lib().jc_linear(t, _act("linear", act), xp, ldx, wp, ldw,
                            _vector("linear", "bias", bias, n), rp, ldres, yp, ldy, zp, ldz, m, n, k,
-                           _stream(stream)), "jc_linear")
+                           wsp, _stream(stream)), "jc_linear")
 
 
 def linear_backward(dy, x, w, *, z=None, act: str = "none", dx=None, dw=None, dbias=None, ws=None,
                     stream=None) -> None:
     """The gradients of linear (jc_linear_backward), each written if its tensor is given: dx [m, k],
     dw [n, k] of x's type, dbias [n] f32. z (linear's) is read unless act is "none". ws:
-    jc_linear_ws_bytes(m, n, k) bytes (allocated here when not given)."""
+    jc_linear_backward_ws_bytes(...) bytes (allocated here when not given)."""
     op = "linear_backward"
     t = _type(op, x, halves=True)
     m, k = x.shape
@@ -141,7 +151,7 @@ def linear_backward(dy, x, w, *, z=None, act: str = "none", dx=None, dw=None, db
     zp, ldz = _matrix(op, "z", z, m, n, x.dtype)
     dxp, lddx = _matrix(op, "dx", dx, m, k, x.dtype)
     dwp, lddw = _matrix(op, "dw", dw, n, k, x.dtype)
-    need = lib().jc_linear_ws_bytes(m, n, k)
+    need = lib().jc_linear_backward_ws_bytes(xp, ldx, wp, ldw, m, n, k)
     if need and ws is None:
         ws = _scratch(need, torch.uint8, x, stream)
     elif need and ws.numel() * ws.element_size() < need:

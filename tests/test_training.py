@@ -45,13 +45,14 @@ def test_linear_refusals(jc, buf):
     L, p = jc.lib(), buf[1]
 
     def fwd(type=0, act=0, x=p, ldx=8, w=p, ldw=8, bias=None, res=None, ldres=8, y=p, ldy=8, z=None, ldz=8, m=2,
-            n=8, k=8):
-        return L.jc_linear(type, act, x, ldx, w, ldw, bias, res, ldres, y, ldy, z, ldz, m, n, k, None)
+            n=8, k=8, ws=None):
+        return L.jc_linear(type, act, x, ldx, w, ldw, bias, res, ldres, y, ldy, z, ldz, m, n, k, ws, None)
     for kw, why in ((dict(type=2), "JC_F16 or JC_BF16"), (dict(act=1), "act"), (dict(act=RELU | GELU), "act"),
                     (dict(n=0), "must not be 0"), (dict(k=0), "must not be 0"), (dict(x=None), "x is null"),
                     (dict(w=None), "w is null"), (dict(y=None), "y is null"), (dict(ldw=7), "w's rows"),
                     (dict(res=p, ldres=2), "res's rows"), (dict(z=p + 1), "z is not aligned"),
-                    (dict(bias=p + 2), "bias")):
+                    (dict(bias=p + 2), "bias"), (dict(m=20, n=9, k=7, ldx=9, ldy=9), "ws is null"),
+                    (dict(m=20, n=9, k=7, ldx=9, ldy=9, ws=p + 8), "ws is misaligned")):
         assert fwd(**kw) == -1 and why in jc.last_error(), (kw, jc.last_error())
     assert fwd(m=0, x=None, y=None) == 0
 
@@ -62,8 +63,14 @@ def test_linear_refusals(jc, buf):
                     (dict(act=RELU), "z is null"), (dict(lddw=1), "dw's rows"), (dict(ws=None), "ws is null"),
                     (dict(ws=p + 16), "ws is misaligned")):
         assert bwd(**kw) == -1 and why in jc.last_error(), (kw, jc.last_error())
-    assert L.jc_linear_ws_bytes(4096, 2048, 768) >= 4096 * 2048 * 2   # dz
-    assert L.jc_linear_ws_bytes(10, 0, 5) == 0
+    size = L.jc_linear_backward_ws_bytes
+    assert size(p, 768, p, 768, 4096, 2048, 768) >= 4096 * 2048 * 2   # dz
+    assert size(p, 768, p, 768, 10, 0, 5) == 0
+    assert L.jc_linear_ws_bytes(p, 768, p, 768, 4096, 2048, 768) == 0
+    # A copy of x, of w, or of both, their rows on 16-byte boundaries.
+    assert L.jc_linear_ws_bytes(p, 769, p, 768, 100, 64, 768) == 100 * 768 * 2
+    assert L.jc_linear_ws_bytes(p, 768, p + 2, 768, 100, 64, 768) == 64 * 768 * 2
+    assert L.jc_linear_ws_bytes(p, 767, p, 767, 100, 64, 767) == 164 * 768 * 2
 
 
 def test_choice_loss_refusals(jc, buf):
