@@ -26,6 +26,7 @@ struct AdamwParams {
     const float *grad_scale;
     float beta1, beta2, one_minus_beta1, one_minus_beta2, lr, eps;
     float inv_bias1, inv_bias2;  // 1 / (1 - beta^t)
+    float minus_zero;
 };
 
 // The largest of a warp's values, none below 0: their bits order as they do.
@@ -216,19 +217,21 @@ __global__ void __launch_bounds__(ADAMW_THREADS, BITS == 8 ? 3 : 4) adamw_kernel
             const float keep[2] = {k, k}, rate[2] = {up, up}, gs2[2] = {gs, gs}, b1[2] = {p.beta1, p.beta1},
                         b2[2] = {p.beta2, p.beta2}, c1[2] = {p.one_minus_beta1, p.one_minus_beta1},
                         c2[2] = {p.one_minus_beta2, p.one_minus_beta2}, ib2[2] = {p.inv_bias2, p.inv_bias2},
-                        eps[2] = {p.eps, p.eps};
+                        eps[2] = {p.eps, p.eps}, none[2] = {p.minus_zero, p.minus_zero};
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
-                // Each operation of the states rounded by itself, so that an 8-bit code does not
-                // depend on how a compiler contracts them.
+                // Each operation of the states is rounded by itself, so that an 8-bit code is that of the
+                // formula's own operations. A pair's multiplication and addition the assembler fuses
+                // even when both say .rn; a product written as a fused multiply-add of a -0 that it
+                // does not know stays apart.
                 float a[2], b[2];
                 mul2(g + j, g + j, gs2);
-                mul2(m + j, m + j, b1);
-                mul2(a, g + j, c1);
+                fma2(m + j, m + j, b1, none);
+                fma2(a, g + j, c1, none);
                 add2(m + j, m + j, a);
-                mul2(v + j, v + j, b2);
+                fma2(v + j, v + j, b2, none);
                 mul2(a, g + j, c2);
-                mul2(a, a, g + j);
+                fma2(a, a, g + j, none);
                 add2(v + j, v + j, a);
                 // The quotient and root to a few ulp: their error is far below the parameter's own. A
                 // subnormal v divides by ROOT_MIN + eps: finite with eps 0 too.

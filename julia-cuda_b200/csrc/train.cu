@@ -628,6 +628,7 @@ bool launch_adamw(const AdamwStep &a, cudaStream_t s) {
     p.one_minus_beta2 = (float)(1.0 - a.beta2);
     p.lr = a.lr;
     p.eps = a.eps;
+    p.minus_zero = -0.0f;
     p.inv_bias1 = (float)(1.0 / (1.0 - std::pow(a.beta1, (double)a.step)));
     p.inv_bias2 = (float)(1.0 / (1.0 - std::pow(a.beta2, (double)a.step)));
     p.n_chunks = a.n_chunks;

@@ -9,15 +9,26 @@ import ctypes
 
 import torch
 
-from . import EPI_GELU, EPI_RELU, JuliaCudaError, _check, _stream, last_error, lib
+from . import EPI_GELU, EPI_RELU, JuliaCudaError, _check, last_error, lib
 
 F16, BF16, F32 = 0, 1, 2
 _TYPES = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}
 _ACTS = {"none": 0, "relu": EPI_RELU, "gelu": EPI_GELU}
 
 
+# A call's host time is most of a small operator's: these are the cheapest forms of what they ask.
+_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _fail(what: str):
     raise JuliaCudaError(what)
+
+
+def _stream(stream, dev: int):
+    if stream is None:
+        return _raw_stream(dev)
+    return getattr(stream, "cuda_stream", stream)
 
 
 def _matrix(op: str, name: str, t, rows: int, cols: int, dtype):
@@ -44,14 +55,20 @@ def _vector(op: str, name: str, t, n: int, dtype=torch.float32):
     return t.data_ptr()
 
 
-def _type(op: str, t, halves: bool = False) -> int:
+def _type(op: str, t, halves: bool = False):
+    """(element type, device) of x."""
     code = _TYPES.get(t.dtype)
     if code is None or t.dim() != 2 or (halves and code == F32):
         _fail(f"{op}: x must be a matrix of float16{', ' if not halves else ' or '}bfloat16"
               f"{'' if halves else ' or float32'}")
-    if t.get_device() != torch.cuda.current_device():
+    return code, _on_device(op, t)
+
+
+def _on_device(op: str, t) -> int:
+    dev = t.get_device()
+    if dev < 0 or dev != _device():
         _fail(f"{op}: the tensors are not on the current device")
-    return code
+    return dev
 
 
 def _scratch(n: int, dtype, like, stream):
@@ -67,13 +84,13 @@ def layer_norm(x, gamma, beta, y, stats=None, eps: float = 1e-5, stream=None) ->
     """y = (x - mean) rstd gamma + beta per row (jc_layer_norm). x, y [rows, d] of one type (f16, bf16
     or f32), gamma and beta [d] f32 (beta may be None); stats, if given, [rows, 2] f32 receives mean
     and rstd for the backward pass."""
-    t = _type("layer_norm", x)
+    t, dev = _type("layer_norm", x)
     rows, d = x.shape
     xp, ldx = _matrix("layer_norm", "x", x, rows, d, x.dtype)
     yp, ldy = _matrix("layer_norm", "y", y, rows, d, x.dtype)
     _check(lib().jc_layer_norm(t, xp, ldx, _vector("layer_norm", "gamma", gamma, d),
                                _vector("layer_norm", "beta", beta, d), eps, rows, d, yp, ldy,
-                               _vector("layer_norm", "stats", stats, 2 * rows), _stream(stream)),
+                               _vector("layer_norm", "stats", stats, 2 * rows), _stream(stream, dev)),
            "jc_layer_norm")
 
 
@@ -83,7 +100,7 @@ def layer_norm_backward(dy, x, gamma, stats, dx, dgamma=None, dbeta=None, add=No
     reaches x past the norm), dgamma and dbeta [d] f32. ws: jc_layer_norm_ws_floats(rows, d) floats
     (allocated here when not given)."""
     op = "layer_norm_backward"
-    t = _type(op, x)
+    t, dev = _type(op, x)
     rows, d = x.shape
     xp, ldx = _matrix(op, "x", x, rows, d, x.dtype)
     dyp, lddy = _matrix(op, "dy", dy, rows, d, x.dtype)
@@ -99,7 +116,7 @@ def layer_norm_backward(dy, x, gamma, stats, dx, dgamma=None, dbeta=None, add=No
                                         dxp, lddx, _vector(op, "dgamma", dgamma, d),
                                         _vector(op, "dbeta", dbeta, d),
                                         ws.data_ptr() if need else None,
-                                        _stream(stream)), "jc_layer_norm_backward")
+                                        _stream(stream, dev)), "jc_layer_norm_backward")
 
 
 def _act(op: str, act: str) -> int:
@@ -114,7 +131,7 @@ def linear(x, w, y, *, bias=None, act: str = "none", res=None, z=None, ws=None, 
     bias [n] f32. z, if given, keeps the values before the activation for the backward pass. ws:
     jc_linear_ws_bytes(...) bytes, needed where rows of x or w start off 16-byte boundaries (allocated
     here when not given)."""
-    t = _type("linear", x, halves=True)
+    t, dev = _type("linear", x, halves=True)
     m, k = x.shape
     n = w.shape[0]
     xp, ldx = _matrix("linear", "x", x, m, k, x.dtype)
@@ -132,7 +149,7 @@ def linear(x, w, y, *, bias=None, act: str = "none", res=None, z=None, ws=None, 
         wsp = ws.data_ptr() if need else None
     _check(lib().jc_linear(t, _act("linear", act), xp, ldx, wp, ldw,
                            _vector("linear", "bias", bias, n), rp, ldres, yp, ldy, zp, ldz, m, n, k,
-                           wsp, _stream(stream)), "jc_linear")
+                           wsp, _stream(stream, dev)), "jc_linear")
 
 
 def linear_backward(dy, x, w, *, z=None, act: str = "none", dx=None, dw=None, dbias=None, ws=None,
@@ -141,7 +158,7 @@ def linear_backward(dy, x, w, *, z=None, act: str = "none", dx=None, dw=None, db
     dw [n, k] of x's type, dbias [n] f32. z (linear's) is read unless act is "none". ws:
     jc_linear_backward_ws_bytes(...) bytes (allocated here when not given)."""
     op = "linear_backward"
-    t = _type(op, x, halves=True)
+    t, dev = _type(op, x, halves=True)
     m, k = x.shape
     n = w.shape[0]
     a = _act(op, act)
@@ -158,7 +175,7 @@ def linear_backward(dy, x, w, *, z=None, act: str = "none", dx=None, dw=None, db
         _fail(f"{op}: ws needs {need} bytes")
     _check(lib().jc_linear_backward(t, a, dyp, lddy, xp, ldx, wp, ldw, zp, ldz, m, n, k, dxp, lddx,
                                     dwp, lddw, _vector(op, "dbias", dbias, n), ws.data_ptr() if need else None,
-                                    _stream(stream)), "jc_linear_backward")
+                                    _stream(stream, dev)), "jc_linear_backward")
 
 
 def choice_loss(logits, offsets, gold, loss, dlogits=None, weight=None, stream=None) -> None:
@@ -167,13 +184,12 @@ def choice_loss(logits, offsets, gold, loss, dlogits=None, weight=None, stream=N
     none), weight f32 [requests]; writes loss [requests] and dlogits (as logits)."""
     op = "choice_loss"
     n, r = logits.numel(), gold.numel()
-    if logits.get_device() != torch.cuda.current_device():
-        _fail(f"{op}: the tensors are not on the current device")
+    dev = _on_device(op, logits)
     _check(lib().jc_choice_loss(_vector(op, "logits", logits, n), n,
                                 _vector(op, "offsets", offsets, r + 1, torch.int32),
                                 _vector(op, "gold", gold, r, torch.int32),
                                 _vector(op, "weight", weight, r), r, _vector(op, "loss", loss, r),
-                                _vector(op, "dlogits", dlogits, n), _stream(stream)),
+                                _vector(op, "dlogits", dlogits, n), _stream(stream, dev)),
            "jc_choice_loss")
 
 
@@ -201,6 +217,7 @@ class AdamW:
     def __init__(self, params, grads, *, bits: int = 32, weight_decay=0.0, copies=None, exp_avg=None,
                  exp_avg_sq=None, exp_avg_scale=None, exp_avg_sq_scale=None):
         self._h = None
+        self._dev = _device()
         n = len(params)
         if bits not in (8, 32):
             _fail("AdamW: states of 32 or 8 bits")
@@ -225,8 +242,7 @@ class AdamW:
         table = (AdamwTensor * max(n, 1))()
         for i, p in enumerate(self.params):
             k, g, c, at = p.numel(), self.grads[i], self.copies[i], f"of tensor {i}"
-            if p.device.index != torch.cuda.current_device():
-                _fail("AdamW: the tensors are not on the current device")
+            _on_device("AdamW", p)
             if g.dtype not in _TYPES:
                 _fail(f"AdamW: the gradient {at} must be float16, bfloat16 or float32")
             if c is not None and c.dtype not in (torch.float16, torch.bfloat16):
@@ -250,7 +266,8 @@ class AdamW:
              stream=None) -> None:
         """Step t (from 1). grad_scale: one f32 on the device that every gradient is multiplied by."""
         _check(lib().jc_adamw_step(self._h, t, lr, betas[0], betas[1], eps,
-                                   _vector("AdamW", "grad_scale", grad_scale, 1), _stream(stream)),
+                                   _vector("AdamW", "grad_scale", grad_scale, 1),
+                                   _stream(stream, self._dev)),
                "jc_adamw_step")
 
     def close(self) -> None:

@@ -562,6 +562,37 @@ def test_adamw(jc, bits, grad, copy, shift):
     opt.close()
 
 
+@pytest.mark.parametrize("grad", TYPES)
+def test_adamw_8bit_codes_are_exact(jc, grad):
+    """Codes and scales are those of the formula's operations rounded one by one in f32 (torch's own
+    multiplications, additions and divisions), bit for bit, over several steps."""
+    g = gen(77)
+    n = 300 * 256
+    p, grads = normal(g, n, std=0.02), normal(g, n, std=1e-3, dtype=grad)
+    grads[5 * 256:6 * 256] = 0   # a block without gradients
+    grads[7 * 256 + 3] = 1.0     # and one with a single large one
+    scale = torch.full((1,), 0.37, device="cuda")
+    opt = jc.AdamW([p], [grads], bits=8)
+    m = v = torch.zeros(300, 256, device="cuda")
+    for t in range(1, 6):
+        grads.copy_(grads.float() * (1 + 0.1 * t))
+        opt.step(t, lr=1e-3, betas=(0.9, 0.999), grad_scale=scale)
+        gf = grads.float().view(300, 256) * scale
+        m = (m * 0.9) + (gf * (1 - 0.9))
+        v = (v * 0.999) + (gf * (1 - 0.999)) * gf
+        out = []
+        for x, floor in ((m, False), (v, True)):
+            sc = x.abs().amax(1) * torch.tensor(1.0 / 448.0, dtype=torch.float32, device="cuda")
+            y = x / torch.where(sc > 0, sc, 1.0)[:, None]
+            y = torch.where(x > 0, y.clamp_min(2.0 ** -9), y) if floor else y
+            out.append((y.clamp(-448, 448).to(torch.float8_e4m3fn), sc))
+        (mc, ms), (vc, vs) = out
+        assert torch.equal(opt.exp_avg_scale[0], ms) and torch.equal(opt.exp_avg_sq_scale[0], vs), t
+        assert torch.equal(opt.exp_avg[0].view(torch.uint8), mc.view(-1).view(torch.uint8)), t
+        assert torch.equal(opt.exp_avg_sq[0].view(torch.uint8), vc.view(-1).view(torch.uint8)), t
+        m, v = mc.float() * ms[:, None], vc.float() * vs[:, None]
+
+
 def test_adamw_does_not_touch_its_neighbours(jc):
     base = torch.full((3000,), 5.0, device="cuda")
     grads = torch.ones(3000, device="cuda")
