@@ -155,7 +155,7 @@ int jc_linear(uint32_t type, uint32_t act, const void *x, size_t ldx, const void
         if (!check_matrix(op, "x", x, ldx, k, 2, any) || !check_matrix(op, "w", w, ldw, k, 2, true) ||
             !check_vector(op, "bias", bias, 4, false) || !check_matrix(op, "res", res, ldres, n, 2, false) ||
             !check_matrix(op, "y", y, ldy, n, 2, any) || !check_matrix(op, "z", z, ldz, n, 2, false) ||
-            !check_vector(op, "ws", ws, 256, any && jc::linear_ws_bytes(x, ldx, w, ldw, m, n, k) > 0))
+            !check_vector(op, "ws", ws, 256, any && !ws && jc::linear_ws_bytes(x, ldx, w, ldw, m, n, k) > 0))
             return -1;
         jc::LinearArgs a;
         a.ws = ws;
@@ -202,7 +202,7 @@ int jc_linear_backward(uint32_t type, uint32_t act, const void *dy, size_t lddy,
             !check_matrix(op, "z", z, ldz, n, 2, any && act) ||
             !check_matrix(op, "dx", dx, lddx, k, 2, false) || !check_matrix(op, "dw", dw, lddw, k, 2, false) ||
             !check_vector(op, "dbias", dbias, 4, false) ||
-            !check_vector(op, "ws", ws, 256, any && jc::linear_bwd_ws_bytes(dw ? x : nullptr, ldx, dx ? w : nullptr, ldw, m, n, k) > 0))
+            !check_vector(op, "ws", ws, 256, any && !ws && jc::linear_bwd_ws_bytes(dw ? x : nullptr, ldx, dx ? w : nullptr, ldw, m, n, k) > 0))
             return -1;
         jc::LinearBwdArgs a;
         a.type = type;

@@ -328,10 +328,16 @@ static double tc_us(uint32_t m, uint32_t n, uint32_t k, Tiling t, uint32_t split
     return (double)((items + units - 1) / units) * (0.28 * blocks + 0.5) + 2.0 + 0.008 * t.bn;
 }
 
-static Tiling pick_tiling(uint32_t m, uint32_t n, uint32_t k, uint32_t splits, uint32_t sms) {
+static Tiling pick_tiling(uint32_t m, uint32_t n, uint32_t k, uint32_t splits, uint32_t sms, double *us = nullptr) {
     Tiling best = TILINGS[0];
-    for (const Tiling &t : TILINGS)
-        if (tc_us(m, n, k, t, splits, sms) <= tc_us(m, n, k, best, splits, sms)) best = t;
+    double least = 1e30;
+    for (const Tiling &t : TILINGS) {
+        const double v = tc_us(m, n, k, t, splits, sms);
+        if (v > least) continue;
+        best = t;
+        least = v;
+    }
+    if (us) *us = least;
     return best;
 }
 
@@ -459,8 +465,11 @@ static LinearBwdPlan plan_linear_bwd(const void *x, size_t ldx, const void *w, s
         return p;
     }
     double best = 1e30;
-    for (uint32_t s = 1; s <= std::min(32u, std::max(1u, blocks)); s++) {
-        const double us = tc_us(n, k, m, pick_tiling(n, k, m, s, sms), s, sms) + (s > 1 ? 2.0 + 8e-6 * s * n * k / 3.0 : 0.0);
+    for (uint32_t s : {1u, 2u, 3u, 4u, 5u, 6u, 8u, 12u, 16u, 24u, 32u}) {
+        if (s > std::max(1u, blocks)) break;
+        double us;
+        pick_tiling(n, k, m, s, sms, &us);
+        if (s > 1) us += 2.0 + 8e-6 * s * n * k / 3.0;  // the partial sums, written and read
         if (us < best) {
             best = us;
             p.splits = s;
