@@ -14,7 +14,9 @@
 // epilogue of one tile under the main loop of the next (two accumulators). CTAS 2: pairs of CTAs on 256 x
 // BN tiles (cta_group::2), each with 128 rows of a and half of the rows of b, for a third fewer operand
 // bytes per SM than a 128 x 256 tile: alone, such a tile asks an SM for 48 KB per 512 tensor cycles, more
-// than the 64 bytes a cycle it can take in.
+// than the 64 bytes a cycle it can take in. The two products of the backward pass, whose second operands
+// lie alike, are one launch (GRADS): dw's few long items first, dx's many short ones after them, so no SM
+// waits for the other product's last tiles and dw's partial sums go out under dx's main loop.
 #pragma once
 #include <type_traits>
 
@@ -39,8 +41,7 @@ __host__ __device__ constexpr uint32_t lt_idesc(int m, int n, bool a_mn, bool b_
 //   K-major:  rows of 64 contracted elements (128 bytes), 8-row groups 1024 bytes apart.
 //   MN-major: blocks of 64 rows of the contracted axis x 64 elements of the other (8 KB); the next
 //             8 contracted rows 1024 bytes on, the next 64 of the other axis a block on.
-template <bool MN>
-__device__ __forceinline__ uint64_t lt_desc(uint32_t saddr) {
+__device__ __forceinline__ uint64_t lt_desc(uint32_t saddr, bool MN) {
     uint64_t d = umma_desc_sw128(saddr);
     if (MN) d = (d & ~((uint64_t)0x3FFF << 16)) | ((uint64_t)(8192 >> 4) << 16);
     return d;
@@ -48,8 +49,7 @@ __device__ __forceinline__ uint64_t lt_desc(uint32_t saddr) {
 
 // Descriptor step (16-byte units) for the next 16 contracted elements: 32 bytes inside a row, or 16
 // rows on.
-template <bool MN>
-constexpr uint32_t LT_STEP = MN ? (16 * 128) >> 4 : 32 >> 4;
+__device__ __forceinline__ uint32_t lt_step(bool MN) { return MN ? (16 * 128) >> 4 : 32 >> 4; }
 
 struct LinearTcParams {
     uint32_t m, n, k;
@@ -63,12 +63,14 @@ struct LinearTcParams {
     float *ws;        // split over k: [splits][m][n] partial sums instead of c
     uint32_t splits;
     uint32_t tiles_m, tiles_n;
-    unsigned int *err;
 };
 
+// One product, or (GRADS) dw's and dx's, dw's a MN-major. Items of the second follow the first's.
 struct LinearTcKernelParams {
-    CUtensorMap map_a, map_b;
-    LinearTcParams p;
+    CUtensorMap map_a[2], map_b[2];
+    LinearTcParams p[2];
+    uint32_t items[2];
+    unsigned int *err;
 };
 
 template <int BN>
@@ -212,7 +214,8 @@ __device__ __forceinline__ void lt_acc(uint32_t taddr, float *v) {
 // One warp's share of a finished tile: rows 32 (warp % 4).. and half warp / 4 of the columns. `acc`:
 // the tile's accumulator; `bias`, `res`: the first chunk's, requested before the accumulator was ready
 // (the residual only with VEC).
-template <class T, int BN, uint32_t ACT, bool VEC>
+// GRADS: partial sums or plain values, nothing added.
+template <class T, int BN, bool GRADS, uint32_t ACT, bool VEC>
 __device__ __forceinline__ void lt_epilogue(const LinearTcParams &p, uint32_t acc, uint8_t *buf, uint32_t warp,
                                             uint32_t m0, uint32_t n0, uint32_t split,
                                             LtBias<LtShape<BN>::CW> &bias, LtRes<LtShape<BN>::CW> &res) {
@@ -225,7 +228,7 @@ __device__ __forceinline__ void lt_epilogue(const LinearTcParams &p, uint32_t ac
         const uint32_t cc = (warp >> 2) * (BN / 2) + ch * CW, c0 = n0 + cc;
         float v[CW];
         lt_acc<CW>(lane_acc + cc, v);
-        if (p.ws) {
+        if (GRADS && p.ws) {
             // Partial sums, f32, 32 columns (128 bytes) at a time.
             uint8_t *ws = reinterpret_cast<uint8_t *>(p.ws + (size_t)split * p.m * p.n);
             constexpr int PW = 32;
@@ -242,11 +245,11 @@ __device__ __forceinline__ void lt_epilogue(const LinearTcParams &p, uint32_t ac
             }
             continue;
         }
-        if (p.bias) {
+        if (!GRADS && p.bias) {
             bias.add(buf, v);
             if (ch + 1 < S::CHUNKS) bias.load(p.bias, c0 + CW, p.n);
         }
-        if (p.z) {
+        if (!GRADS && p.z) {
             __syncwarp();
             lt_put_row<T, CW>(buf, v);
             __syncwarp();
@@ -256,7 +259,7 @@ __device__ __forceinline__ void lt_epilogue(const LinearTcParams &p, uint32_t ac
 #pragma unroll
             for (int j = 0; j < CW; j++) v[j] = act_fwd<ACT>(v[j]);
         }
-        if (p.res) {
+        if (!GRADS && p.res) {
             const uint8_t *g = static_cast<const uint8_t *>(p.res);
             __syncwarp();
             if constexpr (VEC) {
@@ -303,14 +306,14 @@ struct LtTcSmem {
 
 constexpr int LT_TC_THREADS = 32 * (LT_EPI_WARPS + 2);
 
-template <class T, int BN, int CTAS, bool A_MN, bool B_MN, uint32_t ACT, bool VEC>
+template <class T, int BN, int CTAS, bool GRADS, uint32_t ACT, bool VEC>
 __global__ void __launch_bounds__(LT_TC_THREADS, 1)
     linear_tc_kernel(const __grid_constant__ LinearTcKernelParams kp) {
     using S = LtShape<BN>;
     using M = LtTcSmem<BN, CTAS>;
     constexpr int STAGES = M::STAGES;
-    const LinearTcParams &p = kp.p;
-    dev_err_bind(p.err);
+    constexpr bool B_MN = GRADS;
+    dev_err_bind(kp.err);
     extern __shared__ uint8_t smem_raw[];
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *bufs = base + STAGES * M::STAGE;
@@ -350,20 +353,33 @@ __global__ void __launch_bounds__(LT_TC_THREADS, 1)
     pdl_wait();
     pdl_launch_dependents();
 
-    const uint32_t tiles = p.tiles_m * p.tiles_n, items = tiles * p.splits;
-    const uint32_t blocks = (p.k + LT_BK - 1) / LT_BK;
+    // Item i: which product (w), its tile's first column and row, its split and its k-blocks.
+    struct Item {
+        uint32_t w, n0, m0, z, k0, k1;
+    };
+    const uint32_t items = kp.items[0] + (GRADS ? kp.items[1] : 0);
+    auto item = [&](uint32_t i) {
+        Item e;
+        e.w = GRADS && i >= kp.items[0];
+        const LinearTcParams &p = kp.p[e.w];
+        const uint32_t j = e.w ? i - kp.items[0] : i, tiles = p.tiles_m * p.tiles_n, t = j % tiles;
+        const uint32_t blocks = (p.k + LT_BK - 1) / LT_BK;
+        e.z = j / tiles;
+        e.n0 = t % p.tiles_n * BN;
+        e.m0 = (t / p.tiles_n * CTAS + rank) * LT_BM;
+        e.k0 = (uint32_t)((uint64_t)blocks * e.z / p.splits);
+        e.k1 = (uint32_t)((uint64_t)blocks * (e.z + 1) / p.splits);
+        return e;
+    };
     if (warp == LT_EPI_WARPS) {
         if (lane == 0) {
-            tma_prefetch_desc(&kp.map_a);
-            tma_prefetch_desc(&kp.map_b);
             const uint32_t leader = CTAS == 2 ? map_to_rank(smem_u32(full), 0) : 0;
             uint32_t it = 0;
             bool ok = true;
             for (uint32_t i = unit; ok && i < items; i += units) {
-                const uint32_t t = i % tiles, z = i / tiles;
-                const uint32_t n0 = t % p.tiles_n * BN + rank * (BN / CTAS), m0 = (t / p.tiles_n * CTAS + rank) * LT_BM;
-                const uint32_t k1 = (uint32_t)((uint64_t)blocks * (z + 1) / p.splits);
-                for (uint32_t kb = (uint32_t)((uint64_t)blocks * z / p.splits); kb < k1; kb++, it++) {
+                const Item e = item(i);
+                const CUtensorMap *map_a = &kp.map_a[e.w], *map_b = &kp.map_b[e.w];
+                for (uint32_t kb = e.k0; kb < e.k1; kb++, it++) {
                     const uint32_t s = it % STAGES, round = it / STAGES;
                     if (round > 0 && !mbar_wait(&empty[s], (round & 1) ^ 1, JC_DEV_TIMEOUT_EMPTY)) {
                         ok = false;
@@ -371,8 +387,12 @@ __global__ void __launch_bounds__(LT_TC_THREADS, 1)
                     }
                     uint8_t *st = base + s * M::STAGE;
                     if (rank == 0) mbar_arrive_expect_tx(&full[s], CTAS * M::STAGE);
-                    lt_tma<CTAS, LT_BM, A_MN>(st, &kp.map_a, &full[s], leader + s * 8, m0, kb * LT_BK);
-                    lt_tma<CTAS, BN / CTAS, B_MN>(st + M::A_BYTES, &kp.map_b, &full[s], leader + s * 8, n0, kb * LT_BK);
+                    if (GRADS && e.w == 0)
+                        lt_tma<CTAS, LT_BM, true>(st, map_a, &full[s], leader + s * 8, e.m0, kb * LT_BK);
+                    else
+                        lt_tma<CTAS, LT_BM, false>(st, map_a, &full[s], leader + s * 8, e.m0, kb * LT_BK);
+                    lt_tma<CTAS, BN / CTAS, B_MN>(st + M::A_BYTES, map_b, &full[s], leader + s * 8,
+                                                  e.n0 + rank * (BN / CTAS), kb * LT_BK);
                 }
             }
             // Every stage in use is released before the CTA may leave: all its copies have landed and
@@ -382,31 +402,31 @@ __global__ void __launch_bounds__(LT_TC_THREADS, 1)
         }
     } else if (warp == LT_EPI_WARPS + 1) {
         if (lane == 0 && rank == 0) {
-            constexpr uint32_t idesc = lt_idesc<T>(CTAS * LT_BM, BN, A_MN, B_MN);
             uint32_t it = 0, done = 0;
             bool ok = true;
             for (uint32_t i = unit; ok && i < items; i += units, done++) {
-                const uint32_t z = i / tiles, buf = done & 1, use = done >> 1;
+                const Item e = item(i);
+                const bool a_mn = GRADS && e.w == 0;
+                const uint32_t idesc = lt_idesc<T>(CTAS * LT_BM, BN, a_mn, B_MN), a_step = lt_step(a_mn), b_step = lt_step(B_MN);
+                const uint32_t buf = done & 1, use = done >> 1;
                 if (use > 0 && !mbar_wait(&acc_empty[buf], (use & 1) ^ 1, JC_DEV_TIMEOUT_MMA)) break;
                 tc_fence_after();
                 const uint32_t acc = tmem + buf * BN;
-                const uint32_t k0 = (uint32_t)((uint64_t)blocks * z / p.splits);
-                const uint32_t k1 = (uint32_t)((uint64_t)blocks * (z + 1) / p.splits);
-                for (uint32_t kb = k0; kb < k1; kb++, it++) {
+                for (uint32_t kb = e.k0; kb < e.k1; kb++, it++) {
                     const uint32_t s = it % STAGES;
                     if (!mbar_wait(&full[s], (it / STAGES) & 1, JC_DEV_TIMEOUT_FULL)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint64_t ad = lt_desc<A_MN>(smem_u32(base + s * M::STAGE));
-                    const uint64_t bd = lt_desc<B_MN>(smem_u32(base + s * M::STAGE + M::A_BYTES));
+                    const uint64_t ad = lt_desc(smem_u32(base + s * M::STAGE), a_mn);
+                    const uint64_t bd = lt_desc(smem_u32(base + s * M::STAGE + M::A_BYTES), B_MN);
 #pragma unroll
                     for (int kk = 0; kk < LT_BK / 16; kk++) {
                         if constexpr (CTAS == 2)
-                            tc_mma_f16_pair(acc, ad + kk * LT_STEP<A_MN>, bd + kk * LT_STEP<B_MN>, idesc, kb > k0 || kk > 0);
+                            tc_mma_f16_pair(acc, ad + kk * a_step, bd + kk * b_step, idesc, kb > e.k0 || kk > 0);
                         else
-                            tc_mma_f16(acc, ad + kk * LT_STEP<A_MN>, bd + kk * LT_STEP<B_MN>, idesc, kb > k0 || kk > 0);
+                            tc_mma_f16(acc, ad + kk * a_step, bd + kk * b_step, idesc, kb > e.k0 || kk > 0);
                     }
                     if constexpr (CTAS == 2)
                         tc_commit_pair(&empty[s]);
@@ -426,15 +446,16 @@ __global__ void __launch_bounds__(LT_TC_THREADS, 1)
         LtRes<S::CW> res;
         uint32_t done = 0;
         for (uint32_t i = unit; i < items; i += units, done++) {
-            const uint32_t t = i % tiles, n0 = t % p.tiles_n * BN, m0 = (t / p.tiles_n * CTAS + rank) * LT_BM;
+            const Item e = item(i);
+            const LinearTcParams &p = kp.p[e.w];
             // The first chunk's bias and residual are on their way while the accumulator is being summed.
-            bias.load(p.bias, n0 + (warp >> 2) * (BN / 2), p.n);
-            if (VEC && p.res)
-                res.load(static_cast<const uint8_t *>(p.res), p.ldres, m0 + 32 * (warp & 3),
-                         n0 + (warp >> 2) * (BN / 2), p.m, p.n);
+            if (!GRADS) bias.load(p.bias, e.n0 + (warp >> 2) * (BN / 2), p.n);
+            if (!GRADS && VEC && p.res)
+                res.load(static_cast<const uint8_t *>(p.res), p.ldres, e.m0 + 32 * (warp & 3),
+                         e.n0 + (warp >> 2) * (BN / 2), p.m, p.n);
             if (!mbar_wait_sleep(&acc_full[done & 1], (done >> 1) & 1, JC_DEV_TIMEOUT_MMA)) break;
             tc_fence_after();
-            lt_epilogue<T, BN, ACT, VEC>(p, tmem + (done & 1) * BN, buf, warp, m0, n0, i / tiles, bias, res);
+            lt_epilogue<T, BN, GRADS, ACT, VEC>(p, tmem + (done & 1) * BN, buf, warp, e.m0, e.n0, e.z, bias, res);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {

@@ -281,23 +281,33 @@ static bool out_vec(const Product &q) {
            (!q.res || aligned16(q.res, q.ldres, 2));
 }
 
-template <class T, int BN, int CTAS, bool A_MN, bool B_MN, uint32_t ACT, bool VEC>
-static bool launch_tc(const Product &q, LinearTcParams &p, cudaStream_t s) {
+// Runs the forward product (q[0]) or (GRADS) dw's and dx's, either of which may be without rows.
+template <class T, int BN, int CTAS, bool GRADS, uint32_t ACT, bool VEC>
+static bool launch_tc(const Product *q, cudaStream_t s) {
     static std::atomic<uint64_t> smem_set{0};
-    auto kern = linear_tc_kernel<T, BN, CTAS, A_MN, B_MN, ACT, VEC>;
-    LinearTcKernelParams kp;
-    kp.p = p;
-    kp.p.tiles_m = (q.m + CTAS * LT_BM - 1) / (CTAS * LT_BM);
-    kp.p.tiles_n = (q.n + BN - 1) / BN;
-    const uint64_t items = (uint64_t)kp.p.tiles_m * kp.p.tiles_n * p.splits;
-    if (items > 0x7FFFFFFFull) {
-        set_error("linear: too many tiles");
-        return false;
-    }
+    auto kern = linear_tc_kernel<T, BN, CTAS, GRADS, ACT, VEC>;
+    LinearTcKernelParams kp{};
+    kp.err = module_error_word();
     using Mem = LtTcSmem<BN, CTAS>;
-    if (!ensure_smem(kern, Mem::BYTES, smem_set) || !make_operand_map<T>(&kp.map_a, q.a, q.m, q.k, A_MN, LT_BM) ||
-        !make_operand_map<T>(&kp.map_b, q.b, q.n, q.k, B_MN, BN / CTAS))
-        return false;
+    if (!kp.err || !ensure_smem(kern, Mem::BYTES, smem_set)) return false;
+    uint64_t items = 0;
+    for (int w = 0; w < (GRADS ? 2 : 1); w++) {
+        const Product &r = q[w];
+        if (r.m == 0) continue;
+        const uint32_t tiles_m = (r.m + CTAS * LT_BM - 1) / (CTAS * LT_BM), tiles_n = (r.n + BN - 1) / BN;
+        const uint64_t mine = (uint64_t)tiles_m * tiles_n * r.splits;
+        items += mine;
+        if (items > 0x7FFFFFFFull) {
+            set_error("linear: too many tiles");
+            return false;
+        }
+        kp.items[w] = (uint32_t)mine;
+        kp.p[w] = LinearTcParams{r.m,     r.n, r.k,   r.bias, r.res, r.ldres,  r.c,     r.ldc,
+                                 r.z,     r.ldz, r.ws, r.splits, tiles_m, tiles_n};
+        if (!make_operand_map<T>(&kp.map_a[w], r.a, r.m, r.k, GRADS && w == 0, LT_BM) ||
+            !make_operand_map<T>(&kp.map_b[w], r.b, r.n, r.k, GRADS, BN / CTAS))
+            return false;
+    }
     if constexpr (CTAS == 1) {
         const uint32_t grid = (uint32_t)std::min<uint64_t>(items, (uint64_t)sm_count());
         return launch_ex(kern, dim3(grid), dim3(LT_TC_THREADS), Mem::BYTES, s, true, "linear", kp);
@@ -319,52 +329,35 @@ struct Tiling {
 };
 constexpr Tiling TILINGS[] = {{1, 64}, {1, 128}, {2, 128}, {2, 256}};
 
-// Microseconds a product takes with a tiling: the busiest unit's items, each a main loop of about 0.28
-// us per 64 contracted elements (one thread's MMAs complete in order at about 130 cycles each whatever
-// their width), plus the first loads and the last epilogue, which nothing hides.
-static double tc_us(uint32_t m, uint32_t n, uint32_t k, Tiling t, uint32_t splits, uint32_t sms) {
-    const uint64_t items = (uint64_t)((m + t.ctas * LT_BM - 1) / (t.ctas * LT_BM)) * ((n + t.bn - 1) / t.bn) * splits;
-    const uint32_t blocks = ((k + LT_BK - 1) / LT_BK + splits - 1) / splits, units = sms / t.ctas;
-    return (double)((items + units - 1) / units) * (0.28 * blocks + 0.5) + 2.0 + 0.008 * t.bn;
+// An item's microseconds: about 0.36 us per 64 contracted elements (one thread's MMAs complete in order at
+// about 130 cycles each whatever their width; the clock under load is what it is), and 0.5 us.
+struct Items {
+    uint64_t count = 0;
+    double us = 0.0;
+};
+static Items tc_items(uint32_t m, uint32_t n, uint32_t k, Tiling t, uint32_t splits) {
+    if (m == 0) return {};
+    const uint32_t rows = t.ctas * LT_BM, blocks = ((k + LT_BK - 1) / LT_BK + splits - 1) / splits;
+    return {(uint64_t)((m + rows - 1) / rows) * ((n + t.bn - 1) / t.bn) * splits, 0.36 * blocks + 0.5};
 }
 
-static Tiling pick_tiling(uint32_t m, uint32_t n, uint32_t k, uint32_t splits, uint32_t sms, double *us = nullptr) {
-    Tiling best = TILINGS[0];
-    double least = 1e30;
-    for (const Tiling &t : TILINGS) {
-        const double v = tc_us(m, n, k, t, splits, sms);
-        if (v > least) continue;
-        best = t;
-        least = v;
-    }
-    if (us) *us = least;
-    return best;
+// Microseconds of a launch of two kinds of items: whole rounds of each (dw's items spread over the units
+// beside dx's cost more than the sum of the work says: at 12288 x 768 x 2048 two splits, 48 items beside
+// dx's 144, take 138 us, three, 72 items for 74 pairs, 98), then the first loads and the last epilogue.
+static double tc_us(Items a, Items b, Tiling t, uint32_t sms) {
+    const uint32_t units = sms / t.ctas;
+    return (double)((a.count + units - 1) / units) * a.us + (double)((b.count + units - 1) / units) * b.us + 2.0 +
+           0.008 * t.bn;
 }
 
-// Runs a product: A_MN / B_MN say that the operand's contiguous axis is not the contracted one.
-template <class T, bool A_MN, bool B_MN, uint32_t ACT>
-static bool launch_product(const Product &q, cudaStream_t s) {
-    LinearTcParams p{};
-    p.m = q.m;
-    p.n = q.n;
-    p.k = q.k;
-    p.bias = q.bias;
-    p.res = q.res;
-    p.ldres = q.ldres;
-    p.c = q.c;
-    p.ldc = q.ldc;
-    p.z = q.z;
-    p.ldz = q.ldz;
-    p.ws = q.ws;
-    p.splits = q.splits;
-    p.err = module_error_word();
-    if (!p.err) return false;
-    const Tiling t = pick_tiling(q.m, q.n, q.k, q.splits, (uint32_t)sm_count());
-    const bool vec = out_vec(q);
+// Runs products with a tiling.
+template <class T, bool GRADS, uint32_t ACT>
+static bool launch_products(const Product *q, Tiling t, cudaStream_t s) {
+    bool vec = true;
+    for (int w = 0; w < (GRADS ? 2 : 1); w++) vec = vec && (q[w].m == 0 || out_vec(q[w]));
     auto run = [&](auto c, auto w) {
         constexpr int CTAS = decltype(c)::value, BN = decltype(w)::value;
-        return vec ? launch_tc<T, BN, CTAS, A_MN, B_MN, ACT, true>(q, p, s)
-                   : launch_tc<T, BN, CTAS, A_MN, B_MN, ACT, false>(q, p, s);
+        return vec ? launch_tc<T, BN, CTAS, GRADS, ACT, true>(q, s) : launch_tc<T, BN, CTAS, GRADS, ACT, false>(q, s);
     };
     if (t.ctas == 2) return t.bn == 256 ? run(Int<2>(), Int<256>()) : run(Int<2>(), Int<128>());
     return t.bn == 128 ? run(Int<1>(), Int<128>()) : run(Int<1>(), Int<64>());
@@ -427,9 +420,17 @@ bool launch_linear(const LinearArgs &a, cudaStream_t s) {
     q.ldc = a.ldy;
     q.z = a.z;
     q.ldz = a.ldz;
+    Tiling best = TILINGS[0];
+    double least = 1e30;
+    for (const Tiling &t : TILINGS) {
+        const double us = tc_us(tc_items(a.m, a.n, a.k, t, 1), {}, t, (uint32_t)sm_count());
+        if (us > least) continue;
+        best = t;
+        least = us;
+    }
     return with_half(a.type, [&](auto t) {
         return with_act(a.act, [&](auto act) {
-            return launch_product<decltype(t), false, false, decltype(act)::value>(q, s);
+            return launch_products<decltype(t), false, decltype(act)::value>(&q, best, s);
         });
     });
 }
@@ -446,6 +447,7 @@ struct LinearBwdPlan {
     uint32_t thin_blocks;  // n <= LTHIN_MAX: blocks along the rows, each with its sums; nothing else used
     size_t lddz, part_at, ws_at, bytes;
     Pad w, x;
+    Tiling tiling;
 };
 
 static LinearBwdPlan plan_linear_bwd(const void *x, size_t ldx, const void *w, size_t ldw, uint32_t m, uint32_t n,
@@ -456,7 +458,7 @@ static LinearBwdPlan plan_linear_bwd(const void *x, size_t ldx, const void *w, s
     p.lddz = (n + 7) / 8 * 8;
     p.part_at = up((size_t)m * p.lddz * 2);
     p.ws_at = p.part_at + up((size_t)p.dz_parts * n * 4);
-    // dw's contraction runs over the rows: split so that its few tiles still fill the SMs.
+    // dw's contraction runs over the rows: split so that its few tiles still fill the SMs, beside dx's.
     const uint32_t sms = 148, blocks = (m + LT_BK - 1) / LT_BK;
     p.splits = 1;
     if (n <= LTHIN_MAX) {
@@ -465,16 +467,18 @@ static LinearBwdPlan plan_linear_bwd(const void *x, size_t ldx, const void *w, s
         return p;
     }
     double best = 1e30;
-    for (uint32_t s : {1u, 2u, 3u, 4u, 5u, 6u, 8u, 12u, 16u, 24u, 32u}) {
-        if (s > std::max(1u, blocks)) break;
-        double us;
-        pick_tiling(n, k, m, s, sms, &us);
-        if (s > 1) us += 2.0 + 8e-6 * s * n * k / 3.0;  // the partial sums, written and read
-        if (us < best) {
-            best = us;
-            p.splits = s;
+    for (const Tiling &t : TILINGS)
+        for (uint32_t s : {1u, 2u, 3u, 4u, 5u, 6u, 8u, 12u, 16u, 24u, 32u}) {
+            if (s > std::max(1u, blocks)) break;
+            // By the shape alone: a gradient has the same bits whichever others are asked for.
+            double us = tc_us(tc_items(n, k, m, t, s), tc_items(m, k, n, t, 1), t, sms);
+            if (s > 1) us += 2.0 + 1.2e-6 * s * n * k;  // the partial sums, written and read
+            if (us <= best) {
+                best = us;
+                p.tiling = t;
+                p.splits = s;
+            }
         }
-    }
     p.bytes = p.ws_at + (p.splits > 1 ? up((size_t)p.splits * n * k * 4) : 0);
     p.w = plan_pad(w, ldw, n, k, p.bytes);
     p.x = plan_pad(x, ldx, m, k, p.bytes + p.w.bytes);
@@ -551,39 +555,35 @@ bool launch_linear_bwd(const LinearBwdArgs &a, cudaStream_t s) {
         const void *x = a.x, *w = a.w;
         size_t ldx = a.ldx, ldw = a.ldw;
         if (a.m > 0 && !launch_pads(ws, plan.w, &w, &ldw, a.n, a.k, plan.x, &x, &ldx, a.m, a.k, s)) return false;
-        if (a.dx && a.m > 0) {
-            Product q;
-            q.a = LinearOperand{dz, lddz, 1};
-            q.b = LinearOperand{w, 1, ldw};
-            q.m = a.m;
-            q.n = a.k;
-            q.k = a.n;
-            q.c = a.dx;
-            q.ldc = a.lddx;
-            if (!launch_product<T, false, true, 0>(q, s)) return false;
-        }
         LinearFinishParams f{};
-        if (a.dw) {
-            if (a.m > 0) {
-                Product q;
-                q.a = LinearOperand{dz, 1, lddz};
-                q.b = LinearOperand{x, 1, ldx};
-                q.m = a.n;
-                q.n = a.k;
-                q.k = a.m;
-                q.c = a.dw;
-                q.ldc = a.lddw;
-                q.splits = plan.splits;
-                if (plan.splits > 1) f.ws = q.ws = reinterpret_cast<float *>(ws + plan.ws_at);
-                if (!launch_product<T, true, true, 0>(q, s)) return false;
-            }
-            if (f.ws || a.m == 0) {
-                f.splits = a.m ? plan.splits : 0;
-                f.m = a.n;
-                f.n = a.k;
-                f.c = a.dw;
-                f.ldc = a.lddw;
-            }
+        Product q[2];  // dw, dx
+        if (a.dw && a.m > 0) {
+            q[0].a = LinearOperand{dz, 1, lddz};
+            q[0].b = LinearOperand{x, 1, ldx};
+            q[0].m = a.n;
+            q[0].n = a.k;
+            q[0].k = a.m;
+            q[0].c = a.dw;
+            q[0].ldc = a.lddw;
+            q[0].splits = plan.splits;
+            if (plan.splits > 1) f.ws = q[0].ws = reinterpret_cast<float *>(ws + plan.ws_at);
+        }
+        if (a.dx && a.m > 0) {
+            q[1].a = LinearOperand{dz, lddz, 1};
+            q[1].b = LinearOperand{w, 1, ldw};
+            q[1].m = a.m;
+            q[1].n = a.k;
+            q[1].k = a.n;
+            q[1].c = a.dx;
+            q[1].ldc = a.lddx;
+        }
+        if ((q[0].m || q[1].m) && !launch_products<T, true, 0>(q, plan.tiling, s)) return false;
+        if (a.dw && (f.ws || a.m == 0)) {
+            f.splits = a.m ? plan.splits : 0;
+            f.m = a.n;
+            f.n = a.k;
+            f.c = a.dw;
+            f.ldc = a.lddw;
         }
         const bool vec = f.n % 8 == 0 && aligned16(f.c, f.ldc, 2);
         const uint64_t threads = (uint64_t)f.m * (vec ? f.n / 8 : f.n);
