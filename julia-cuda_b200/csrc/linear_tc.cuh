@@ -93,12 +93,13 @@ __device__ __forceinline__ void lt_copy_out(const uint8_t *buf, uint8_t *g, size
     if constexpr (VEC) {
         constexpr int PER = CW * W / 16, STEP = 32 / PER;  // 16-byte chunks a row, rows a pass
         const uint32_t c = lane % PER;
+        const uint32_t left = c0 + c * (16 / W) < cols && r0 < rows ? rows - r0 : 0;  // rows this lane writes
+        uint8_t *d = g + ((size_t)(r0 + lane / PER) * ld + c0) * W + c * 16;
 #pragma unroll
-        for (int i = 0; i < 32 / STEP; i++) {
+        for (int i = 0; i < 32 / STEP; i++, d += (size_t)STEP * ld * W) {
             const uint32_t r = i * STEP + lane / PER;
             const uint4 v = *reinterpret_cast<const uint4 *>(buf + r * 128 + ((c ^ (r & 7)) << 4));
-            if (r0 + r < rows && c0 + c * (16 / W) < cols)
-                *reinterpret_cast<uint4 *>(g + ((size_t)(r0 + r) * ld + c0) * W + c * 16) = v;
+            if (r < left) *reinterpret_cast<uint4 *>(d) = v;
         }
     } else {
         for (uint32_t e = lane; e < 32u * CW; e += 32) {
@@ -115,31 +116,26 @@ __device__ __forceinline__ void lt_copy_out(const uint8_t *buf, uint8_t *g, size
     }
 }
 
-// The 16-byte chunks lt_copy_out would write, read instead: into registers, then into the buffer.
+// The 16-byte chunks lt_copy_out would write, brought into the buffer instead, asynchronously: the
+// residual waits there rather than in registers, which it made spill (lt_res_wait, then __syncwarp).
 template <int CW>
-struct LtRes {
-    static constexpr int PER = CW * 2 / 16, STEP = 32 / PER, N = 32 / STEP;
-    uint4 v[N];
-    __device__ __forceinline__ void load(const uint8_t *g, size_t ld, uint32_t r0, uint32_t c0, uint32_t rows,
-                                         uint32_t cols) {
-        const uint32_t lane = threadIdx.x & 31, c = lane % PER;
+__device__ __forceinline__ void lt_res_request(uint8_t *buf, const uint8_t *g, size_t ld, uint32_t r0, uint32_t c0,
+                                               uint32_t rows, uint32_t cols) {
+    constexpr int PER = CW * 2 / 16, STEP = 32 / PER;
+    const uint32_t lane = threadIdx.x & 31, c = lane % PER;
+    const uint32_t left = c0 + c * 8 < cols && r0 < rows ? rows - r0 : 0;
+    const uint8_t *s = g + ((size_t)(r0 + lane / PER) * ld + c0) * 2 + c * 16;
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const uint32_t r = i * STEP + lane / PER;
-            v[i] = make_uint4(0, 0, 0, 0);
-            if (r0 + r < rows && c0 + c * 8 < cols)
-                v[i] = *reinterpret_cast<const uint4 *>(g + ((size_t)(r0 + r) * ld + c0) * 2 + c * 16);
-        }
+    for (int i = 0; i < 32 / STEP; i++, s += (size_t)STEP * ld * 2) {
+        const uint32_t r = i * STEP + lane / PER;
+        if (r < left)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(buf + r * 128 + ((c ^ (r & 7)) << 4))),
+                         "l"(s)
+                         : "memory");
     }
-    __device__ __forceinline__ void stage(uint8_t *buf) const {
-        const uint32_t lane = threadIdx.x & 31, c = lane % PER;
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const uint32_t r = i * STEP + lane / PER;
-            *reinterpret_cast<uint4 *>(buf + r * 128 + ((c ^ (r & 7)) << 4)) = v[i];
-        }
-    }
-};
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void lt_res_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
 // Any alignment: element by element into the buffer.
 template <int CW>
@@ -154,31 +150,21 @@ __device__ __forceinline__ void lt_copy_in(uint8_t *buf, const uint8_t *g, size_
     }
 }
 
-// A chunk's bias: requested early, a lane or two columns each; added by way of the staging buffer (16
-// broadcast reads of 16 bytes). Read from global memory where it is used, each of those reads would
-// wait for the one before it: 3.4 us a tile.
+// A chunk's bias: requested early, a lane or two columns each, and passed round the warp. Read from global
+// memory where it is used, each of those reads would wait for the one before it: 3.4 us a tile.
 template <int CW>
 struct LtBias {
-    float v[CW > 32 ? 2 : 1];
+    float v[CW / 32];
     __device__ __forceinline__ void load(const float *bias, uint32_t c0, uint32_t n) {
 #pragma unroll
-        for (int i = 0; i < (CW > 32 ? 2 : 1); i++) {
+        for (int i = 0; i < CW / 32; i++) {
             const uint32_t c = c0 + 32 * i + (threadIdx.x & 31);
             v[i] = bias && c < n ? __ldg(bias + c) : 0.0f;
         }
     }
-    __device__ __forceinline__ void add(uint8_t *buf, float *acc) const {
-        float *s = reinterpret_cast<float *>(buf);
-        __syncwarp();
+    __device__ __forceinline__ void add(float *acc) const {
 #pragma unroll
-        for (int i = 0; i < (CW > 32 ? 2 : 1); i++) s[32 * i + (threadIdx.x & 31)] = v[i];
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < CW; j += 4) {
-            const float4 b = *reinterpret_cast<const float4 *>(s + j);
-            acc[j] += b.x; acc[j + 1] += b.y; acc[j + 2] += b.z; acc[j + 3] += b.w;
-        }
-        __syncwarp();
+        for (int j = 0; j < CW; j++) acc[j] += __shfl_sync(0xffffffffu, v[j / 32], j & 31);
     }
 };
 
@@ -212,13 +198,13 @@ __device__ __forceinline__ void lt_acc(uint32_t taddr, float *v) {
 }
 
 // One warp's share of a finished tile: rows 32 (warp % 4).. and half warp / 4 of the columns. `acc`:
-// the tile's accumulator; `bias`, `res`: the first chunk's, requested before the accumulator was ready
-// (the residual only with VEC).
+// the tile's accumulator; `bias`: the first chunk's. Its residual, too, was requested before the
+// accumulator was ready, into the buffer (VEC; where z does not go through the buffer first).
 // GRADS: partial sums or plain values, nothing added.
 template <class T, int BN, bool GRADS, uint32_t ACT, bool VEC>
 __device__ __forceinline__ void lt_epilogue(const LinearTcParams &p, uint32_t acc, uint8_t *buf, uint32_t warp,
                                             uint32_t m0, uint32_t n0, uint32_t split,
-                                            LtBias<LtShape<BN>::CW> &bias, LtRes<LtShape<BN>::CW> &res) {
+                                            LtBias<LtShape<BN>::CW> &bias) {
     using S = LtShape<BN>;
     constexpr int CW = S::CW;
     const uint32_t r0 = m0 + 32 * (warp & 3);
@@ -246,7 +232,7 @@ __device__ __forceinline__ void lt_epilogue(const LinearTcParams &p, uint32_t ac
             continue;
         }
         if (!GRADS && p.bias) {
-            bias.add(buf, v);
+            bias.add(v);
             if (ch + 1 < S::CHUNKS) bias.load(p.bias, c0 + CW, p.n);
         }
         if (!GRADS && p.z) {
@@ -254,28 +240,27 @@ __device__ __forceinline__ void lt_epilogue(const LinearTcParams &p, uint32_t ac
             lt_put_row<T, CW>(buf, v);
             __syncwarp();
             lt_copy_out<CW, 2, VEC>(buf, static_cast<uint8_t *>(p.z), p.ldz, r0, c0, p.m, p.n);
+            __syncwarp();
+            if (VEC && p.res) lt_res_request<CW>(buf, static_cast<const uint8_t *>(p.res), p.ldres, r0, c0, p.m, p.n);
         }
         if constexpr (ACT != 0) {
 #pragma unroll
             for (int j = 0; j < CW; j++) v[j] = act_fwd<ACT>(v[j]);
         }
         if (!GRADS && p.res) {
-            const uint8_t *g = static_cast<const uint8_t *>(p.res);
-            __syncwarp();
-            if constexpr (VEC) {
-                // This chunk's residual into the buffer, the next one's requested.
-                res.stage(buf);
-                if (ch + 1 < S::CHUNKS) res.load(g, p.ldres, r0, c0 + CW, p.m, p.n);
-            } else {
-                lt_copy_in<CW>(buf, g, p.ldres, r0, c0, p.m, p.n);
-            }
+            if constexpr (VEC)
+                lt_res_wait();
+            else
+                lt_copy_in<CW>(buf, static_cast<const uint8_t *>(p.res), p.ldres, r0, c0, p.m, p.n);
             __syncwarp();
             lt_add_row<T, CW>(buf, v);
         }
-        __syncwarp();
-        lt_put_row<T, CW>(buf, v);
+        lt_put_row<T, CW>(buf, v);  // a lane's own row: read above, if anything, by the lane itself
         __syncwarp();
         lt_copy_out<CW, 2, VEC>(buf, static_cast<uint8_t *>(p.c), p.ldc, r0, c0, p.m, p.n);
+        __syncwarp();
+        if (!GRADS && VEC && p.res && !p.z && ch + 1 < S::CHUNKS)
+            lt_res_request<CW>(buf, static_cast<const uint8_t *>(p.res), p.ldres, r0, c0 + CW, p.m, p.n);
     }
 }
 
@@ -443,19 +428,18 @@ __global__ void __launch_bounds__(LT_TC_THREADS, 1)
         uint8_t *buf = bufs + warp * LT_STAGE_BUF;
         const uint32_t leader = CTAS == 2 ? map_to_rank(smem_u32(acc_empty), 0) : 0;
         LtBias<S::CW> bias;
-        LtRes<S::CW> res;
         uint32_t done = 0;
         for (uint32_t i = unit; i < items; i += units, done++) {
             const Item e = item(i);
             const LinearTcParams &p = kp.p[e.w];
             // The first chunk's bias and residual are on their way while the accumulator is being summed.
             if (!GRADS) bias.load(p.bias, e.n0 + (warp >> 2) * (BN / 2), p.n);
-            if (!GRADS && VEC && p.res)
-                res.load(static_cast<const uint8_t *>(p.res), p.ldres, e.m0 + 32 * (warp & 3),
-                         e.n0 + (warp >> 2) * (BN / 2), p.m, p.n);
+            if (!GRADS && VEC && p.res && !p.z)
+                lt_res_request<S::CW>(buf, static_cast<const uint8_t *>(p.res), p.ldres, e.m0 + 32 * (warp & 3),
+                                      e.n0 + (warp >> 2) * (BN / 2), p.m, p.n);
             if (!mbar_wait_sleep(&acc_full[done & 1], (done >> 1) & 1, JC_DEV_TIMEOUT_MMA)) break;
             tc_fence_after();
-            lt_epilogue<T, BN, GRADS, ACT, VEC>(p, tmem + (done & 1) * BN, buf, warp, e.m0, e.n0, e.z, bias, res);
+            lt_epilogue<T, BN, GRADS, ACT, VEC>(p, tmem + (done & 1) * BN, buf, warp, e.m0, e.n0, e.z, bias);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
