@@ -122,7 +122,7 @@ bool launch_norm(const NormArgs &a, cudaStream_t s) {
                 int per_sm = 0;
                 if (!ensure_smem(kern, S::SMEM, set) || !blocks_per_sm(kern, S::THREADS, S::SMEM, resident, &per_sm))
                     return false;
-                const dim3 grid(norm_blocks(a.rows, S::GROUPS, l.period, (uint32_t)(sm_count() * per_sm)));
+                const dim3 grid(norm_blocks(a.rows, S::GROUPS * S::ROWS, l.period, (uint32_t)(sm_count() * per_sm)));
                 return launch_ex(kern, grid, dim3(S::THREADS), S::SMEM, s, true, "layer_norm", p);
             };
             static std::atomic<uint64_t> set_v{0}, set_1{0};
