@@ -148,13 +148,13 @@ struct DzParams {
     size_t lddy;
     const void *z;
     size_t ldz;
-    uint32_t m, n;
+    uint32_t m, n, rows;  // rows: of a block
     void *dz;  // [m][n], or nullptr
     size_t lddz;
     float *part;  // [gridDim.y][n] column sums, or nullptr
 };
 
-constexpr int DZ_ROWS = 64;  // rows a block covers
+constexpr uint32_t DZ_ROWS = 64;  // rows a block covers
 
 // dz = dy act'(z) and its sums over each block's rows: a thread walks V columns down every eighth
 // row, the block's eight warps meet in shared memory in order.
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const DzParams p) {
     for (int i = 0; i < V; i++) sum[i] = 0.0f;
     if (c < p.n)
 #pragma unroll 2
-        for (uint32_t r = blockIdx.y * DZ_ROWS + warp; r < min(p.m, (blockIdx.y + 1) * DZ_ROWS); r += 8) {
+        for (uint32_t r = blockIdx.y * p.rows + warp; r < min(p.m, (blockIdx.y + 1) * p.rows); r += 8) {
             float d[V];
             Elem<T, V>::load(static_cast<const T *>(p.dy) + r * p.lddy + c, d);
             if constexpr (ACT != 0) {

@@ -440,10 +440,37 @@ size_t linear_ws_bytes(const void *x, size_t ldx, const void *w, size_t ldw, uin
     return plan_pad(x, ldx, m, k, 0).bytes + plan_pad(w, ldw, n, k, 0).bytes;
 }
 
+// The tiling of both gradients' products and the splits of dw's contraction, which runs over the rows: its
+// few tiles are split so that they still fill the SMs. By the shape alone, so that a gradient has the same
+// bits whichever others are asked for. The last shape's plan is kept (weighing the choices takes 2 us).
+struct GradPlan {
+    uint32_t m = 0, n = 0, k = 0, splits = 1;
+    Tiling tiling{};
+};
+static GradPlan plan_grads(uint32_t m, uint32_t n, uint32_t k) {
+    static thread_local GradPlan p;
+    if (p.m == m && p.n == n && p.k == k && p.tiling.bn) return p;
+    p = GradPlan{m, n, k};
+    const uint32_t sms = 148, blocks = (m + LT_BK - 1) / LT_BK;
+    double best = 1e30;
+    for (const Tiling &t : TILINGS)
+        for (uint32_t s : {1u, 2u, 3u, 4u, 5u, 6u, 8u, 12u, 16u, 24u, 32u}) {
+            if (s > std::max(1u, blocks)) break;
+            double us = tc_us(tc_items(n, k, m, t, s), tc_items(m, k, n, t, 1), t, sms);
+            if (s > 1) us += 2.0 + 1.2e-6 * s * n * k;  // the partial sums, written and read
+            if (us <= best) {
+                best = us;
+                p.tiling = t;
+                p.splits = s;
+            }
+        }
+    return p;
+}
+
 // The backward pass's workspace: dz (16 bits, rows padded to 16 bytes), the column sums' parts, dw's
 // partial products, the copies of w and x where TMA cannot load them, each from a 256-byte boundary.
 struct LinearBwdPlan {
-    uint32_t dz_parts, splits;
+    uint32_t dz_rows, dz_parts, splits;
     uint32_t thin_blocks;  // n <= LTHIN_MAX: blocks along the rows, each with its sums; nothing else used
     size_t lddz, part_at, ws_at, bytes;
     Pad w, x;
@@ -454,31 +481,20 @@ static LinearBwdPlan plan_linear_bwd(const void *x, size_t ldx, const void *w, s
                                      uint32_t k) {
     LinearBwdPlan p{};
     auto up = [](size_t v) { return round_up(v, 256); };
-    p.dz_parts = (m + DZ_ROWS - 1) / DZ_ROWS;
+    // Rows a block of the dz kernel takes: few rows go to one, which then writes dbias itself.
+    p.dz_rows = m <= 2 * DZ_ROWS ? 2 * DZ_ROWS : DZ_ROWS;
+    p.dz_parts = (m + p.dz_rows - 1) / p.dz_rows;
     p.lddz = (n + 7) / 8 * 8;
     p.part_at = up((size_t)m * p.lddz * 2);
     p.ws_at = p.part_at + up((size_t)p.dz_parts * n * 4);
-    // dw's contraction runs over the rows: split so that its few tiles still fill the SMs, beside dx's.
-    const uint32_t sms = 148, blocks = (m + LT_BK - 1) / LT_BK;
-    p.splits = 1;
     if (n <= LTHIN_MAX) {
-        p.thin_blocks = std::max(1u, std::min((m + 31) / 32, sms * 2));
+        p.thin_blocks = std::max(1u, std::min((m + 31) / 32, 148u * 2));
         p.bytes = up((size_t)p.thin_blocks * ((size_t)n * k + n) * 4);
         return p;
     }
-    double best = 1e30;
-    for (const Tiling &t : TILINGS)
-        for (uint32_t s : {1u, 2u, 3u, 4u, 5u, 6u, 8u, 12u, 16u, 24u, 32u}) {
-            if (s > std::max(1u, blocks)) break;
-            // By the shape alone: a gradient has the same bits whichever others are asked for.
-            double us = tc_us(tc_items(n, k, m, t, s), tc_items(m, k, n, t, 1), t, sms);
-            if (s > 1) us += 2.0 + 1.2e-6 * s * n * k;  // the partial sums, written and read
-            if (us <= best) {
-                best = us;
-                p.tiling = t;
-                p.splits = s;
-            }
-        }
+    const GradPlan g = plan_grads(m, n, k);
+    p.tiling = g.tiling;
+    p.splits = g.splits;
     p.bytes = p.ws_at + (p.splits > 1 ? up((size_t)p.splits * n * k * 4) : 0);
     p.w = plan_pad(w, ldw, n, k, p.bytes);
     p.x = plan_pad(x, ldx, m, k, p.bytes + p.w.bytes);
@@ -533,7 +549,8 @@ bool launch_linear_bwd(const LinearBwdArgs &a, cudaStream_t s) {
         // dz is dy itself where there is no activation and TMA can load dy.
         const bool write = (a.dx || a.dw) && (a.act || !aligned16(a.dy, a.lddy, 2));
         if (a.m > 0 && (write || a.dbias)) {
-            const DzParams p{a.dy, a.lddy, a.z, a.ldz, a.m, a.n, write ? ws : nullptr, plan.lddz, a.dbias ? part : nullptr};
+            const DzParams p{a.dy, a.lddy, a.z, a.ldz, a.m, a.n, plan.dz_rows, write ? ws : nullptr, plan.lddz,
+                             a.dbias ? (plan.dz_parts == 1 ? a.dbias : part) : nullptr};
             if (write) {
                 dz = ws;
                 lddz = plan.lddz;
@@ -588,7 +605,7 @@ bool launch_linear_bwd(const LinearBwdArgs &a, cudaStream_t s) {
         const bool vec = f.n % 8 == 0 && aligned16(f.c, f.ldc, 2);
         const uint64_t threads = (uint64_t)f.m * (vec ? f.n / 8 : f.n);
         f.join_blocks = (uint32_t)std::min<uint64_t>((threads + 255) / 256, 148 * 16);
-        if (a.dbias) {
+        if (a.dbias && !(a.m > 0 && plan.dz_parts == 1)) {
             f.part = part;
             f.parts = a.m ? plan.dz_parts : 0;
             f.bias_n = a.n;
