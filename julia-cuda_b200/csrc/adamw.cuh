@@ -122,8 +122,7 @@ __device__ __forceinline__ void div2(float *x, const float *minus_s, const float
     fma2(x, r, inv, q);
 }
 
-// One thread's eight elements as they lie in memory.
-template <int BITS>
+// One thread's eight elements as they lie in memory, with 8-bit states.
 struct AdamwRaw {
     uint4 g[2], p[2];
     uint2 m, v;
@@ -135,7 +134,10 @@ struct AdamwRaw {
 // memory, while the current one's data is on its way: looked up when needed, the two dependent reads in
 // front of every chunk left the memory idle for a third of the time. With 8-bit states, whose elements
 // are half the bytes for more arithmetic, the next chunk's data is requested before the current one is
-// worked on too (485 -> 470 us for a model of 160 million; with 32-bit states the bus is full without).
+// worked on too (485 -> 470 us for 160 million elements; with 32-bit states the bus is full without).
+// Bound by memory: 160 million elements with bf16 gradients and copies, 32-bit states 701 us, 6.4 TB/s, as
+// fast as a copy; 8-bit states 505 us from three models in turn, 5.1 TB/s: a third of the issue slots is
+// taken, the rest waits for loads that 24 warps a SM keep too few of in flight.
 constexpr uint32_t ADAMW_WORDS = sizeof(AdamwTensor) / 4;
 
 template <int BITS>
@@ -157,8 +159,8 @@ __global__ void __launch_bounds__(ADAMW_THREADS, BITS == 8 ? 3 : 4) adamw_kernel
     look_up(blockIdx.x + g1, next, 1);
     const float gs = p.grad_scale ? *p.grad_scale : 1.0f;
     __syncthreads();
-    AdamwRaw<BITS> raw, coming;
-    auto request = [&](const AdamwTensor &t, uint32_t chunk, AdamwRaw<BITS> &r) {
+    AdamwRaw raw, coming;
+    auto request = [&](const AdamwTensor &t, uint32_t chunk, AdamwRaw &r) {
         const uint64_t at = (uint64_t)chunk * ADAMW_CHUNK + tid * 8;
         if (!t.aligned || at + 8 > t.n) return;
         const uint4 *g = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(t.g) + at * (t.grad_type == JC_F32 ? 4 : 2));

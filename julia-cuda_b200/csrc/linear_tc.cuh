@@ -17,6 +17,12 @@
 // than the 64 bytes a cycle it can take in. The two products of the backward pass, whose second operands
 // lie alike, are one launch (GRADS): dw's few long items first, dx's many short ones after them, so no SM
 // waits for the other product's last tiles and dw's partial sums go out under dx's main loop.
+//
+// Bound by the matrix rate: 12288 x 2048 x 768 bf16, inputs in L2, takes 27.7 us (1.40 PFLOP/s, 85% of the
+// measured burst rate; a library product of that shape 28.4), 30.2 with bias and residual; from memory
+// 38. Its 144 tiles are two rounds of 72 pairs; what is left is the clock under load, the first tiles'
+// loads and the last epilogue. Short contractions are bound by the epilogue: 12288 x 768 x 2048 with
+// GELU and z 65 us.
 #pragma once
 #include <type_traits>
 
