@@ -6,45 +6,35 @@ queued on the current stream (or `stream`). Also available from the package itse
 from __future__ import annotations
 
 import ctypes
+import importlib.util
+import os
 
 import torch
 
-from . import EPI_GELU, EPI_RELU, JuliaCudaError, _check, last_error, lib
+from . import HERE, JuliaCudaError, last_error, lib
 
 F16, BF16, F32 = 0, 1, 2
 _TYPES = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32}
-_ACTS = {"none": 0, "relu": EPI_RELU, "gelu": EPI_GELU}
 
 
-# A call's host time is most of a small operator's: these are the cheapest forms of what they ask.
-_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream
+def _load_binding():
+    """The compiled checks and calls (csrc/torch_binding.cpp)."""
+    path = os.path.join(HERE, "_binding.so")
+    if not os.path.exists(path):
+        raise JuliaCudaError(f"{path} is not built (run build() / make -C julia-cuda_b200)")
+    lib()
+    spec = importlib.util.spec_from_file_location("_binding", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    module.set_error(JuliaCudaError)
+    return module
+
+
+_b = _load_binding()
 
 
 def _fail(what: str):
     raise JuliaCudaError(what)
-
-
-def _stream(stream, dev: int):
-    if stream is None:
-        return _raw_stream(dev)
-    return getattr(stream, "cuda_stream", stream)
-
-
-def _matrix(op: str, name: str, t, rows: int, cols: int, dtype):
-    """(pointer, row stride) of a [rows, cols] device tensor with contiguous rows; (None, 0) of
-    None."""
-    if t is None:
-        return None, 0
-    if t.dtype is not dtype or t.shape != (rows, cols) or not t.is_cuda:
-        _fail(f"{op}: {name} must be a [{rows}, {cols}] device tensor of {dtype}, "
-              f"not {list(t.shape)} of {t.dtype}")
-    if t.is_contiguous():
-        return t.data_ptr(), cols
-    sr, sc = t.stride()
-    if (cols > 1 and sc != 1) or (rows > 1 and sr < cols):
-        _fail(f"{op}: {name} must have contiguous rows that do not overlap")
-    return t.data_ptr(), sr if rows > 1 else cols
 
 
 def _vector(op: str, name: str, t, n: int, dtype=torch.float32):
@@ -55,43 +45,11 @@ def _vector(op: str, name: str, t, n: int, dtype=torch.float32):
     return t.data_ptr()
 
 
-def _type(op: str, t, halves: bool = False):
-    """(element type, device) of x."""
-    code = _TYPES.get(t.dtype)
-    if code is None or t.dim() != 2 or (halves and code == F32):
-        _fail(f"{op}: x must be a matrix of float16{', ' if not halves else ' or '}bfloat16"
-              f"{'' if halves else ' or float32'}")
-    return code, _on_device(op, t)
-
-
-def _on_device(op: str, t) -> int:
-    dev = t.get_device()
-    if dev < 0 or dev != _device():
-        _fail(f"{op}: the tensors are not on the current device")
-    return dev
-
-
-def _scratch(n: int, dtype, like, stream):
-    """Scratch of the allocator's own, which must not reuse it before `stream` is done with it."""
-    ws = torch.empty(n, dtype=dtype, device=like.device)
-    if stream is not None:
-        ws.record_stream(stream if isinstance(stream, torch.cuda.Stream)
-                         else torch.cuda.ExternalStream(stream))
-    return ws
-
-
 def layer_norm(x, gamma, beta, y, stats=None, eps: float = 1e-5, stream=None) -> None:
     """y = (x - mean) rstd gamma + beta per row (jc_layer_norm). x, y [rows, d] of one type (f16, bf16
     or f32), gamma and beta [d] f32 (beta may be None); stats, if given, [rows, 2] f32 receives mean
     and rstd for the backward pass."""
-    t, dev = _type("layer_norm", x)
-    rows, d = x.shape
-    xp, ldx = _matrix("layer_norm", "x", x, rows, d, x.dtype)
-    yp, ldy = _matrix("layer_norm", "y", y, rows, d, x.dtype)
-    _check(lib().jc_layer_norm(t, xp, ldx, _vector("layer_norm", "gamma", gamma, d),
-                               _vector("layer_norm", "beta", beta, d), eps, rows, d, yp, ldy,
-                               _vector("layer_norm", "stats", stats, 2 * rows), _stream(stream, dev)),
-           "jc_layer_norm")
+    _b.layer_norm(x, gamma, beta, y, stats, eps, stream)
 
 
 def layer_norm_backward(dy, x, gamma, stats, dx, dgamma=None, dbeta=None, add=None, ws=None,
@@ -99,31 +57,7 @@ def layer_norm_backward(dy, x, gamma, stats, dx, dgamma=None, dbeta=None, add=No
     """The gradients of layer_norm (jc_layer_norm_backward): dx (plus `add`, the gradient that
     reaches x past the norm), dgamma and dbeta [d] f32. ws: jc_layer_norm_ws_floats(rows, d) floats
     (allocated here when not given)."""
-    op = "layer_norm_backward"
-    t, dev = _type(op, x)
-    rows, d = x.shape
-    xp, ldx = _matrix(op, "x", x, rows, d, x.dtype)
-    dyp, lddy = _matrix(op, "dy", dy, rows, d, x.dtype)
-    dxp, lddx = _matrix(op, "dx", dx, rows, d, x.dtype)
-    ap, ldadd = _matrix(op, "add", add, rows, d, x.dtype)
-    need = lib().jc_layer_norm_ws_floats(rows, d) if dgamma is not None or dbeta is not None else 0
-    if need and ws is None:
-        ws = _scratch(need, torch.float32, x, stream)
-    elif need and ws.numel() < need:
-        _fail(f"{op}: ws needs {need} floats")
-    _check(lib().jc_layer_norm_backward(t, dyp, lddy, xp, ldx, _vector(op, "gamma", gamma, d),
-                                        _vector(op, "stats", stats, 2 * rows), ap, ldadd, rows, d,
-                                        dxp, lddx, _vector(op, "dgamma", dgamma, d),
-                                        _vector(op, "dbeta", dbeta, d),
-                                        ws.data_ptr() if need else None,
-                                        _stream(stream, dev)), "jc_layer_norm_backward")
-
-
-def _act(op: str, act: str) -> int:
-    code = _ACTS.get(act)
-    if code is None:
-        _fail(f"{op}: act must be one of {', '.join(_ACTS)}")
-    return code
+    _b.layer_norm_backward(dy, x, gamma, stats, dx, dgamma, dbeta, add, ws, stream)
 
 
 def linear(x, w, y, *, bias=None, act: str = "none", res=None, z=None, ws=None, stream=None) -> None:
@@ -131,25 +65,7 @@ def linear(x, w, y, *, bias=None, act: str = "none", res=None, z=None, ws=None, 
     bias [n] f32. z, if given, keeps the values before the activation for the backward pass. ws:
     jc_linear_ws_bytes(...) bytes, needed where rows of x or w start off 16-byte boundaries (allocated
     here when not given)."""
-    t, dev = _type("linear", x, halves=True)
-    m, k = x.shape
-    n = w.shape[0]
-    xp, ldx = _matrix("linear", "x", x, m, k, x.dtype)
-    wp, ldw = _matrix("linear", "w", w, n, k, x.dtype)
-    rp, ldres = _matrix("linear", "res", res, m, n, x.dtype)
-    yp, ldy = _matrix("linear", "y", y, m, n, x.dtype)
-    zp, ldz = _matrix("linear", "z", z, m, n, x.dtype)
-    wsp = None
-    if (xp | wp | 2 * ldx | 2 * ldw) % 16:
-        need = lib().jc_linear_ws_bytes(xp, ldx, wp, ldw, m, n, k)
-        if need and ws is None:
-            ws = _scratch(need, torch.uint8, x, stream)
-        elif need and ws.numel() * ws.element_size() < need:
-            _fail(f"linear: ws needs {need} bytes")
-        wsp = ws.data_ptr() if need else None
-    _check(lib().jc_linear(t, _act("linear", act), xp, ldx, wp, ldw,
-                           _vector("linear", "bias", bias, n), rp, ldres, yp, ldy, zp, ldz, m, n, k,
-                           wsp, _stream(stream, dev)), "jc_linear")
+    _b.linear(x, w, y, bias, act, res, z, ws, stream)
 
 
 def linear_backward(dy, x, w, *, z=None, act: str = "none", dx=None, dw=None, dbias=None, ws=None,
@@ -157,40 +73,14 @@ def linear_backward(dy, x, w, *, z=None, act: str = "none", dx=None, dw=None, db
     """The gradients of linear (jc_linear_backward), each written if its tensor is given: dx [m, k],
     dw [n, k] of x's type, dbias [n] f32. z (linear's) is read unless act is "none". ws:
     jc_linear_backward_ws_bytes(...) bytes (allocated here when not given)."""
-    op = "linear_backward"
-    t, dev = _type(op, x, halves=True)
-    m, k = x.shape
-    n = w.shape[0]
-    a = _act(op, act)
-    xp, ldx = _matrix(op, "x", x, m, k, x.dtype)
-    wp, ldw = _matrix(op, "w", w, n, k, x.dtype)
-    dyp, lddy = _matrix(op, "dy", dy, m, n, x.dtype)
-    zp, ldz = _matrix(op, "z", z, m, n, x.dtype)
-    dxp, lddx = _matrix(op, "dx", dx, m, k, x.dtype)
-    dwp, lddw = _matrix(op, "dw", dw, n, k, x.dtype)
-    need = lib().jc_linear_backward_ws_bytes(xp, ldx, wp, ldw, m, n, k)
-    if need and ws is None:
-        ws = _scratch(need, torch.uint8, x, stream)
-    elif need and ws.numel() * ws.element_size() < need:
-        _fail(f"{op}: ws needs {need} bytes")
-    _check(lib().jc_linear_backward(t, a, dyp, lddy, xp, ldx, wp, ldw, zp, ldz, m, n, k, dxp, lddx,
-                                    dwp, lddw, _vector(op, "dbias", dbias, n), ws.data_ptr() if need else None,
-                                    _stream(stream, dev)), "jc_linear_backward")
+    _b.linear_backward(dy, x, w, z, act, dx, dw, dbias, ws, stream)
 
 
 def choice_loss(logits, offsets, gold, loss, dlogits=None, weight=None, stream=None) -> None:
     """Each request's loss over its own markers and its gradient (jc_choice_loss): logits f32,
     offsets int32 [requests + 1], gold int32 [requests] (the right marker of each request, below 0:
     none), weight f32 [requests]; writes loss [requests] and dlogits (as logits)."""
-    op = "choice_loss"
-    n, r = logits.numel(), gold.numel()
-    dev = _on_device(op, logits)
-    _check(lib().jc_choice_loss(_vector(op, "logits", logits, n), n,
-                                _vector(op, "offsets", offsets, r + 1, torch.int32),
-                                _vector(op, "gold", gold, r, torch.int32),
-                                _vector(op, "weight", weight, r), r, _vector(op, "loss", loss, r),
-                                _vector(op, "dlogits", dlogits, n), _stream(stream, dev)),
-           "jc_choice_loss")
+    _b.choice_loss(logits, offsets, gold, loss, dlogits, weight, stream)
 
 
 class AdamwTensor(ctypes.Structure):
@@ -217,7 +107,7 @@ class AdamW:
     def __init__(self, params, grads, *, bits: int = 32, weight_decay=0.0, copies=None, exp_avg=None,
                  exp_avg_sq=None, exp_avg_scale=None, exp_avg_sq_scale=None):
         self._h = None
-        self._dev = _device()
+        self._dev = torch.cuda.current_device()
         n = len(params)
         if bits not in (8, 32):
             _fail("AdamW: states of 32 or 8 bits")
@@ -242,7 +132,8 @@ class AdamW:
         table = (AdamwTensor * max(n, 1))()
         for i, p in enumerate(self.params):
             k, g, c, at = p.numel(), self.grads[i], self.copies[i], f"of tensor {i}"
-            _on_device("AdamW", p)
+            if p.get_device() != self._dev:
+                _fail("AdamW: the tensors are not on the current device")
             if g.dtype not in _TYPES:
                 _fail(f"AdamW: the gradient {at} must be float16, bfloat16 or float32")
             if c is not None and c.dtype not in (torch.float16, torch.bfloat16):
@@ -265,10 +156,9 @@ class AdamW:
     def step(self, t: int, *, lr: float, betas=(0.9, 0.999), eps: float = 1e-8, grad_scale=None,
              stream=None) -> None:
         """Step t (from 1). grad_scale: one f32 on the device that every gradient is multiplied by."""
-        _check(lib().jc_adamw_step(self._h, t, lr, betas[0], betas[1], eps,
-                                   _vector("AdamW", "grad_scale", grad_scale, 1),
-                                   _stream(stream, self._dev)),
-               "jc_adamw_step")
+        if not self._h:
+            _fail("AdamW: closed")
+        _b.adamw_step(self._h, self._dev, t, lr, betas[0], betas[1], eps, grad_scale, stream)
 
     def close(self) -> None:
         if self._h:
