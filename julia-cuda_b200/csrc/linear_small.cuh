@@ -1,8 +1,8 @@
 // The linear layer where one dimension is tiny: nothing fills a 128-row tensor tile, and the time is
 // that of one trip to memory.
 //
-//   linear_rows_kernel      up to 16 rows (a request's markers): the weights are read once, straight
-//                           into mma.sync fragments
+//   linear_rows_kernel      few rows (a request's markers): the weights are read once for each 16 of
+//                           them, straight into mma.sync fragments
 //   linear_thin_kernel,     up to 8 output columns (a scorer's last layer): x is read once; forward a
 //   linear_thin_bwd_kernel  dot product a row, backward one pass for dx, dw and dbias
 #pragma once

@@ -372,9 +372,26 @@ static bool with_thin(uint32_t n, F &&f) {
     return f(Int<8>());
 }
 
-// Up to this many rows the weights are read straight into mma.sync fragments (a 16-row block each);
-// beyond it the tensor tiles of 128 rows are faster.
-constexpr uint32_t LINEAR_ROWS = 16;
+static Tiling forward_tiling(uint32_t m, uint32_t n, uint32_t k, double *us) {
+    Tiling best = TILINGS[0];
+    *us = 1e30;
+    for (const Tiling &t : TILINGS) {
+        const double v = tc_us(tc_items(m, n, k, t, 1), {}, t, (uint32_t)sm_count());
+        if (v > *us) continue;
+        best = t;
+        *us = v;
+    }
+    return best;
+}
+
+// Whether few rows go to linear_rows_kernel, which reads the weights once for 16 of them: 1.8 us and 0.55
+// for a million products of 16 rows (384 x 768: 1.9 us at 16 rows, 3.4 at 128; 2304 x 768: 5.3 at 64, 8.7
+// at 128), where the tensor tiles of 128 rows take what tc_us says less a fifth when they are few (384 x
+// 768 5.6 to 5.9 us, 2304 x 768 5.8 to 6.0, 768 x 2048 11.2 to 11.5 against 5.9 and 8.1 at 64 and 128).
+static bool few_rows(uint32_t m, uint32_t n, uint32_t k, double tc) {
+    const uint32_t groups = (m + 15) / 16;
+    return groups <= 65535 && 1.8 + 0.55e-6 * groups * (double)n * k < 0.8 * tc;
+}
 
 bool launch_linear(const LinearArgs &a, cudaStream_t s) {
     if (a.m == 0) return true;
@@ -393,7 +410,9 @@ bool launch_linear(const LinearArgs &a, cudaStream_t s) {
                 });
             });
         });
-    if (a.m <= LINEAR_ROWS)
+    double tc = 0.0;
+    const Tiling tiling = forward_tiling(a.m, a.n, a.k, &tc);
+    if (few_rows(a.m, a.n, a.k, tc))
         return with_half(a.type, [&](auto t) {
             return with_act(a.act, [&](auto act) {
                 using T = decltype(t);
@@ -420,24 +439,19 @@ bool launch_linear(const LinearArgs &a, cudaStream_t s) {
     q.ldc = a.ldy;
     q.z = a.z;
     q.ldz = a.ldz;
-    Tiling best = TILINGS[0];
-    double least = 1e30;
-    for (const Tiling &t : TILINGS) {
-        const double us = tc_us(tc_items(a.m, a.n, a.k, t, 1), {}, t, (uint32_t)sm_count());
-        if (us > least) continue;
-        best = t;
-        least = us;
-    }
     return with_half(a.type, [&](auto t) {
         return with_act(a.act, [&](auto act) {
-            return launch_products<decltype(t), false, decltype(act)::value>(&q, best, s);
+            return launch_products<decltype(t), false, decltype(act)::value>(&q, tiling, s);
         });
     });
 }
 
 size_t linear_ws_bytes(const void *x, size_t ldx, const void *w, size_t ldw, uint32_t m, uint32_t n, uint32_t k) {
-    if (n <= LTHIN_MAX || m <= LINEAR_ROWS) return 0;
-    return plan_pad(x, ldx, m, k, 0).bytes + plan_pad(w, ldw, n, k, 0).bytes;
+    const size_t bytes = plan_pad(x, ldx, m, k, 0).bytes + plan_pad(w, ldw, n, k, 0).bytes;
+    if (bytes == 0 || n <= LTHIN_MAX) return 0;
+    double tc = 0.0;
+    forward_tiling(m, n, k, &tc);
+    return few_rows(m, n, k, tc) ? 0 : bytes;
 }
 
 // The tiling of both gradients' products and the splits of dw's contraction, which runs over the rows: its

@@ -51,8 +51,8 @@ def test_linear_refusals(jc, buf):
                     (dict(n=0), "must not be 0"), (dict(k=0), "must not be 0"), (dict(x=None), "x is null"),
                     (dict(w=None), "w is null"), (dict(y=None), "y is null"), (dict(ldw=7), "w's rows"),
                     (dict(res=p, ldres=2), "res's rows"), (dict(z=p + 1), "z is not aligned"),
-                    (dict(bias=p + 2), "bias"), (dict(m=20, n=9, k=7, ldx=9, ldy=9), "ws is null"),
-                    (dict(m=20, n=9, k=7, ldx=9, ldy=9, ws=p + 8), "ws is misaligned")):
+                    (dict(bias=p + 2), "bias"), (dict(m=9000, n=600, k=700, ldx=701, ldw=700, ldy=600), "ws is null"),
+                    (dict(m=9000, n=600, k=700, ldx=701, ldw=700, ldy=600, ws=p + 8), "ws is misaligned")):
         assert fwd(**kw) == -1 and why in jc.last_error(), (kw, jc.last_error())
     assert fwd(m=0, x=None, y=None) == 0
 
@@ -68,9 +68,10 @@ def test_linear_refusals(jc, buf):
     assert size(p, 768, p, 768, 10, 0, 5) == 0
     assert L.jc_linear_ws_bytes(p, 768, p, 768, 4096, 2048, 768) == 0
     # A copy of x, of w, or of both, their rows on 16-byte boundaries.
-    assert L.jc_linear_ws_bytes(p, 769, p, 768, 100, 64, 768) == 100 * 768 * 2
-    assert L.jc_linear_ws_bytes(p, 768, p + 2, 768, 100, 64, 768) == 64 * 768 * 2
-    assert L.jc_linear_ws_bytes(p, 767, p, 767, 100, 64, 767) == 164 * 768 * 2
+    m, n = 9000, 600
+    assert L.jc_linear_ws_bytes(p, 769, p, 768, m, n, 768) == m * 768 * 2
+    assert L.jc_linear_ws_bytes(p, 768, p + 2, 768, m, n, 768) == n * 768 * 2
+    assert L.jc_linear_ws_bytes(p, 767, p, 767, m, n, 767) == (m + n) * 768 * 2
 
 
 def test_choice_loss_refusals(jc, buf):

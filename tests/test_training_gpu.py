@@ -255,7 +255,7 @@ def dact64(z, act):
 SHAPES = [(1, 1, 1), (1, 384, 768), (12, 384, 768), (3, 1, 384), (129, 1, 96), (64, 64, 64),
           (128, 256, 64), (127, 136, 72), (130, 257, 65), (293, 768, 768), (300, 2048, 768),
           (513, 768, 2048), (257, 100, 50), (1000, 7, 1001), (33, 1001, 8), (700, 384, 1536),
-          (5, 2304, 768), (2100, 264, 200)]
+          (5, 2304, 768), (2100, 264, 200), (901, 999, 1001), (1300, 777, 770), (640, 1001, 1000), (1500, 1000, 333)]
 
 
 @pytest.mark.parametrize("t", HALVES)
