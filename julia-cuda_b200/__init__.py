@@ -3,7 +3,8 @@
 A thin ctypes layer over libjulia_cuda.so (include/julia_cuda.h), mirroring the reference's own
 FFI surface: the engine calls of src/capi.rs (julia_cuda_load / run / free / device / tier) and the
 kernel-level launches of src/gemm.rs, src/attn.rs and src/lib.rs. torch tensors are used only for
-device memory and streams. There is no CPU fallback: importing this package on a machine without
+device memory and streams (the fine-tuning operators, which are many short calls, go through a compiled
+binding instead: training.py). There is no CPU fallback: importing this package on a machine without
 the built library raises, and every kernel call fails loudly if its launch fails.
 
 The directory name is not an identifier; import it with importlib.import_module("julia-cuda_b200").

@@ -64,7 +64,7 @@ constexpr int LR_WARPS = 8, LR_AHEAD = 4;
 // their sums meet in shared memory, in order. The contraction's order is free, so a lane loads the 16
 // bytes (8 elements) that make its fragments of two MMAs: lane 4 g + q holds elements 8 q .. 8 q + 7 of
 // column g of w, and of rows g and g + 8 of x, and takes them in pairs as the MMA's k places 2 q, 2 q + 8.
-// Bound by latency: 12 x 768 x 384 4.9 us from cold caches, where a tensor tile took 7.6.
+// Bound by latency: 12 x 768 x 384 takes 1.9 us, 4.9 from cold caches, where a tensor tile takes 5.6.
 template <class T, uint32_t ACT, bool VEC>
 __global__ void __launch_bounds__(32 * LR_WARPS) linear_rows_kernel(const LinearRowsParams p) {
     __shared__ float sums[LR_WARPS][128];
@@ -197,8 +197,8 @@ struct LinearThinBwdParams {
 
 // blockIdx.y: 256 of the k columns, eight a lane; blockIdx.x: rows, a warp every gridDim.x * 8th. The
 // sums for dw stay in registers, the block's warps add theirs up in shared memory in order. dz stays
-// f32 here: nothing multiplies it on the tensor cores. 1531 x 384 x 1 with the kernel after it: 15 us a
-// call, the launches; by tensor tiles 25.
+// f32 here: nothing multiplies it on the tensor cores. 1531 x 384 x 1 with the kernel after it: 6.6 us a
+// call, two launches; by tensor tiles, whose launches were four, 10 us more.
 template <class T, int N, bool VEC, uint32_t ACT>
 __global__ void __launch_bounds__(256) linear_thin_bwd_kernel(const LinearThinBwdParams p) {
     __shared__ float s[8][257];
