@@ -21,6 +21,9 @@ struct LossParams {
     unsigned int *err;
 };
 
+// exp(x), x at most 0: what would be subnormal is 0 (its handling is half of the function).
+__device__ __forceinline__ float exp_below(float x) { return ex2_approx(x * 1.44269504f); }
+
 // Request r's span and right marker, checked: false (recorded) if they are out of range.
 __device__ __forceinline__ bool loss_request(const LossParams &p, uint32_t r, uint32_t &a, uint32_t &b, int32_t &gold,
                                              float &w) {
@@ -89,15 +92,15 @@ __device__ __forceinline__ void loss_group(const LossParams &p, uint32_t r, uint
     if (top == -INFINITY) top = 0.0f;
     float sum = 0.0f;
 #pragma unroll
-    for (int k = 0; k < LOSS_KEEP; k++) sum += __expf(v[k] - top);
-    for (uint32_t i = LOSS_KEEP * G + t; i < b - a; i += G) sum += __expf(p.logits[a + i] - top);
+    for (int k = 0; k < LOSS_KEEP; k++) sum += exp_below(v[k] - top);
+    for (uint32_t i = LOSS_KEEP * G + t; i < b - a; i += G) sum += exp_below(p.logits[a + i] - top);
     sum = loss_sum<G>(sum, part);
     const bool counts = gold >= 0 && w != 0.0f && sum != 0.0f;
     if (t == 0) p.loss[r] = counts ? w * (top + logf(sum) - right) : 0.0f;
     if (!p.dlogits) return;
     const float inv = 1.0f / sum;
     auto grad = [&](uint32_t i, float l) {
-        p.dlogits[a + i] = counts ? w * (__expf(l - top) * inv - (i == (uint32_t)gold ? 1.0f : 0.0f)) : 0.0f;
+        p.dlogits[a + i] = counts ? w * (exp_below(l - top) * inv - (i == (uint32_t)gold ? 1.0f : 0.0f)) : 0.0f;
     };
 #pragma unroll
     for (int k = 0; k < LOSS_KEEP; k++)
@@ -182,11 +185,11 @@ __global__ void __launch_bounds__(32 * LOSS_WARPS, 8) loss_short_kernel(const Lo
                 if (i < longest)
 #pragma unroll
                     for (int j = i; j < i + 4; j++) {
-                        v[j] = __expf(v[j] - top);
+                        v[j] = exp_below(v[j] - top);
                         sum += v[j];
                     }
         } else {
-            for (uint32_t i = 0; i < len; i++) sum += __expf(l[i] - top);
+            for (uint32_t i = 0; i < len; i++) sum += exp_below(l[i] - top);
         }
         const bool counts = q.gold >= 0 && q.w != 0.0f && sum != 0.0f;
         if (t < n) p.loss[r0 + t] = counts ? q.w * (top + logf(sum) - right) : 0.0f;
@@ -200,7 +203,7 @@ __global__ void __launch_bounds__(32 * LOSS_WARPS, 8) loss_short_kernel(const Lo
                     for (int j = i; j < i + 4; j++)
                         if (j < len) out[j] = counts ? v[j] * f : 0.0f;
         } else {
-            for (uint32_t i = 0; i < len; i++) out[i] = counts ? __expf(l[i] - top) * f : 0.0f;
+            for (uint32_t i = 0; i < len; i++) out[i] = counts ? exp_below(l[i] - top) * f : 0.0f;
         }
         if (counts) out[q.gold] -= q.w;
         __syncwarp();
