@@ -473,7 +473,7 @@ JcAdamW *jc_adamw_create(const jc_adamw_tensor *tensors, size_t count, uint32_t 
  * p = p (1 - lr weight_decay) - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps), all in
  * f32. grad_scale: one f32 in device memory (NULL: 1), so a clipping factor need not visit the host.
  * 8-bit states are read, updated in f32, and rounded to the nearest e4m3 under their 256 elements'
- * new scale (largest magnitude / 448); a v above 0 stays above 0. */
+ * new scale (largest magnitude / 448); a v above 0 keeps a code above 0. */
 int jc_adamw_step(JcAdamW *opt, uint64_t t, float lr, double beta1, double beta2, float eps,
                   const float *grad_scale, void *stream);
 void jc_adamw_free(JcAdamW *opt);

@@ -6,8 +6,8 @@
 //
 // p, and m and v with 32-bit states, are f32. With 8-bit states m and v are e4m3 codes with one f32
 // scale for each 256 consecutive elements (the largest magnitude / 448), taken up and written back
-// each step around the same f32 arithmetic; a v above 0 never rounds to 0, so no step divides by
-// eps alone. v itself is held, not its root: nearest rounding then follows the 32-bit average with
+// each step around the same f32 arithmetic; a v above 0 never takes the code 0, so no step divides by
+// eps alone while f32 holds the block's v at all. v itself is held, not its root: nearest rounding then follows the 32-bit average with
 // no bias (its root within 0.85..1.25 of it for 90% of elements at beta2 0.999, 256 elements of
 // log-normal scale sharing a block; a root in e4m3: 0.78..1.34).
 #pragma once
@@ -111,10 +111,21 @@ __device__ __forceinline__ float div_fast(float a, float b) {
 }
 constexpr float ROOT_MIN = 1.0842022e-19f;  // the root of the smallest normal f32
 
-// x / s for a pair, given -s and inv = 1 / s rounded to nearest: the product's remainder, exact in one
-// fused multiply-add, corrects it (Markstein, "Computation of elementary functions on the IBM RISC
-// System/6000 processor", 1990). The correctly rounded quotient wherever that remainder does not
-// underflow, at a fifth of a division's instructions; below that a code is 0 either way.
+// Brings a block's scale s below 2^-64, and the values x that it will divide, up by 2^64, which rounds
+// nothing and leaves the quotients as they are. A scale fades with its block's gradients (the first
+// moment's to below 2^-128 in some 700 steps without any), and the reciprocal of such a one is infinite.
+__device__ __forceinline__ void lift8(float *x, float &s) {
+    if (s >= 0x1p-64f) return;  // alike in the whole warp
+    s *= 0x1p64f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] *= 0x1p64f;
+}
+
+// x / s for a pair, s at least 2^-85 (lift8), given -s and inv = 1 / s rounded to nearest: the product's
+// remainder, exact in one fused multiply-add, corrects it (Markstein, "Computation of elementary functions
+// on the IBM RISC System/6000 processor", 1990). The correctly rounded quotient wherever that remainder
+// does not underflow, at a fifth of a division's instructions. It underflows only for an x below 2^-95,
+// a thousandth of the scale, whose code is 0 either way.
 __device__ __forceinline__ void div2(float *x, const float *minus_s, const float *inv) {
     float q[2], r[2];
     mul2(q, x, inv);
@@ -260,7 +271,9 @@ __global__ void __launch_bounds__(ADAMW_THREADS, BITS == 8 ? 3 : 4) adamw_kernel
                 }
                 mm = __fmul_rn(warp_max_positive(mm), 1.0f / FP8_MAX);
                 vm = __fmul_rn(warp_max_positive(vm), 1.0f / FP8_MAX);
-                const float sm = mm > 0.0f ? mm : 1.0f, sv = vm > 0.0f ? vm : 1.0f;
+                float sm = mm > 0.0f ? mm : 1.0f, sv = vm > 0.0f ? vm : 1.0f;
+                lift8(m, sm);
+                lift8(v, sv);
                 const float im = __frcp_rn(sm), iv = __frcp_rn(sv);
                 const float nsm[2] = {-sm, -sm}, nsv[2] = {-sv, -sv}, im2[2] = {im, im}, iv2[2] = {iv, iv};
 #pragma unroll

@@ -1,0 +1,54 @@
+"""The fine-tuning operators where their ranges end: states that fade away, logits far from 0, empty
+batches, scratch of other streams, very many rows."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def normal(g, *shape, std=1.0, mean=0.0, dtype=torch.float32):
+    return (torch.randn(*shape, generator=g, device="cuda") * std + mean).to(dtype)
+
+
+def test_adamw_8bit_blocks_that_lose_their_gradients(jc):
+    """Three steps with gradients and 1300 without: the moments shrink with their blocks' scales, through
+    the subnormal numbers. Nothing becomes NaN, and codes and scales stay those of the formula's
+    operations rounded one by one in f32 (torch's own), bit for bit."""
+    g = gen(41)
+    n, size = 4, 3 * 256 + 100
+    pad = n * 256 - size
+    p, grad = normal(g, size, std=0.02), normal(g, size, std=1e-3)
+    grad[256:512:3] = 0                              # elements that never had a gradient
+    grad[512:768] *= 10.0 ** torch.linspace(-6, 0, 256, device="cuda")
+    before = p.clone()
+    opt = jc.AdamW([p], [grad], bits=8)
+    m = v = torch.zeros(n, 256, device="cuda")
+    lowest = math.inf
+    for t in range(1, 1304):
+        if t == 4:
+            grad.zero_()
+        opt.step(t, lr=1e-4, betas=(0.9, 0.9))
+        gf = torch.nn.functional.pad(grad, (0, pad)).view(n, 256)
+        m = (m * 0.9) + (gf * (1 - 0.9))
+        v = (v * 0.9) + (gf * (1 - 0.9)) * gf
+        out = []
+        for x, floor in ((m, False), (v, True)):
+            sc = x.abs().amax(1) * torch.tensor(1.0 / 448.0, dtype=torch.float32, device="cuda")
+            y = x / torch.where(sc > 0, sc, 1.0)[:, None]
+            y = torch.where(x > 0, y.clamp_min(2.0 ** -9), y) if floor else y
+            out.append((y.clamp(-448, 448).to(torch.float8_e4m3fn), sc))
+        (mc, ms), (vc, vs) = out
+        assert torch.equal(opt.exp_avg_scale[0], ms) and torch.equal(opt.exp_avg_sq_scale[0], vs), t
+        assert torch.equal(opt.exp_avg[0].view(torch.uint8), mc.view(-1)[:size].view(torch.uint8)), t
+        assert torch.equal(opt.exp_avg_sq[0].view(torch.uint8), vc.view(-1)[:size].view(torch.uint8)), t
+        m, v = mc.float() * ms[:, None], vc.float() * vs[:, None]
+        lowest = min(lowest, float(ms.max()))
+    assert lowest < 1e-43                            # the scales did go through the subnormals
+    # Three steps of lr at most each way, then a tail of beta1's powers: 1 / (1 - 0.9) more of them.
+    assert p.isfinite().all() and float((p - before).abs().max()) < 1e-4 * (3 + 10) * 10
