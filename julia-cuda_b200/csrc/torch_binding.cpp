@@ -8,8 +8,8 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
-#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -124,8 +124,8 @@ Queue queue_of(PyObject *o, int dev) {
     return {p, false};
 }
 
-// Scratch of `bytes`: the caller's `ws`, or torch's, which must not hand it out again before a stream that
-// is not the current one is done with it.
+// Scratch of `bytes`: the caller's `ws`, or torch's, from the pool of the stream that will use it: a block
+// of another stream's pool may still be in use by what that stream has queued.
 void *scratch(const Name &n, PyObject *ws, size_t bytes, const at::Tensor &like, const Queue &q, int dev, at::Tensor *keep) {
     if (bytes == 0) return nullptr;
     if (const at::Tensor *t = tensor(n, ws, false)) {
@@ -133,11 +133,10 @@ void *scratch(const Name &n, PyObject *ws, size_t bytes, const at::Tensor &like,
             fail(n.str() + " needs " + std::to_string(bytes) + " contiguous bytes on the current device");
         return t->data_ptr();
     }
-    *keep = at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+    c10::cuda::OptionalCUDAStreamGuard on;
     if (!q.current)
-        c10::cuda::CUDACachingAllocator::recordStream(
-            keep->storage().data_ptr(),
-            c10::cuda::getStreamFromExternal(static_cast<cudaStream_t>(q.handle), (c10::DeviceIndex)dev));
+        on.reset_stream(c10::cuda::getStreamFromExternal(static_cast<cudaStream_t>(q.handle), (c10::DeviceIndex)dev));
+    *keep = at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
     return keep->data_ptr();
 }
 

@@ -52,3 +52,49 @@ def test_adamw_8bit_blocks_that_lose_their_gradients(jc):
     assert lowest < 1e-43                            # the scales did go through the subnormals
     # Three steps of lr at most each way, then a tail of beta1's powers: 1 / (1 - 0.9) more of them.
     assert p.isfinite().all() and float((p - before).abs().max()) < 1e-4 * (3 + 10) * 10
+
+
+def test_scratch_comes_from_the_pool_of_the_stream_that_uses_it(jc):
+    """Backward calls queued on two streams side by side, none waiting for the other, have scratch of their
+    own: the bits of calls one after the other."""
+    g = gen(12)
+    m, n, k, t = 4096, 768, 512, torch.float16
+    x, w = normal(g, m, k + 1, dtype=t)[:, 1:], normal(g, n, k, std=0.05, dtype=t)  # x: copied into scratch
+    gamma, xd = torch.ones(k, device="cuda"), normal(g, m, k, dtype=t)
+    stats = torch.empty(m, 2, device="cuda")
+    y = torch.empty_like(xd)
+    jc.layer_norm(xd, gamma, None, y, stats=stats)
+
+    def calls(dy, dn, stream):
+        out = dict(dx=torch.empty(m, k, dtype=t, device="cuda"), dw=torch.empty_like(w),
+                   dbias=torch.empty(n, device="cuda"))
+        norm = torch.empty_like(xd), torch.empty_like(gamma), torch.empty_like(gamma)
+        forward = torch.empty(m, n, dtype=t, device="cuda")
+        yield (*out.values(), *norm, forward)
+        jc.linear_backward(dy, x, w, z=dy, act="relu", stream=stream, **out)
+        jc.layer_norm_backward(dn, xd, gamma, stats, *norm, stream=stream)
+        jc.linear(x, w, forward, stream=stream)
+        yield None
+    data = [(normal(g, m, n, dtype=t), normal(g, m, k, dtype=t)) for _ in range(2)]
+    want = []
+    for dy, dn in data:
+        c = calls(dy, dn, None)
+        outs = next(c)
+        next(c)
+        torch.cuda.synchronize()
+        want.append([o.clone() for o in outs])
+    torch.cuda.empty_cache()
+    side = torch.cuda.Stream()
+    of_side = lambda: sum(s["total_size"] for s in torch.cuda.memory_snapshot() if s["stream"] == side.cuda_stream)  # noqa: E731
+    assert of_side() == 0
+    for stream in (side, side.cuda_stream):
+        cs = [calls(*data[i % 2], stream if i % 2 else None) for i in range(12)]
+        outs = [next(c) for c in cs]
+        torch.cuda.synchronize()     # the outputs' storage is free on every stream
+        for c in cs:
+            next(c)
+        torch.cuda.synchronize()
+        for i, got in enumerate(outs):
+            assert all(torch.equal(a, b) for a, b in zip(got, want[i % 2])), i
+    assert of_side() >= m * n * 2    # dz at least
+    assert jc.device_error() == 0
