@@ -306,7 +306,10 @@ JcAdamW *jc_adamw_create(const jc_adamw_tensor *tensors, size_t count, uint32_t 
             if (!jc::cuda_ok(cudaMalloc(&opt->tensors, tb), "adamw: cudaMalloc") ||
                 !jc::cuda_ok(cudaMalloc(&opt->chunks, cb), "adamw: cudaMalloc") ||
                 !jc::cuda_ok(cudaMemcpy(opt->tensors, table.data(), tb, cudaMemcpyHostToDevice), "adamw: table") ||
-                !jc::cuda_ok(cudaMemcpy(opt->chunks, chunks.data(), cb, cudaMemcpyHostToDevice), "adamw: table"))
+                !jc::cuda_ok(cudaMemcpy(opt->chunks, chunks.data(), cb, cudaMemcpyHostToDevice), "adamw: table") ||
+                // A copy from pageable memory may return before its data has arrived, and a step's stream
+                // need not be ordered behind it.
+                !jc::cuda_ok(cudaStreamSynchronize(nullptr), "adamw: table"))
                 return nullptr;
         }
         return opt.release();

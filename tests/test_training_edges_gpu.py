@@ -98,3 +98,19 @@ def test_scratch_comes_from_the_pool_of_the_stream_that_uses_it(jc):
             assert all(torch.equal(a, b) for a, b in zip(got, want[i % 2])), i
     assert of_side() >= m * n * 2    # dz at least
     assert jc.device_error() == 0
+
+
+def test_adamw_first_step_on_a_stream_of_its_own(jc):
+    """The table of a few thousand tensors is on the device when AdamW returns: a step at once, on a stream
+    that is ordered behind no other, moves every parameter."""
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        base = torch.zeros(6000 * 300, device="cuda")
+        p, grad = list(base.view(6000, 300)), list(torch.ones_like(base).view(6000, 300))
+        m, v = (list(torch.zeros_like(base).view(6000, 300)) for _ in range(2))
+        torch.cuda.synchronize()
+        opt = jc.AdamW(p, grad, exp_avg=m, exp_avg_sq=v)
+        opt.step(1, lr=0.5, stream=side)
+        side.synchronize()
+        assert (base + 0.5).abs().max() < 1e-6
+        opt.close()
