@@ -148,7 +148,8 @@ class AdamW:
                 _vector("AdamW", f"exp_avg_sq_scale {at}", self.exp_avg_sq_scale[i], sc),
                 None if c is None else _vector("AdamW", f"the copy {at}", c, k, c.dtype), k,
                 float(decay[i]), _TYPES[g.dtype], F32 if c is None else _TYPES[c.dtype])
-        # The table's copy waits for nothing: zeros made above are queued before any step.
+        # The zeros made above are there before a step on whatever stream.
+        torch.cuda.current_stream().synchronize()
         self._h = lib().jc_adamw_create(table, n, bits)
         if not self._h:
             raise JuliaCudaError(last_error())

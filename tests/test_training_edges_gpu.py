@@ -114,3 +114,15 @@ def test_adamw_first_step_on_a_stream_of_its_own(jc):
         side.synchronize()
         assert (base + 0.5).abs().max() < 1e-6
         opt.close()
+
+
+def test_adamw_states_are_zero_before_any_step(jc):
+    """The states made by AdamW are there when it returns, for steps on any stream."""
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        p = torch.ones(1000, device="cuda")
+        side.synchronize()
+        torch.cuda._sleep(int(2e8))   # about 0.1 s
+        opt = jc.AdamW([p], [torch.ones_like(p)], bits=8)
+        assert side.query()
+    opt.close()
