@@ -37,11 +37,12 @@ def _fail(what: str):
     raise JuliaCudaError(what)
 
 
-def _vector(op: str, name: str, t, n: int, dtype=torch.float32):
+def _vector(op: str, name: str, t, n: int, dev: int, dtype=torch.float32):
     if t is None:
         return None
-    if t.dtype is not dtype or t.numel() != n or not t.is_cuda or not t.is_contiguous():
-        _fail(f"{op}: {name} must be a contiguous device tensor of {n} elements of {dtype}")
+    if (t.dtype is not dtype or t.numel() != n or not t.is_cuda or t.get_device() != dev
+            or not t.is_contiguous()):
+        _fail(f"{op}: {name} must be a contiguous tensor on the current device of {n} elements of {dtype}")
     return t.data_ptr()
 
 
@@ -107,7 +108,7 @@ class AdamW:
     def __init__(self, params, grads, *, bits: int = 32, weight_decay=0.0, copies=None, exp_avg=None,
                  exp_avg_sq=None, exp_avg_scale=None, exp_avg_sq_scale=None):
         self._h = None
-        self._dev = torch.cuda.current_device()
+        self._dev = dev = torch.cuda.current_device()
         n = len(params)
         if bits not in (8, 32):
             _fail("AdamW: states of 32 or 8 bits")
@@ -140,13 +141,13 @@ class AdamW:
                 _fail(f"AdamW: the copy {at} must be float16 or bfloat16")
             sc = blocks[i] if scaled else 0
             table[i] = AdamwTensor(
-                _vector("AdamW", f"the parameter {at}", p, k),
-                _vector("AdamW", f"the gradient {at}", g, k, g.dtype),
-                _vector("AdamW", f"exp_avg {at}", self.exp_avg[i], k, state),
-                _vector("AdamW", f"exp_avg_sq {at}", self.exp_avg_sq[i], k, state),
-                _vector("AdamW", f"exp_avg_scale {at}", self.exp_avg_scale[i], sc),
-                _vector("AdamW", f"exp_avg_sq_scale {at}", self.exp_avg_sq_scale[i], sc),
-                None if c is None else _vector("AdamW", f"the copy {at}", c, k, c.dtype), k,
+                _vector("AdamW", f"the parameter {at}", p, k, dev),
+                _vector("AdamW", f"the gradient {at}", g, k, dev, g.dtype),
+                _vector("AdamW", f"exp_avg {at}", self.exp_avg[i], k, dev, state),
+                _vector("AdamW", f"exp_avg_sq {at}", self.exp_avg_sq[i], k, dev, state),
+                _vector("AdamW", f"exp_avg_scale {at}", self.exp_avg_scale[i], sc, dev),
+                _vector("AdamW", f"exp_avg_sq_scale {at}", self.exp_avg_sq_scale[i], sc, dev),
+                None if c is None else _vector("AdamW", f"the copy {at}", c, k, dev, c.dtype), k,
                 float(decay[i]), _TYPES[g.dtype], F32 if c is None else _TYPES[c.dtype])
         # The zeros made above are there before a step on whatever stream.
         torch.cuda.current_stream().synchronize()
