@@ -1,7 +1,8 @@
 // The loss of requests that each choose one of their own markers, and its gradient.
 //
 //   request r: logits l[a..b), a = offsets[r], b = offsets[r + 1], the right one gold[r] (< 0: none)
-//   loss[r] = w[r] (log(sum(exp(l))) - l[a + gold[r]])
+//   loss[r] = w[r] (log(sum(exp(l - top))) + (top - l[a + gold[r]])), top = max(l): from differences
+//             alone, or logits far from 0 would round away a confident request's small loss
 //   dlogits[i] = w[r] (exp(l[i]) / sum(exp(l)) - (i == a + gold[r]))
 //
 // A request without an answer, with weight 0, without logits, or with only logits of -infinity
@@ -96,7 +97,7 @@ __device__ __forceinline__ void loss_group(const LossParams &p, uint32_t r, uint
     for (uint32_t i = LOSS_KEEP * G + t; i < b - a; i += G) sum += exp_below(p.logits[a + i] - top);
     sum = loss_sum<G>(sum, part);
     const bool counts = gold >= 0 && w != 0.0f && sum != 0.0f;
-    if (t == 0) p.loss[r] = counts ? w * (top + logf(sum) - right) : 0.0f;
+    if (t == 0) p.loss[r] = counts ? w * (logf(sum) + (top - right)) : 0.0f;
     if (!p.dlogits) return;
     const float inv = 1.0f / sum;
     auto grad = [&](uint32_t i, float l) {
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(32 * LOSS_WARPS, 8) loss_short_kernel(const Lo
             for (uint32_t i = 0; i < len; i++) sum += exp_below(l[i] - top);
         }
         const bool counts = q.gold >= 0 && q.w != 0.0f && sum != 0.0f;
-        if (t < n) p.loss[r0 + t] = counts ? q.w * (top + logf(sum) - right) : 0.0f;
+        if (t < n) p.loss[r0 + t] = counts ? q.w * (logf(sum) + (top - right)) : 0.0f;
         if (!p.dlogits) continue;
         const float f = q.w / sum;
         if (regs) {

@@ -126,3 +126,27 @@ def test_adamw_states_are_zero_before_any_step(jc):
         opt = jc.AdamW([p], [torch.ones_like(p)], bits=8)
         assert side.query()
     opt.close()
+
+
+@pytest.mark.parametrize("lo,hi", [(2, 8), (17, 24), (60, 120), (700, 900)])
+@pytest.mark.parametrize("offset", [0.0, 1000.0, -1000.0, 30000.0])
+def test_choice_loss_far_from_zero(jc, lo, hi, offset):
+    """The loss depends on the logits' differences alone: logits far from 0 cost it nothing. Half of the
+    requests are confident (the right logit leads by about 8). Bound: differences from the largest logit
+    are rounded once, their exponentials off by |x| 2^-23 and 2^-22 of themselves (x e^-x is 0.37 at most)
+    and the sum by its longest chain, 25: 64 x 2^-24 of 1 + the loss in all, whatever the offset."""
+    g = gen(lo)
+    requests = 200
+    n = torch.randint(lo, hi + 1, (requests,), generator=g, device="cuda")
+    off = torch.zeros(requests + 1, dtype=torch.int32, device="cuda")
+    off[1:] = n.cumsum(0)
+    gold = (torch.rand(requests, generator=g, device="cuda") * n).to(torch.int32)
+    gold = torch.minimum(gold, n.to(torch.int32) - 1)
+    lg = normal(g, int(off[-1]))
+    lg[(off[:-1] + gold).long()[::2]] += 8 + math.log(hi)
+    lg += offset
+    loss, dl = torch.full((requests,), math.nan, device="cuda"), torch.full_like(lg, math.nan)
+    jc.choice_loss(lg, off, gold, loss, dlogits=dl)
+    rows = lg.double().split(n.tolist())
+    want = torch.stack([torch.log(torch.exp(l - l.max()).sum()) + (l.max() - l[w]) for l, w in zip(rows, gold.tolist())])
+    assert ((loss.double() - want).abs() <= 64 * 2.0 ** -24 * (1 + want)).all()
