@@ -523,7 +523,8 @@ size_t linear_bwd_ws_bytes(const void *x, size_t ldx, const void *w, size_t ldw,
 static bool launch_linear_thin_bwd(const LinearBwdArgs &a, uint32_t blocks, cudaStream_t s) {
     return with_half(a.type, [&](auto t) {
         using T = decltype(t);
-        float *part = a.dw || a.dbias ? static_cast<float *>(a.ws) : nullptr;
+        const bool sums = a.dw || a.dbias;
+        float *part = sums ? static_cast<float *>(a.ws) : nullptr;  // without rows there may be none
         if (a.m > 0) {
             const LinearThinBwdParams p{a.dy, a.lddy, a.x, a.ldx, a.w, a.ldw, a.z, a.ldz, a.m, a.n, a.k,
                                         a.dx, a.lddx, part, a.dw != nullptr};
@@ -544,7 +545,7 @@ static bool launch_linear_thin_bwd(const LinearBwdArgs &a, uint32_t blocks, cuda
                 }))
                 return false;
         }
-        if (!part) return true;
+        if (!sums) return true;
         return launch_ex(linear_thin_finish_kernel<T>, dim3((a.n * a.k + a.n + 31) / 32), dim3(1024), 0, s, true,
                          "linear_backward", (const float *)part, a.m ? blocks : 0u, a.n, a.k, static_cast<T *>(a.dw),
                          a.lddw, a.dbias);

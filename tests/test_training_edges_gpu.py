@@ -150,3 +150,21 @@ def test_choice_loss_far_from_zero(jc, lo, hi, offset):
     rows = lg.double().split(n.tolist())
     want = torch.stack([torch.log(torch.exp(l - l.max()).sum()) + (l.max() - l[w]) for l, w in zip(rows, gold.tolist())])
     assert ((loss.double() - want).abs() <= 64 * 2.0 ** -24 * (1 + want)).all()
+
+
+@pytest.mark.parametrize("n", [1, 3, 8, 9])
+def test_linear_backward_of_no_rows_without_scratch(jc, n):
+    """No rows: the gradients of the parameters are 0, and no scratch is asked for."""
+    L, k = jc.lib(), 40
+    w, dw = torch.ones(n, k, device="cuda", dtype=torch.float16), torch.full((n, k), math.nan, device="cuda", dtype=torch.float16)
+    db = torch.full((n,), math.nan, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    args = (0, 0, None, n, None, k, w.data_ptr(), k, None, n, 0, n, k, None, k)
+    assert L.jc_linear_backward(*args, dw.data_ptr(), k, db.data_ptr(), None, stream) == 0, jc.last_error()
+    assert (dw == 0).all() and (db == 0).all()
+    dw.fill_(math.nan)
+    assert L.jc_linear_backward(*args, dw.data_ptr(), k, None, None, stream) == 0, jc.last_error()
+    assert (dw == 0).all()
+    db.fill_(math.nan)
+    assert L.jc_linear_backward(*args, None, k, db.data_ptr(), None, stream) == 0, jc.last_error()
+    assert (db == 0).all()
