@@ -237,8 +237,9 @@ __global__ void __launch_bounds__(NormShape<T, V, G, E>::THREADS, NormShape<T, V
 #pragma unroll
                 for (int q = 0; q < R; q++) {
                     const uint64_t r = at(i + q);
-                    if (r < p.rows && !copied(r))
-                        for (uint32_t j = row.t; j < p.d; j += G) stage[q * G * E + row.shift + j] = x[r * p.ldx + j];
+                    if (r >= p.rows || copied(r)) continue;
+                    for (uint32_t j = row.t; j < p.d; j += G) stage[q * G * E + row.shift + j] = x[r * p.ldx + j];
+                    fence_proxy_async();  // these stores come before the bulk copy that takes the stage next
                 }
             }
             if (G == 32)
@@ -425,6 +426,7 @@ __global__ void __launch_bounds__(NormBwdShape<T, V, G, E>::THREADS, 1) norm_bwd
                     stage[ELEMS + row.shift + j] = dy[r * p.lddy + j];
                     if (p.add) stage[2 * ELEMS + row.shift + j] = add[r * p.ldadd + j];
                 }
+                fence_proxy_async();  // these stores come before the bulk copies that take the stage next
             }
             if (G == 32)
                 __syncwarp();

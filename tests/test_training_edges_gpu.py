@@ -168,3 +168,30 @@ def test_linear_backward_of_no_rows_without_scratch(jc, n):
     db.fill_(math.nan)
     assert L.jc_linear_backward(*args, None, k, db.data_ptr(), None, stream) == 0, jc.last_error()
     assert (db == 0).all()
+
+
+@pytest.mark.parametrize("d,t", [(771, torch.float16), (1001, torch.bfloat16), (2051, torch.float16), (509, torch.float32)])
+def test_layer_norm_rows_after_the_tensors_first(jc, d, t):
+    """Rows off 16-byte boundaries, many for each block: the first and last rows are copied by the threads,
+    and the bulk copies that follow take their place. Every row is within u of 64 bits, and f32's error
+    of sums (400 x 2^-24 of the magnitudes)."""
+    g = gen(d)
+    rows = 30011
+    x, dy, add = (normal(g, rows, d, dtype=t) for _ in range(3))
+    gamma, y, stats = torch.ones(d, device="cuda"), torch.full_like(x, math.nan), torch.empty(rows, 2, device="cuda")
+    dx, dg, db = torch.full_like(x, math.nan), torch.empty_like(gamma), torch.empty_like(gamma)
+    jc.layer_norm(x, gamma, None, y, stats=stats)
+    jc.layer_norm_backward(dy, x, gamma, stats, dx, dg, db, add=add)
+    assert jc.device_error() == 0
+    u, f32 = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}[t], 400 * 2.0 ** -24
+    x, dy, add = x.double(), dy.double(), add.double()
+    mean = x.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt((x - mean).square().mean(1, keepdim=True) + 1e-5)
+    xh = (x - mean) * rstd
+    mag = (x.abs() + x.abs().mean(1, keepdim=True)) * rstd
+    assert ((y.double() - xh).abs() <= u * xh.abs() + f32 * mag + 2.0 ** -25).all()
+    want = rstd * (dy - dy.mean(1, keepdim=True) - xh * (dy * xh).mean(1, keepdim=True)) + add
+    tol = f32 * (rstd * (dy.abs() + 1 + mag * (1 + (dy * xh).abs().mean(1, keepdim=True))) + add.abs())
+    assert ((dx.double() - want).abs() <= u * want.abs() + 2 * tol + 2.0 ** -25).all()
+    assert ((dg.double() - (dy * xh).sum(0)).abs() <= f32 * (dy.abs() * mag).sum(0)).all()
+    assert ((db.double() - dy.sum(0)).abs() <= f32 * dy.abs().sum(0)).all()
