@@ -402,9 +402,10 @@ int jc_device_error(uint32_t *code);
 #define JC_BF16 1u
 #define JC_F32 2u
 
-/* y = (x - mean) rstd gamma + beta for each of `rows` rows of d elements (d up to 16384; x, y of
- * `type`, gamma and beta [d] f32, beta may be NULL), rstd = 1 / sqrt(variance + eps). stats (may be
- * NULL) receives [rows][2] f32: mean and rstd, which the backward pass reads. y may be x. */
+/* y = (x - mean) rstd gamma + beta for each of `rows` rows (up to 2^31 - 1) of d elements (d up to
+ * 16384; x, y of `type`, gamma and beta [d] f32, beta may be NULL), rstd = 1 / sqrt(variance + eps).
+ * stats (may be NULL) receives [rows][2] f32: mean and rstd, which the backward pass reads. y may be
+ * x. */
 int jc_layer_norm(uint32_t type, const void *x, size_t ldx, const float *gamma, const float *beta,
                   float eps, uint32_t rows, uint32_t d, void *y, size_t ldy, float *stats,
                   void *stream);
@@ -422,9 +423,9 @@ size_t jc_layer_norm_ws_floats(uint32_t rows, uint32_t d);
 /* z = x w^T + bias, y = act(z) + res: x [m][k], w [n][k], y, z, res [m][n] of `type` (JC_F16 or
  * JC_BF16), bias [n] f32; bias, res and z may be NULL. act: 0, JC_EPI_RELU or JC_EPI_GELU. z, when
  * given, keeps the values before the activation, which the backward pass reads. Unlike jc_gemm, any
- * m, n and k, both 16-bit types, strided rows. y may be res. ws: jc_linear_ws_bytes(x, ldx, w, ldw, m,
- * n, k) bytes of scratch, 256-byte aligned: 0 (ws may be NULL) where the rows of x and w start on
- * 16-byte boundaries; others are copied there first. */
+ * m, n and k up to 2^31 - 1, both 16-bit types, strided rows. y may be res. ws: jc_linear_ws_bytes(x,
+ * ldx, w, ldw, m, n, k) bytes of scratch, 256-byte aligned: 0 (ws may be NULL) where the rows of x and w
+ * start on 16-byte boundaries; others are copied there first. */
 int jc_linear(uint32_t type, uint32_t act, const void *x, size_t ldx, const void *w, size_t ldw,
               const float *bias, const void *res, size_t ldres, void *y, size_t ldy, void *z,
               size_t ldz, uint32_t m, uint32_t n, uint32_t k, void *ws, void *stream);

@@ -52,11 +52,26 @@ bool check_act(const char *op, uint32_t type, uint32_t act) {
     return false;
 }
 
-bool check_norm(const char *op, uint32_t type, uint32_t d) {
+// Kernels count rows in 32 bits and step past the last one, and TMA's coordinates are signed.
+constexpr uint32_t MAX_SIZE = 0x7FFFFFFFu;
+
+bool check_norm(const char *op, uint32_t type, uint32_t rows, uint32_t d) {
     if (type > JC_F32)
         jc::set_error(std::string(op) + ": unknown element type");
+    else if (rows > MAX_SIZE)
+        jc::set_error(std::string(op) + ": at most 2^31 - 1 rows");
     else if (d == 0 || d > 16384)
         jc::set_error(std::string(op) + ": rows of 1 to 16384 elements");
+    else
+        return true;
+    return false;
+}
+
+bool check_sizes(const char *op, uint32_t m, uint32_t n, uint32_t k) {
+    if (n == 0 || k == 0)
+        jc::set_error(std::string(op) + ": n and k must not be 0");
+    else if (m > MAX_SIZE || n > MAX_SIZE || k > MAX_SIZE)
+        jc::set_error(std::string(op) + ": m, n and k are at most 2^31 - 1");
     else
         return true;
     return false;
@@ -82,7 +97,7 @@ int jc_layer_norm(uint32_t type, const void *x, size_t ldx, const float *gamma, 
     return guarded(nullptr, 0, [&]() -> int {
         const char *op = "layer_norm";
         const bool any = rows > 0;
-        if (!check_norm(op, type, d)) return -1;
+        if (!check_norm(op, type, rows, d)) return -1;
         if (!(eps >= 0.0f) || std::isinf(eps)) return fail("layer_norm: eps must be finite and not negative");
         const size_t size = type_size(type);
         if (!check_matrix(op, "x", x, ldx, d, size, any) || !check_matrix(op, "y", y, ldy, d, size, any) ||
@@ -114,7 +129,7 @@ int jc_layer_norm_backward(uint32_t type, const void *dy, size_t lddy, const voi
     return guarded(nullptr, 0, [&]() -> int {
         const char *op = "layer_norm_backward";
         const bool any = rows > 0;
-        if (!check_norm(op, type, d)) return -1;
+        if (!check_norm(op, type, rows, d)) return -1;
         const size_t size = type_size(type);
         if (!check_matrix(op, "dy", dy, lddy, d, size, any) || !check_matrix(op, "x", x, ldx, d, size, any) ||
             !check_matrix(op, "add", add, ldadd, d, size, false) ||
@@ -151,7 +166,7 @@ int jc_linear(uint32_t type, uint32_t act, const void *x, size_t ldx, const void
         const char *op = "linear";
         const bool any = m > 0;
         if (!check_act(op, type, act)) return -1;
-        if (n == 0 || k == 0) return fail("linear: n and k must not be 0");
+        if (!check_sizes(op, m, n, k)) return -1;
         if (!check_matrix(op, "x", x, ldx, k, 2, any) || !check_matrix(op, "w", w, ldw, k, 2, true) ||
             !check_vector(op, "bias", bias, 4, false) || !check_matrix(op, "res", res, ldres, n, 2, false) ||
             !check_matrix(op, "y", y, ldy, n, 2, any) || !check_matrix(op, "z", z, ldz, n, 2, false) ||
@@ -196,7 +211,7 @@ int jc_linear_backward(uint32_t type, uint32_t act, const void *dy, size_t lddy,
         const char *op = "linear_backward";
         const bool any = m > 0;
         if (!check_act(op, type, act)) return -1;
-        if (n == 0 || k == 0) return fail("linear_backward: n and k must not be 0");
+        if (!check_sizes(op, m, n, k)) return -1;
         if (!check_matrix(op, "dy", dy, lddy, n, 2, any) || !check_matrix(op, "x", x, ldx, k, 2, any && dw) ||
             !check_matrix(op, "w", w, ldw, k, 2, any && dx) ||
             !check_matrix(op, "z", z, ldz, n, 2, any && act) ||
@@ -238,7 +253,7 @@ int jc_choice_loss(const float *logits, uint32_t n_logits, const int32_t *offset
             !check_vector(op, "weight", weight, 4, false) || !check_vector(op, "loss", loss, 4, any) ||
             !check_vector(op, "dlogits", dlogits, 4, false))
             return -1;
-        if (n_logits > 0x7FFFFFFFu || requests > 0x7FFFFFFFu)
+        if (n_logits > MAX_SIZE || requests > MAX_SIZE)
             return fail("choice_loss: at most 2^31 - 1 logits and requests");
         jc::LossArgs a;
         a.logits = logits;

@@ -87,9 +87,14 @@ int device_of(const char *op, const at::Tensor &t) {
     return dev;
 }
 
+void check_sizes(const char *op, const at::Tensor &t) {
+    for (const int64_t n : t.sizes())
+        if (n > 0x7FFFFFFFll) fail(std::string(op) + ": at most 2^31 - 1 rows and columns");
+}
+
 uint32_t type_of(const char *op, const at::Tensor &x, bool halves) {
     if (x.dim() != 2) fail(std::string(op) + ": x must be a matrix");
-    if (x.size(0) > 0xFFFFFFFFll || x.size(1) > 0xFFFFFFFFll) fail(std::string(op) + ": x is too large");
+    check_sizes(op, x);
     switch (x.scalar_type()) {
         case at::kHalf: return JC_F16;
         case at::kBFloat16: return JC_BF16;
@@ -222,6 +227,7 @@ PyObject *linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const char *op = "linear";
         const at::Tensor &x = *tensor({op, "x"}, a[0]), &w = *tensor({op, "w"}, a[1]);
         const uint32_t type = type_of(op, x, true);
+        check_sizes(op, w);
         const int dev = device_of(op, x);
         const int64_t m = x.size(0), k = x.size(1), c = w.dim() == 2 ? w.size(0) : 0;
         const at::ScalarType st = x.scalar_type();
@@ -245,6 +251,7 @@ PyObject *linear_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const char *op = "linear_backward";
         const at::Tensor &x = *tensor({op, "x"}, a[1]), &w = *tensor({op, "w"}, a[2]);
         const uint32_t type = type_of(op, x, true), act = act_of(op, a[4]);
+        check_sizes(op, w);
         const int dev = device_of(op, x);
         const int64_t m = x.size(0), k = x.size(1), c = w.dim() == 2 ? w.size(0) : 0;
         const at::ScalarType st = x.scalar_type();

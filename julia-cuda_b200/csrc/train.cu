@@ -142,7 +142,7 @@ constexpr uint32_t NORM_BWD_BLOCKS = 148;
 constexpr uint32_t NORM_BWD_ALONE = 8;
 
 size_t norm_bwd_ws_floats(uint32_t rows, uint32_t d) {
-    return rows > NORM_BWD_ALONE ? (size_t)std::min(rows + 7, NORM_BWD_BLOCKS) * 2 * d : 0;
+    return rows > NORM_BWD_ALONE ? std::min<size_t>((size_t)rows + 7, NORM_BWD_BLOCKS) * 2 * d : 0;
 }
 
 static bool launch_column_sum(const float *ws, uint32_t parts, uint32_t n, uint32_t columns, float *a,

@@ -37,3 +37,30 @@ def test_adamw_refuses_tensors_of_another_device(jc, monkeypatch, other):
     states = {k: [v] for k, v in t.items() if k.startswith("exp")}
     with pytest.raises(jc.JuliaCudaError, match="on the current device"):
         training.AdamW([t["param"]], [t["grad"]], bits=8, copies=[t["copy"]], **states)
+
+
+@pytest.mark.parametrize("rows", [2 ** 31, 2 ** 32 - 1])
+def test_more_rows_than_the_kernels_count(jc, rows):
+    """Rows are walked with 32-bit counters that pass the last row by up to a grid's step."""
+    L, p = jc.lib(), 4096
+    assert L.jc_layer_norm(0, p, 1, p, p, 1e-5, rows, 1, p, 1, None, None) == -1 and "2^31 - 1" in jc.last_error()
+    assert L.jc_layer_norm_backward(0, p, 1, p, 1, p, p, None, 0, rows, 1, p, 1, p, p, p, None) == -1
+    assert "2^31 - 1" in jc.last_error()
+    assert L.jc_layer_norm_ws_floats(rows, 1) >= 148 * 2
+
+    def linear(m, n, k):
+        return L.jc_linear(0, 0, p, k, p, k, None, None, n, p, n, None, n, m, n, k, p, None)
+
+    def backward(m, n, k):
+        return L.jc_linear_backward(0, 0, p, n, p, k, p, k, None, n, m, n, k, p, k, p, k, p, p, None)
+    for call in (linear, backward):
+        for size in ((rows, 16, 16), (16, rows, 16), (16, 16, rows)):
+            assert call(*size) == -1 and "2^31 - 1" in jc.last_error(), (size, jc.last_error())
+
+
+def test_tensors_with_more_rows_than_the_kernels_count(jc):
+    x, v = torch.empty(2 ** 31, 1, dtype=torch.float16, device="meta"), torch.empty(1, device="meta")
+    for call in (lambda: jc.layer_norm(x, v, None, x), lambda: jc.layer_norm_backward(x, x, v, v, x),
+                 lambda: jc.linear(x, x, x), lambda: jc.linear_backward(x, x, x, dx=x)):
+        with pytest.raises(jc.JuliaCudaError, match="2\\^31 - 1"):
+            call()
