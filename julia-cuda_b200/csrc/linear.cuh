@@ -155,7 +155,7 @@ struct DzParams {
     float *part;  // [gridDim.y][n] column sums, or nullptr
 };
 
-constexpr uint32_t DZ_ROWS = 64;  // rows a block covers (few rows: twice that)
+constexpr uint32_t DZ_ROWS = 64;  // rows a block covers (few rows: twice that; past 65535 blocks: more)
 
 // dz = dy act'(z) and its sums over each block's rows: a thread walks V columns down every eighth
 // row, the block's eight warps meet in shared memory in order. Bound by memory: 12288 x 2048 f16, two

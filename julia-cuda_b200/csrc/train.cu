@@ -495,8 +495,9 @@ static LinearBwdPlan plan_linear_bwd(const void *x, size_t ldx, const void *w, s
                                      uint32_t k) {
     LinearBwdPlan p{};
     auto up = [](size_t v) { return round_up(v, 256); };
-    // Rows a block of the dz kernel takes: few rows go to one, which then writes dbias itself.
-    p.dz_rows = m <= 2 * DZ_ROWS ? 2 * DZ_ROWS : DZ_ROWS;
+    // Rows a block of the dz kernel takes: few rows go to one, which then writes dbias itself; of very many
+    // each takes more, as a grid has 65535 blocks along y.
+    p.dz_rows = m <= 2 * DZ_ROWS ? 2 * DZ_ROWS : std::max(DZ_ROWS, (m + 65534) / 65535);
     p.dz_parts = (m + p.dz_rows - 1) / p.dz_rows;
     p.lddz = (n + 7) / 8 * 8;
     p.part_at = up((size_t)m * p.lddz * 2);
@@ -573,10 +574,6 @@ bool launch_linear_bwd(const LinearBwdArgs &a, cudaStream_t s) {
             const bool vec = a.n % 8 == 0 && aligned16(a.dy, a.lddy, 2) && (!a.act || aligned16(a.z, a.ldz, 2));
             const uint32_t cols = vec ? 256 : 32;
             const dim3 grid((a.n + cols - 1) / cols, plan.dz_parts);
-            if (grid.y > 65535) {
-                set_error("linear_backward: too many rows");
-                return false;
-            }
             if (!with_act(a.act, [&](auto act) {
                     constexpr uint32_t ACT = decltype(act)::value;
                     return vec ? launch_ex(linear_dz_kernel<T, ACT, 8>, grid, dim3(256), 0, s, true, "dz", p)

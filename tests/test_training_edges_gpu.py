@@ -195,3 +195,25 @@ def test_layer_norm_rows_after_the_tensors_first(jc, d, t):
     assert ((dx.double() - want).abs() <= u * want.abs() + 2 * tol + 2.0 ** -25).all()
     assert ((dg.double() - (dy * xh).sum(0)).abs() <= f32 * (dy.abs() * mag).sum(0)).all()
     assert ((db.double() - dy.sum(0)).abs() <= f32 * dy.abs().sum(0)).all()
+
+
+def test_linear_backward_of_millions_of_rows(jc):
+    """More rows than 65535 blocks of 64. Sums of m values of variance 1 stay below 6 sqrt(m) on their way;
+    the longest chain of additions is an eighth of 65535 partial sums (dbias) and the 16-row steps of one of
+    32 splits (dw), 8300 either way, each addition within 2^-23 of what it adds to."""
+    g = gen(6)
+    m, n, k = 65535 * 64 + 77, 9, 8
+    t = torch.bfloat16
+    dy, x, w = normal(g, m, n, dtype=t), normal(g, m, k, dtype=t), normal(g, n, k, dtype=t)
+    dx, dw, db = torch.full_like(x, math.nan), torch.full_like(w, math.nan), torch.full((n,), math.nan, device="cuda")
+    jc.linear_backward(dy, x, w, dx=dx, dw=dw, dbias=db)
+    assert jc.device_error() == 0
+    u, d64, x64 = 2.0 ** -8, dy.double(), x.double()
+    off = 8300 * 2.0 ** -23 * 6 * math.sqrt(m)
+    assert ((db.double() - d64.sum(0)).abs() <= off).all()
+    want = d64.t() @ x64
+    assert ((dw.double() - want).abs() <= u * want.abs() + off).all()
+    for a in (0, m // 2, m - 1000):
+        d = d64[a:a + 1000]
+        want = d @ w.double()
+        assert ((dx[a:a + 1000].double() - want).abs() <= u * want.abs() + 32 * 2.0 ** -24 * (d.abs() @ w.double().abs())).all()
