@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(32 * LR_WARPS) linear_rows_kernel(const Linear
 // few columns
 
 constexpr int LTHIN_MAX = 8;
+constexpr uint32_t LTHIN_MAX_K = 65535 * 256;  // the backward kernel's grid has 256 of k along y
 
 // Eight of a row's elements for a lane, starting at c0 + 8 lane where rows are on 16-byte boundaries,
 // else c0 + lane, c0 + lane + 32, ...; places past the row are 0.

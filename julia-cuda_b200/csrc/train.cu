@@ -485,7 +485,7 @@ static GradPlan plan_grads(uint32_t m, uint32_t n, uint32_t k) {
 // partial products, the copies of w and x where TMA cannot load them, each from a 256-byte boundary.
 struct LinearBwdPlan {
     uint32_t dz_rows, dz_parts, splits;
-    uint32_t thin_blocks;  // n <= LTHIN_MAX: blocks along the rows, each with its sums; nothing else used
+    uint32_t thin_blocks;  // few columns: blocks along the rows, each with its sums; nothing else used
     size_t lddz, part_at, ws_at, bytes;
     Pad w, x;
     Tiling tiling;
@@ -502,7 +502,7 @@ static LinearBwdPlan plan_linear_bwd(const void *x, size_t ldx, const void *w, s
     p.lddz = (n + 7) / 8 * 8;
     p.part_at = up((size_t)m * p.lddz * 2);
     p.ws_at = p.part_at + up((size_t)p.dz_parts * n * 4);
-    if (n <= LTHIN_MAX) {
+    if (n <= LTHIN_MAX && k <= LTHIN_MAX_K) {
         p.thin_blocks = std::max(1u, std::min((m + 31) / 32, 148u * 2));
         p.bytes = up((size_t)p.thin_blocks * ((size_t)n * k + n) * 4);
         return p;
@@ -532,10 +532,6 @@ static bool launch_linear_thin_bwd(const LinearBwdArgs &a, uint32_t blocks, cuda
             const bool vec = a.k % 8 == 0 && (!a.dw || aligned16(a.x, a.ldx, 2)) &&
                              (!a.dx || (aligned16(a.w, a.ldw, 2) && aligned16(a.dx, a.lddx, 2)));
             const dim3 grid(blocks, (a.k + 255) / 256);
-            if (grid.y > 65535) {
-                set_error("linear_backward: k is too large");
-                return false;
-            }
             if (!with_act(a.act, [&](auto act) {
                     return with_thin(a.n, [&](auto n) {
                         constexpr uint32_t ACT = decltype(act)::value;

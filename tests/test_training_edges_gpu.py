@@ -217,3 +217,19 @@ def test_linear_backward_of_millions_of_rows(jc):
         d = d64[a:a + 1000]
         want = d @ w.double()
         assert ((dx[a:a + 1000].double() - want).abs() <= u * want.abs() + 32 * 2.0 ** -24 * (d.abs() @ w.double().abs())).all()
+
+
+@pytest.mark.parametrize("rows,n", [(3, 1), (0, 8)])
+def test_linear_backward_of_few_columns_and_a_long_contraction(jc, rows, n):
+    """More contracted elements than the grid of the kernel for few columns has: each gradient within two
+    roundings of the type (dz is exact here), dw 0 where there are no rows."""
+    g = gen(n)
+    k, t = 65535 * 256 + 8, torch.float16
+    dy, x, w = normal(g, rows, n, dtype=t), normal(g, rows, k, dtype=t), normal(g, n, k, dtype=t)
+    dx, dw, db = torch.full_like(x, math.nan), torch.full_like(w, math.nan), torch.full((n,), math.nan, device="cuda")
+    jc.linear_backward(dy, x, w, dx=dx, dw=dw, dbias=db)
+    assert jc.device_error() == 0
+    tol = lambda a, b: 2.0 ** -10 * (a.double().abs() @ b.double().abs()) + 2.0 ** -25  # noqa: E731
+    assert ((dx.double() - dy.double() @ w.double()).abs() <= tol(dy, w)).all()
+    assert ((dw.double() - dy.double().t() @ x.double()).abs() <= tol(dy.t(), x)).all()
+    assert ((db.double() - dy.double().sum(0)).abs() <= 2.0 ** -22 * dy.double().abs().sum(0)).all()
