@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import argparse
 import json
+import math
 import sys
 
 import numpy as np
@@ -61,8 +62,13 @@ class ScorerTrainer:
                        for o, n in zip(self._at, shapes)]
         matrix = [len(n) == 2 for n in shapes]
         self.copies = [p.to(dtype) if m else None for p, m in zip(self.params, matrix)]
-        self.grads = [torch.zeros(n, dtype=dtype if m else torch.float32, device="cuda")
-                      for n, m in zip(shapes, matrix)]
+        # One buffer a type, so that a step looks two tensors over for infinities.
+        sizes = [int(np.prod(n)) for n in shapes]
+        flat = {m: torch.zeros(sum(k for k, o in zip(sizes, matrix) if o == m), device="cuda",
+                               dtype=dtype if m else torch.float32) for m in (True, False)}
+        cut = {m: iter(flat[m].split([k for k, o in zip(sizes, matrix) if o == m])) for m in flat}
+        self.grads = [next(cut[m]).view(n) for n, m in zip(shapes, matrix)]
+        self._flat_grads = list(flat.values())
         self.opt = AdamW(self.params, self.grads, bits=bits, copies=self.copies,
                          weight_decay=[weight_decay if m else 0.0 for m in matrix])
 
@@ -81,7 +87,8 @@ class ScorerTrainer:
     def step(self, x, offsets, gold, weight=None):
         """One training step on features x (features()) of requests whose right markers are `gold` (int32,
         counted from the request's first; below 0: none). Returns (each request's loss, the logits before
-        the step), on the device."""
+        the step), on the device. Where a gradient is past what its type holds, nothing is updated and
+        loss_scale is halved for the next step."""
         x = x.to(self.dtype)
         logits, (x, xn, stats, z, h) = self.forward(x)
         loss, dlogits = torch.empty(gold.numel(), device=x.device), torch.empty_like(logits)
@@ -96,6 +103,13 @@ class ScorerTrainer:
         linear_backward(dy, h, w2, dx=dh, dw=dw2, dbias=db2)
         linear_backward(dh, xn, w1, z=z, act="gelu", dx=dxn, dw=dw1, dbias=db1)
         layer_norm_backward(dxn, x, self.params[0], stats, dx, dgamma, dbeta)
+        # The largest magnitudes: infinite or NaN where any gradient is.
+        matrices, vectors = (torch.linalg.vector_norm(g, math.inf) for g in self._flat_grads)
+        if not math.isfinite(matrices + vectors):
+            if self.loss_scale < 2.0 ** -10:
+                raise JuliaCudaError("step: the gradients are not finite at any loss scale")
+            self.loss_scale /= 2
+            return loss, logits
         self.t += 1
         self.opt.step(self.t, lr=self.lr, grad_scale=1.0 / (self.loss_scale * counted))
         return loss, logits

@@ -1,0 +1,50 @@
+"""Fine-tuning the scorer where things go wrong: gradients past their type, nothing to train on."""
+import importlib
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def setup(jc):
+    """The module, a model, and features of requests as the engine would give them."""
+    ft = importlib.import_module("julia-cuda_b200.finetune")
+    cfg = jc.default_config(d_model=128, inter=128, n_layers=3, vocab=500, head_ff=128, scorer_hidden=64,
+                            max_positions=128)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(240, cfg.d_model, generator=g, device="cuda").half()
+    off = torch.arange(0, 241, 4, dtype=torch.int32, device="cuda")
+    gold = torch.randint(0, 4, (60,), generator=g, device="cuda").int()
+    return ft, cfg, jc.init_random(cfg, 5), x, off, gold
+
+
+def test_gradients_past_f16_skip_the_step(setup):
+    """A loss scale that overflows f16 leaves the scorer and the optimizer as they were, and is halved until
+    steps go through."""
+    ft, cfg, raw, x, off, gold = setup
+    tr = ft.ScorerTrainer(cfg, raw, loss_scale=2.0 ** 19)
+    before = [p.clone() for p in tr.params]
+    tr.step(x, off, gold)
+    assert tr.t == 0 and tr.loss_scale == 2.0 ** 18
+    assert all(torch.equal(a, b) for a, b in zip(before, tr.params))
+    assert all((s == 0).all() for s in tr.opt.exp_avg)
+    for _ in range(20):
+        tr.step(x, off, gold)
+    assert tr.t > 0 and all(p.isfinite().all() for p in tr.params)
+    assert not torch.equal(before[2], tr.params[2])
+
+
+def test_features_that_are_not_finite_end_in_an_error(jc, setup):
+    ft, cfg, raw, x, off, gold = setup
+    tr = ft.ScorerTrainer(cfg, raw)
+    before = [p.clone() for p in tr.params]
+    bad = x.clone()
+    bad[7, 5] = math.nan
+    with pytest.raises(jc.JuliaCudaError, match="not finite"):
+        for _ in range(60):
+            tr.step(bad, off, gold)
+    assert tr.t == 0 and all(torch.equal(a, b) for a, b in zip(before, tr.params))
