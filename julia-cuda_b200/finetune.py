@@ -142,6 +142,8 @@ def train(engine: Engine, raw: np.ndarray, seqs, gold, *, epochs: int = 10, batc
     """Trains the scorer on the requests and returns the new raw model. kw: ScorerTrainer's."""
     if len(seqs) != len(gold) or any(g >= len(s[1]) for s, g in zip(seqs, gold)):
         raise JuliaCudaError("train: one right marker for each request, among its markers")
+    if not seqs:
+        raise JuliaCudaError("train: no requests")
     x, offsets = features(engine, seqs)
     at = offsets.tolist()
     trainer = ScorerTrainer(engine.cfg, raw, **kw)

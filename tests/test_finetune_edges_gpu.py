@@ -48,3 +48,20 @@ def test_features_that_are_not_finite_end_in_an_error(jc, setup):
         for _ in range(60):
             tr.step(bad, off, gold)
     assert tr.t == 0 and all(torch.equal(a, b) for a, b in zip(before, tr.params))
+
+
+def test_nothing_to_train_on(jc, setup, tmp_path, capsys):
+    """No requests is an error of the call and of the command; requests without markers train nothing."""
+    ft, cfg, raw = setup[:3]
+    eng = jc.Engine.load_raw(cfg, raw, max_length=64)
+    with pytest.raises(jc.JuliaCudaError, match="no requests"):
+        ft.train(eng, raw, [], [], epochs=1)
+    new = ft.train(eng, raw, [(list(range(9)), [], 0)] * 3, [-1] * 3, epochs=2, weight_decay=0.0)
+    assert np.array_equal(new, raw)
+    eng.close()
+    (tmp_path / "model").mkdir()
+    (tmp_path / "out").mkdir()
+    jc.save_checkpoint(str(tmp_path / "model"), cfg, raw)
+    (tmp_path / "empty.jsonl").write_text("\n")
+    args = [str(tmp_path / n) for n in ("model", "empty.jsonl", "empty.jsonl", "out")]
+    assert ft.main(args) == 1 and "no requests" in capsys.readouterr().err
