@@ -25,18 +25,35 @@ from . import (AdamW, Engine, JuliaCudaError, choice_loss, layer_norm, layer_nor
 QTYPES = {"choice": 0, "score": 1, "noul": 2}
 
 
+def _checked(engine: Engine, seqs):
+    """The requests as arrays. Like julia_cuda_run, all are looked over before any is queued: the device
+    calls follow the token ids and markers that they are given."""
+    out = []
+    for i, (ids, markers, qtype) in enumerate(seqs):
+        ids, markers, qtype = np.asarray(ids, np.int64), np.asarray(markers, np.int64), int(qtype)
+        past = ids[(ids < 0) | (ids >= engine.cfg.vocab)]
+        why = ("no tokens" if not ids.size
+               else f"token id {past[0]} is past the vocabulary" if past.size
+               else "a marker is past the sequence" if ((markers < 0) | (markers >= ids.size)).any()
+               else f"no question type {qtype}" if not 0 <= qtype < engine.cfg.n_qtypes else "")
+        if why:
+            raise JuliaCudaError(f"features: sequence {i}: {why}")
+        out.append((ids, markers, qtype))
+    return out
+
+
 def features(engine: Engine, seqs):
     """The scorer's inputs, the head's outputs at the marker rows: ([markers, D] f16, offsets int32
     [requests + 1]) of requests (ids, markers, qtype), on the engine's device."""
     rows, at = [], [0]
     layers = engine.cfg.n_head_layers + 1
-    for ids, markers, qtype in seqs:
-        ids = torch.as_tensor(np.asarray(ids, np.int64).astype(np.int32), device="cuda")
-        mk = torch.as_tensor(np.asarray(markers, np.int64).astype(np.int32), device="cuda")
+    for ids, markers, qtype in _checked(engine, seqs):
+        ids = torch.as_tensor(ids.astype(np.int32), device="cuda")
+        mk = torch.as_tensor(markers.astype(np.int32), device="cuda")
         trace = torch.empty(layers, ids.numel(), engine.cfg.d_model, dtype=torch.float16,
                             device="cuda")
         logits = torch.empty(max(mk.numel(), 1), device="cuda")
-        engine.forward_trace(ids, mk, int(qtype), logits, head_trace=trace)
+        engine.forward_trace(ids, mk, qtype, logits, head_trace=trace)
         rows.append(trace[-1][mk.long()])
         at.append(at[-1] + mk.numel())
     if engine.device_error():
