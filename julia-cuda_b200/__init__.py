@@ -453,6 +453,7 @@ class Engine:
     def __init__(self, handle, cfg: Config):
         self._h = handle
         self.cfg = cfg
+        self.head_length = 0  # set_head_length's
 
     @classmethod
     def load_raw(cls, cfg: Config, raw: np.ndarray, max_length: int = 1024, device: int = 0):
@@ -603,6 +604,7 @@ class Engine:
         """The head runs on the first `rows` rows of later requests (0: all rows)."""
         if lib().julia_cuda_set_head_length(self._h, rows) != 0:
             raise JuliaCudaError("set_head_length: no engine")
+        self.head_length = rows
 
     def launches_per_forward(self, n: int, n_markers: int, layer_fused=False) -> int:
         return lib().julia_cuda_launches_per_forward(self._h, n, n_markers, int(layer_fused))

@@ -25,6 +25,11 @@ from . import (AdamW, Engine, JuliaCudaError, choice_loss, layer_norm, layer_nor
 QTYPES = {"choice": 0, "score": 1, "noul": 2}
 
 
+def _head_rows(engine: Engine, n: int) -> int:
+    """How many of a request's n rows the head runs on (Engine.set_head_length)."""
+    return min(engine.head_length or n, n)
+
+
 def _checked(engine: Engine, seqs):
     """The requests as arrays. Like julia_cuda_run, all are looked over before any is queued: the device
     calls follow the token ids and markers that they are given."""
@@ -32,10 +37,16 @@ def _checked(engine: Engine, seqs):
     for i, (ids, markers, qtype) in enumerate(seqs):
         ids, markers, qtype = np.asarray(ids, np.int64), np.asarray(markers, np.int64), int(qtype)
         past = ids[(ids < 0) | (ids >= engine.cfg.vocab)]
-        why = ("no tokens" if not ids.size
-               else f"token id {past[0]} is past the vocabulary" if past.size
-               else "a marker is past the sequence" if ((markers < 0) | (markers >= ids.size)).any()
-               else f"no question type {qtype}" if not 0 <= qtype < engine.cfg.n_qtypes else "")
+        head = _head_rows(engine, ids.size)
+        why = ""
+        if not ids.size:
+            why = "no tokens"
+        elif past.size:
+            why = f"token id {past[0]} is past the vocabulary"
+        elif ((markers < 0) | (markers >= head)).any():
+            why = f"a marker is past the {'sequence' if head == ids.size else 'head rows'}"
+        elif not 0 <= qtype < engine.cfg.n_qtypes:
+            why = f"no question type {qtype}"
         if why:
             raise JuliaCudaError(f"features: sequence {i}: {why}")
         out.append((ids, markers, qtype))
@@ -50,8 +61,8 @@ def features(engine: Engine, seqs):
     for ids, markers, qtype in _checked(engine, seqs):
         ids = torch.as_tensor(ids.astype(np.int32), device="cuda")
         mk = torch.as_tensor(markers.astype(np.int32), device="cuda")
-        trace = torch.empty(layers, ids.numel(), engine.cfg.d_model, dtype=torch.float16,
-                            device="cuda")
+        trace = torch.empty(layers, _head_rows(engine, ids.numel()), engine.cfg.d_model,
+                            dtype=torch.float16, device="cuda")
         logits = torch.empty(max(mk.numel(), 1), device="cuda")
         engine.forward_trace(ids, mk, qtype, logits, head_trace=trace)
         rows.append(trace[-1][mk.long()])

@@ -65,3 +65,24 @@ def test_nothing_to_train_on(jc, setup, tmp_path, capsys):
     (tmp_path / "empty.jsonl").write_text("\n")
     args = [str(tmp_path / n) for n in ("model", "empty.jsonl", "empty.jsonl", "out")]
     assert ft.main(args) == 1 and "no requests" in capsys.readouterr().err
+
+
+def test_features_under_a_head_length(jc, setup):
+    """An engine whose head runs on the first rows of a request only: the scorer over its features gives the
+    engine's own logits, and markers past those rows are refused."""
+    ft, cfg, raw = setup[:3]
+    eng = jc.Engine.load_raw(cfg, raw, max_length=128)
+    rng = np.random.default_rng(4)
+    seqs = [(rng.integers(0, 500, n).tolist(), sorted(rng.choice(min(n, 20), 4, replace=False).tolist()), 0)
+            for n in (90, 12, 33, 20, 64)]
+    eng.set_head_length(20)
+    x, off = ft.features(eng, seqs)
+    logits, _ = ft.ScorerTrainer(cfg, raw).forward(x)
+    want = torch.from_numpy(np.concatenate(eng.run(seqs)[0])).cuda()
+    # f16 rounds the scorer's two layers and the logits once each, and the engine lin1's folded weights.
+    assert (logits - want).abs().max() < 8 * 2.0 ** -11 * max(1.0, float(want.abs().max()))
+    with pytest.raises(jc.JuliaCudaError, match="sequence 1: a marker is past the head rows"):
+        ft.features(eng, [seqs[0], (list(range(40)), [20], 0)])
+    eng.set_head_length(0)
+    assert ft.features(eng, [(list(range(40)), [20], 0)])[0].shape == (1, cfg.d_model)
+    eng.close()
