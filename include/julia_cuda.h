@@ -449,7 +449,8 @@ size_t jc_linear_backward_ws_bytes(const void *x, size_t ldx, const void *w, siz
  * exp(logit)) - logit of the right marker), dlogits (may be NULL) its gradient, weight[r]
  * (softmax - one-hot); weight NULL: 1. A request with no right marker, weight 0, no logits or only
  * logits of -infinity gives 0 and 0. Offsets or a right marker out of range record device error 6
- * (JC_DEV_BAD_INDEX, read by jc_device_error), give loss 0 and leave the request's dlogits alone. */
+ * (JC_DEV_BAD_INDEX, read by jc_device_error), give loss 0 and leave the request's dlogits alone, as
+ * are those of logits before the first request's and after the last one's. */
 int jc_choice_loss(const float *logits, uint32_t n_logits, const int32_t *offsets,
                    const int32_t *gold, const float *weight, uint32_t requests, float *loss,
                    float *dlogits, void *stream);

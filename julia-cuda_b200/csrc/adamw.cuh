@@ -146,9 +146,10 @@ struct AdamwRaw {
 // front of every chunk left the memory idle for a third of the time. With 8-bit states, whose elements
 // are half the bytes for more arithmetic, the next chunk's data is requested before the current one is
 // worked on too (485 -> 470 us for 160 million elements; with 32-bit states the bus is full without).
-// Bound by memory: 160 million elements with bf16 gradients and copies, 32-bit states 701 us, 6.4 TB/s, as
-// fast as a copy; 8-bit states 505 us from three models in turn, 5.1 TB/s: a third of the issue slots is
-// taken, the rest waits for loads that 24 warps a SM keep too few of in flight.
+// Bound by memory: 160 million elements with bf16 gradients and copies, 32-bit states 686 us, 6.5 TB/s, as
+// fast as a copy; 8-bit states 492 to 497 us from three models in turn, 5.2 TB/s: half of the issue slots
+// are taken, the rest waits for loads that 24 warps a SM (80 registers, 28 bytes spilled) keep too few of
+// in flight.
 constexpr uint32_t ADAMW_WORDS = sizeof(AdamwTensor) / 4;
 
 template <int BITS>

@@ -17,8 +17,9 @@ namespace jc {
 // The module-wide error word: 0, or the first JC_DEV_* code a kernel recorded. It serves the
 // per-kernel entry points (jc_gemm, jc_attention, ...), which have no engine; an engine passes
 // its own word in every launch's parameters, so two engines on one GPU (or an engine beside bare
-// jc_* calls) never see or clear each other's errors. (All kernels live in one translation unit,
-// kernels.cu, so this is the only definition.)
+// jc_* calls) never see or clear each other's errors. Each translation unit that includes this file
+// has a definition of its own: kernels.cu's is the one that is read, and the kernels of other units
+// are given its address (module_error_word) and bind that.
 __device__ unsigned int g_dev_error = 0;
 
 // The word the running CTA records errors into. Every kernel that can record an error binds it

@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(256) linear_pad_kernel(const PadParams p) {
 // The backward pass's last kernel: the first `join_blocks` blocks write c [m][n] = the sum of `splits`
 // partial products in ws, in their order, V columns a thread; the others dbias = the sums of `parts`
 // rows of column sums, 32 columns a block, eight threads a column. The partial sums come from L2 (three of
-// 2048 x 768: 5 us).
+// 2048 x 768: 6.8 us, 8.4 from cold caches).
 struct LinearFinishParams {
     const float *ws;
     uint32_t splits, m, n, join_blocks;
@@ -159,7 +159,7 @@ constexpr uint32_t DZ_ROWS = 64;  // rows a block covers (few rows: twice that; 
 
 // dz = dy act'(z) and its sums over each block's rows: a thread walks V columns down every eighth
 // row, the block's eight warps meet in shared memory in order. Bound by memory: 12288 x 2048 f16, two
-// reads and a write, 19 us.
+// reads and a write, 25 us.
 template <class T, uint32_t ACT, int V>
 __global__ void __launch_bounds__(256) linear_dz_kernel(const DzParams p) {
     __shared__ float s[8][32 * V];

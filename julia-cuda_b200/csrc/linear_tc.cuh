@@ -22,7 +22,7 @@
 // measured burst rate; a library product of that shape 28.4), 30.2 with bias and residual; from memory
 // 38. Its 144 tiles are two rounds of 72 pairs; what is left is the clock under load, the first tiles'
 // loads and the last epilogue. Short contractions are bound by the epilogue: 12288 x 768 x 2048 with
-// GELU and z 65 us.
+// GELU and z 52 us in short bursts, where its operations would take 24.
 #pragma once
 #include <type_traits>
 

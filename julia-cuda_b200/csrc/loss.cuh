@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) loss_group_kernel(const Los
 // to LOSS_REGS of them in registers; the gradients go out through the warp's part of shared memory in
 // whole lines. Warps stay and walk the requests, the next ones' spans requested ahead. A warp whose
 // gradients do not fit (a long request among short ones), or whose requests lie out of order, takes them
-// one by one instead. A million requests of 6.5 logits: 22.7 us, 3.0 TB/s; bound by the latency of the
+// one by one instead. A million requests of 6.5 logits: 22.2 us, 3.1 TB/s; bound by the latency of the
 // reads one behind the other (spans, logits), of which 32 warps a SM hide half.
 constexpr int LOSS_WARPS = 4, LOSS_SMEM = 768, LOSS_REGS = 16;
 

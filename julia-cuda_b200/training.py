@@ -80,7 +80,8 @@ def linear_backward(dy, x, w, *, z=None, act: str = "none", dx=None, dw=None, db
 def choice_loss(logits, offsets, gold, loss, dlogits=None, weight=None, stream=None) -> None:
     """Each request's loss over its own markers and its gradient (jc_choice_loss): logits f32,
     offsets int32 [requests + 1], gold int32 [requests] (the right marker of each request, below 0:
-    none), weight f32 [requests]; writes loss [requests] and dlogits (as logits)."""
+    none), weight f32 [requests]; writes loss [requests] and dlogits (as logits; those of logits that no
+    request has are left alone)."""
     _b.choice_loss(logits, offsets, gold, loss, dlogits, weight, stream)
 
 
